@@ -1,5 +1,5 @@
 /*
- * mpserve_amd — MI355X (gfx950) FP8 + Huffman-sidecar weight path, C ABI.
+ * mpserve_amd — MI355X (gfx950) FP8 + Huffman-sidecar weight path and MXFP4 operators, C ABI.
  *
  * Plain pointers and sizes only. Every pointer named "device" is HIP device
  * memory on the current device; host pointers are named so. All entry points
@@ -301,6 +301,88 @@ int mps_fp8_sidecar_free(mps_fp8_sidecar *sc);
  * flags of decodes on any stream of the device accumulate in it. It is a
  * module global of the library (no allocation). Synchronises `stream` first. */
 int mps_fp8_read_status(int device, void *stream, uint32_t *status_out);
+
+/* ---------------------------------------------------------------- MXFP4 and experts
+ * No counterpart in the reference, whose 4-bit weights are AWQ int4 ones. All
+ * calls are asynchronous on `stream`, allocate nothing, and can be captured
+ * into a graph. Workspaces are the caller's device memory, 16-byte aligned,
+ * and are free again when the call's work on `stream` has ended. */
+
+/* Element types. */
+#define MPS_TYPE_BF16 0
+#define MPS_TYPE_F16 1
+#define MPS_TYPE_F32 2
+#define MPS_TYPE_MXFP4 3 /* operands of mps_mxfp4_multiply only */
+
+#define MPS_MAX_EXPERTS 1024
+
+/* MXFP4 of x[rows, k] (`row_stride` elements from row to row): codes
+ * [rows, 16 * ceil(k / 32)], two codes a byte, the earlier element in the low
+ * half, a row's last block filled up with zero codes; scales
+ * [rows, ceil(k / 32)], the byte s of 2^(s - 127). The scale is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; a code is the nearest value,
+ * ties to the even code, magnitudes above 6 to 6. A block with an infinity or
+ * a NaN gets scale 255 (it reads back as NaN) and zero codes. */
+int mps_mxfp4_quantize(const void *x, int32_t type, int64_t rows, int64_t k, int64_t row_stride, uint8_t *codes,
+                       uint8_t *scales, void *stream);
+/* The values [rows, k] of MXFP4 codes, rounded to `type` (exact in BF16 and
+ * FP32 except where 6 * 2^127 overflows). */
+int mps_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t k, void *out, int32_t type,
+                         void *stream);
+
+/* out[rows, n] = x[rows, k] times the transpose of w[n, k], plus bias[n], with
+ * w in MXFP4 and x in BF16, FP16 or MXFP4; FP32 sums, one rounding to
+ * out_type. With experts > 0, w is [experts, n, k] and bias [experts, n]:
+ * rows offsets[e] .. offsets[e + 1] are multiplied by expert e's weight and
+ * rows from offsets[experts] on are set to zero. With `gather`, row j of the
+ * product is made of x's row order[j] / top instead of its row j. The offsets
+ * and the order are mps_expert_sort's (or hold its promises: offsets rise
+ * from 0 to at most rows, the order's entries are below the rows of x times
+ * top). Codes are 16-byte aligned; those past column k in a row's last block
+ * are zero, as mps_mxfp4_quantize writes them. */
+typedef struct mps_mxfp4_product {
+  const void *x;           /* [rows, k] with x_stride, or MXFP4 codes */
+  const uint8_t *x_scales; /* MXFP4 only */
+  int64_t x_stride;        /* elements from row to row; unused for MXFP4 */
+  const uint8_t *w;
+  const uint8_t *w_scales;
+  const void *bias; /* may be NULL */
+  void *out;
+  const int32_t *offsets; /* [experts + 1] */
+  const int32_t *order;   /* [rows], gather only */
+  int64_t rows, n, k;
+  int64_t experts; /* 0: one weight for all rows */
+  int64_t top;
+  int32_t gather;
+  int32_t x_type, bias_type, out_type;
+} mps_mxfp4_product;
+int mps_mxfp4_product_workspace(const mps_mxfp4_product *product, int64_t *bytes);
+int mps_mxfp4_multiply(const mps_mxfp4_product *product, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Sort the pairs of tokens and experts: ids[tokens, top] (int32, or int64 with
+ * ids_64) names each pair's expert; a pair whose id is not in [0, experts) has
+ * none. Pairs are ordered by expert, those of an expert as they come, those
+ * of none last: order[j] is the pair (token * top + slot) at place j,
+ * positions[pair] its place, -1 for a pair of no expert, and
+ * offsets[0 .. experts] where each expert's pairs begin and the last one's end. */
+int mps_expert_sort_workspace(int64_t tokens, int64_t top, int64_t experts, int64_t *bytes);
+int mps_expert_sort(const void *ids, int32_t ids_64, int64_t tokens, int64_t top, int64_t experts, int32_t *order,
+                    int32_t *positions, int32_t *offsets, void *workspace, int64_t workspace_bytes, void *stream);
+/* rows[tokens * top, width]: row j is x's row order[j] / top; rows from
+ * offsets[experts] on are zero. */
+int mps_expert_gather(const void *x, int32_t type, int64_t tokens, int64_t top, int64_t experts, int64_t width,
+                      const int32_t *order, const int32_t *offsets, void *rows, void *stream);
+/* out[tokens, width]: row t is the sum over its pairs' places p of
+ * weights[pair] * y[p] (weights NULL: of y[p]), in FP32 and in the pairs'
+ * order, without the pairs of no expert. Also the gradient of the gather. */
+int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t weights_type, int64_t tokens,
+                       int64_t top, int64_t width, const int32_t *positions, void *out, void *stream);
+/* Gradients of mps_expert_combine: dy[j] = weights[pair] * dout[token] and
+ * dweights[pair] = <y[j], dout[token]> for the pair at place j; zero for the
+ * pairs of no expert. */
+int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const void *weights, int32_t weights_type,
+                            int64_t tokens, int64_t top, int64_t experts, int64_t width, const int32_t *order,
+                            const int32_t *offsets, void *dy, void *dweights, void *stream);
 
 #ifdef __cplusplus
 }

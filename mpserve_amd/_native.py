@@ -76,6 +76,22 @@ class MpsAwqEncodeIn(ctypes.Structure):
     ]
 
 
+#: MPS_TYPE_* by torch dtype name; MXFP4 is an operand type of mps_mxfp4_multiply only
+MPS_TYPE_BF16, MPS_TYPE_F16, MPS_TYPE_F32, MPS_TYPE_MXFP4 = 0, 1, 2, 3
+MPS_MAX_EXPERTS = 1024
+
+
+class MpsMxfp4Product(ctypes.Structure):
+    """mps_mxfp4_product: operands of a product with MXFP4 weights, device pointers."""
+
+    _fields_ = [
+        ("x", _p), ("x_scales", _p), ("x_stride", _i64), ("w", _p), ("w_scales", _p), ("bias", _p), ("out", _p),
+        ("offsets", _p), ("order", _p), ("rows", _i64), ("n", _i64), ("k", _i64), ("experts", _i64), ("top", _i64),
+        ("gather", ctypes.c_int32), ("x_type", ctypes.c_int32), ("bias_type", ctypes.c_int32),
+        ("out_type", ctypes.c_int32),
+    ]
+
+
 #: mps_encode_alloc: (ctx, slot, bytes) -> device pointer, or None for no memory
 ENCODE_ALLOC = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, _i64)
 
@@ -121,6 +137,20 @@ def lib():
     L.mps_awq_plan_info.argtypes = [_p, ctypes.POINTER(_i64)]
     L.mps_awq_plan_read_status.argtypes = [_p, _p, ctypes.POINTER(ctypes.c_uint32)]
     L.mps_awq_plan_destroy.argtypes = [_p]
+    i32 = ctypes.c_int32
+    L.mps_mxfp4_quantize.argtypes = [_p, i32, _i64, _i64, _i64, _p, _p, _p]
+    L.mps_mxfp4_dequantize.argtypes = [_p, _p, _i64, _i64, _p, i32, _p]
+    L.mps_mxfp4_product_workspace.argtypes = [ctypes.POINTER(MpsMxfp4Product), ctypes.POINTER(_i64)]
+    L.mps_mxfp4_multiply.argtypes = [ctypes.POINTER(MpsMxfp4Product), _p, _i64, _p]
+    L.mps_expert_sort_workspace.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
+    L.mps_expert_sort.argtypes = [_p, i32, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]
+    L.mps_expert_gather.argtypes = [_p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p]
+    L.mps_expert_combine.argtypes = [_p, i32, _p, i32, _i64, _i64, _i64, _p, _p, _p]
+    L.mps_expert_combine_grad.argtypes = [_p, _p, i32, _p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p]
+    for name in ("mps_mxfp4_quantize", "mps_mxfp4_dequantize", "mps_mxfp4_product_workspace", "mps_mxfp4_multiply",
+                 "mps_expert_sort_workspace", "mps_expert_sort", "mps_expert_gather", "mps_expert_combine",
+                 "mps_expert_combine_grad"):
+        getattr(L, name).restype = ctypes.c_int
     for name in ("mps_clock_rate_khz", "mps_fp8_decode", "mps_fp8_plan_create", "mps_fp8_plan_decode",
                  "mps_fp8_plan_decode_into", "mps_fp8_plan_info", "mps_fp8_plan_read_status",
                  "mps_fp8_plan_destroy", "mps_fp8_read_status", "mps_fp8_decode_batch_noalloc", "mps_stream_capture_id",

@@ -24,12 +24,13 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmpserve_amd.so")
 ARCH = os.environ.get("MPS_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = ["fp8_decode.hip", "fp8_decode_flat.hip", "fp8_encode.hip", "awq_decode.hip",
+SOURCES = ["mxfp4.hip", "mxfp4_product.hip", "experts.hip",
+           "fp8_decode.hip", "fp8_decode_flat.hip", "fp8_encode.hip", "awq_decode.hip",
            *(f"awq_decode_flat_{m}.hip" for m in (31, 11, 30, 13, 14))]
 
 HIPCC_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}",
-    # Packed FP32 VALU forms stay off (no float code here, but keep the rule global).
+    # Packed FP32 VALU forms stay off.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
