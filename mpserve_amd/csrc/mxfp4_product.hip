@@ -7,74 +7,10 @@
 //
 // For experts, rows of x belong to experts by ranges (offsets) and each expert has weights of
 // its own; rows may be gathered from a token's row by the sorted order.
-#include "mxfp4_common.h"
+#include "mxfp4_product.h"
 
 namespace mps {
 namespace {
-
-struct Args {
-  const void *x;
-  const uint8_t *x_scales;
-  int64_t x_stride;  // elements (16-bit x) from row to row
-  const uint8_t *w, *w_scales;
-  const void *bias;
-  void *out;
-  const int32_t *offsets, *order;  // experts only
-  int32_t rows, x_rows, n, row_blocks, k;
-  int32_t experts, top, gather;
-  int32_t bias_type, out_type;
-};
-
-// The expert and the rows of tile `tile`, where every expert's rows are cut into tiles of `size`
-// rows and the rows past the last expert's into more tiles, as those of expert `experts`.
-// All lanes get the same answer; {-1, 0, 0} past the last tile.
-struct Tile {
-  int32_t expert, first, end;
-};
-__device__ inline Tile find_tile(const int32_t *offsets, int32_t experts, int32_t rows, int32_t size, int32_t tile) {
-  const int lane = threadIdx.x & 63;
-  int32_t before = 0;
-  for (int32_t e0 = 0; e0 <= experts; e0 += 64) {
-    const int32_t e = e0 + lane;
-    int32_t first = 0, end = 0;
-    if (e <= experts) {
-      first = min(max(offsets[e], 0), rows);  // bad offsets give bad sums, never bad addresses
-      end = e < experts ? max(first, min(offsets[e + 1], rows)) : rows;
-    }
-    const int32_t tiles = (end - first + size - 1) / size;
-    int32_t upto = tiles;
-    for (int d = 1; d < 64; d *= 2) {
-      const int32_t v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
-    }
-    const uint64_t hit = __ballot(before + upto > tile);
-    if (hit) {
-      const int at = __ffsll((unsigned long long)hit) - 1;
-      const int32_t in = tile - before - (__shfl(upto, at) - __shfl(tiles, at));
-      const int32_t f = __shfl(first, at) + in * size;
-      return {e0 + at, f, min(f + size, __shfl(end, at))};
-    }
-    before += __shfl(upto, 63);
-  }
-  return {-1, 0, 0};
-}
-
-// Eight elements of a 16-bit row from `col` on, as bits; zeros past column k.
-__device__ inline u32x4 load_row8(const uint16_t *row, int64_t col, int64_t k, bool whole) {
-  if (whole && col + 8 <= k) return *reinterpret_cast<const u32x4 *>(row + col);
-  u32x4 v = {0, 0, 0, 0};
-  for (int i = 0; i < 8; ++i)
-    if (col + i < k) v[i / 2] |= (uint32_t)row[col + i] << (16 * (i % 2));
-  return v;
-}
-
-__device__ inline void split_f16(u32x4 v, bf16x8 &hi, bf16x8 &lo) {
-  for (int i = 0; i < 8; ++i) {
-    const float f = Elem<MPS_TYPE_F16>::get((uint16_t)(v[i / 2] >> (16 * (i % 2))));
-    hi[i] = (__bf16)f;
-    lo[i] = (__bf16)(f - (float)hi[i]);
-  }
-}
 
 // Few rows: a workgroup takes 16 weight rows and kTiles * 16 rows of x, and its waves take the
 // blocks of k in turn and add up their sums through LDS. A lane's 16 bytes of codes are one block
@@ -82,7 +18,7 @@ __device__ inline void split_f16(u32x4 v, bf16x8 &hi, bf16x8 &lo) {
 constexpr int kWaves = 4;
 
 template <int kX, int kTiles>
-__global__ __launch_bounds__(kWaves * 64) void mxfp4_few_rows_kernel(Args a) {
+__global__ __launch_bounds__(kWaves * 64) void mxfp4_few_rows_kernel(ProductArgs a) {
   __shared__ float sums[kWaves][kTiles * 4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   Tile tile = {0, (int32_t)blockIdx.y * kTiles * 16, 0};
@@ -170,7 +106,7 @@ __global__ __launch_bounds__(kWaves * 64) void mxfp4_few_rows_kernel(Args a) {
 }
 
 template <int kX>
-void launch(const Args &a, hipStream_t stream) {
+void launch(const ProductArgs &a, hipStream_t stream) {
   constexpr int kTiles = 4;
   const int64_t tiles = (a.rows + kTiles * 16 - 1) / (kTiles * 16) + (a.offsets ? a.experts : 0);
   const dim3 grid((unsigned)((a.n + 15) / 16), (unsigned)tiles);
@@ -185,8 +121,9 @@ int check(const mps_mxfp4_product *p) {
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: unknown output or bias type");
   if (p->rows < 0 || p->n < 0 || p->k < 0 || p->experts < 0)
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: negative size");
-  if (p->rows > INT32_MAX - 1024 || p->n > INT32_MAX - 1024 || p->k > INT32_MAX - 1024)
+  if (p->rows > INT32_MAX - 1024 || p->n > INT32_MAX - 1024)
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: a size is over 2^31 - 1025");
+  if (p->k > kMaxProductK) return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: k is over %d", kMaxProductK);
   if (p->experts > MPS_MAX_EXPERTS)
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: %lld experts are over %d", (long long)p->experts, MPS_MAX_EXPERTS);
   if (p->rows == 0 || p->n == 0) return MPS_OK;
@@ -203,6 +140,23 @@ int check(const mps_mxfp4_product *p) {
   return MPS_OK;
 }
 
+// Which kernel takes a product, and what it needs.
+struct Way {
+  bool tiles;         // mxfp4_tile.hip; else few rows
+  bool packed;        // x is packed into the workspace first
+  int32_t planes;     // BF16 rows a row of x becomes
+  int64_t x_rows, workspace;
+};
+Way way_of(const mps_mxfp4_product *p) {
+  Way w = {};
+  w.x_rows = p->gather ? p->rows / p->top : p->rows;
+  w.planes = p->x_type == MPS_TYPE_F16 ? 2 : 1;
+  w.tiles = p->rows > 64 * (p->experts > 0 ? p->experts : 1);
+  w.packed = w.tiles && (p->x_type == MPS_TYPE_F16 || (p->x_type == MPS_TYPE_BF16 && !tile_rows(p->x, p->x_stride, p->k)));
+  if (w.packed) w.workspace = w.x_rows * w.planes * packed_width(p->k) * 2;
+  return w;
+}
+
 }  // namespace
 }  // namespace mps
 
@@ -215,7 +169,7 @@ int mps_mxfp4_product_workspace(const mps_mxfp4_product *p, int64_t *bytes) {
   const int rc = check(p);
   if (rc != MPS_OK) return rc;
   if (!bytes) return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: null pointer");
-  *bytes = 0;
+  *bytes = p->rows > 0 && p->n > 0 ? way_of(p).workspace : 0;
   return MPS_OK;
 }
 
@@ -223,15 +177,26 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
   last_error().clear();
   const int rc = check(p);
   if (rc != MPS_OK || p->rows == 0 || p->n == 0) return rc;
-  Args a = {};
+  const Way way = way_of(p);
+  if (way.workspace > 0 && (!workspace || workspace_bytes < way.workspace || !aligned16(workspace)))
+    return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: %lld bytes of workspace are needed, 16-byte aligned",
+                (long long)way.workspace);
+  ProductArgs a = {};
   a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride;
   a.w = p->w, a.w_scales = p->w_scales, a.bias = p->bias, a.out = p->out;
   a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
-  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)(p->gather ? p->rows / p->top : p->rows), a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
+  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)way.x_rows, a.planes = 1, a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
   a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
   a.bias_type = p->bias_type, a.out_type = p->out_type;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (p->x_type == MPS_TYPE_MXFP4)
+  if (way.packed) {
+    a.x_stride = way.planes * packed_width(p->k), a.x_plane = packed_width(p->k), a.planes = way.planes;
+    launch_pack(p->x, p->x_type, way.x_rows, p->x_stride, a, workspace, s);
+    a.x = workspace;
+  }
+  if (way.tiles)
+    launch_tiles(a, p->x_type, s);
+  else if (p->x_type == MPS_TYPE_MXFP4)
     launch<MPS_TYPE_MXFP4>(a, s);
   else if (p->x_type == MPS_TYPE_BF16)
     launch<MPS_TYPE_BF16>(a, s);
