@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmpserve_amd.so")
 ARCH = os.environ.get("MPS_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = ["mxfp4.hip", "mxfp4_product.hip", "mxfp4_tile.hip", "experts.hip",
+SOURCES = ["mxfp4.hip", "mxfp4_product.hip", "mxfp4_tile.hip", "mxfp4_rows.hip", "experts.hip",
            "fp8_decode.hip", "fp8_decode_flat.hip", "fp8_encode.hip", "awq_decode.hip",
            *(f"awq_decode_flat_{m}.hip" for m in (31, 11, 30, 13, 14))]
 

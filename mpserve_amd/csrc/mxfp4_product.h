@@ -72,20 +72,72 @@ __device__ inline void split_f16(u32x4 v, bf16x8 &hi, bf16x8 &lo) {
   }
 }
 
-constexpr int32_t kMaxProductK = 1 << 24;  // offsets inside a tile fit 32 bits
-
-// Rows in tiles of `size`: an upper bound that does not need the offsets.
-inline int64_t product_tiles(const ProductArgs &a, int64_t size) {
-  return (a.rows + size - 1) / size + (a.offsets ? a.experts : 0);
+__device__ inline bf16x8 widen(uint32_t codes, float scale) {
+  u32x4 v;
+  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+  v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+  v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+  return __builtin_bit_cast(bf16x8, v);
 }
 
-// Many rows (mxfp4_tile.hip). x is MXFP4, or BF16 in rows of whole 128-byte pieces at 16-byte
+__device__ inline void copy16(const uint8_t *from, uint8_t *lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+// 16 scale bytes of a row from block `b` on; zeros (2^-127, which takes any product to zero or
+// leaves a zero x as it is) past the row's last block. Rows start at any address.
+__device__ inline u32x4 load_scales(const uint8_t *row, int32_t b, int32_t blocks) {
+  u32x4 v = {0, 0, 0, 0};
+  if (blocks >= 16) {  // the last 16 bytes of a row that ends earlier, moved down
+    const int32_t past = max(0, b + 16 - blocks);
+    __builtin_memcpy(&v, row + b - past, 16);
+    if (past > 0) {
+      unsigned __int128 w = __builtin_bit_cast(unsigned __int128, v);
+      v = __builtin_bit_cast(u32x4, past < 16 ? w >> (8 * past) : (unsigned __int128)0);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < blocks - b; ++i) v[i / 4] |= (uint32_t)row[b + i] << (8 * (i % 4));
+  }
+  return v;
+}
+
+// Four neighbouring columns of a row of the output; `quads`: rows are whole quads at aligned addresses.
+__device__ inline void store4(const ProductArgs &a, int64_t row, int32_t col, f32x4 v, bool quads) {
+  const int64_t at = row * a.n + col;
+  if (!quads) {
+    for (int j = 0; j < 4; ++j)
+      if (col + j < a.n) store_as(a.out, a.out_type, at + j, v[j]);
+  } else if (a.out_type == MPS_TYPE_F32) {
+    *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
+  } else {
+    uint64_t h = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      h |= (uint64_t)(a.out_type == MPS_TYPE_BF16 ? Elem<MPS_TYPE_BF16>::put(v[j]) : Elem<MPS_TYPE_F16>::put(v[j])) << (16 * j);
+    *reinterpret_cast<uint64_t *>(static_cast<uint16_t *>(a.out) + at) = h;
+  }
+}
+
+constexpr int32_t kMaxProductK = 1 << 24;  // offsets inside a tile fit 32 bits
+
+// Tiles of `size` rows: m ranges that are not empty have at most (rows + m (size - 1)) / size, which
+// does not need the offsets.
+inline int64_t product_tiles(const ProductArgs &a, int64_t size) {
+  const int64_t ranges = a.offsets ? (a.experts < a.rows ? a.experts + 1 : a.rows) : 1;
+  return (a.rows + ranges * (size - 1)) / size;
+}
+
+// Few rows (mxfp4_rows.hip). x is MXFP4, or 16-bit rows of whole 16-byte pieces.
+void launch_rows(const ProductArgs &a, int32_t x_type, hipStream_t stream);
+inline bool piece_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 8 == 0; }
+
+// Many rows (mxfp4_tile.hip). x is MXFP4, or BF16 in rows of whole 128-byte steps at 16-byte
 // addresses; `planes` of them, x_plane elements apart, add up to a row of x.
 void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream);
-inline bool tile_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 64 == 0; }
-// Writes x[rows, a.k] as such rows, a.x_plane elements wide, with zeros past column k.
-void launch_pack(const void *x, int32_t x_type, int64_t rows, int64_t stride, const ProductArgs &a, void *out,
-                 hipStream_t stream);
+inline bool step_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 64 == 0; }
 inline int64_t packed_width(int64_t k) { return (k + 63) / 64 * 64; }
 
 }  // namespace mps

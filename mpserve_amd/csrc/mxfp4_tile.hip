@@ -20,38 +20,6 @@ __device__ inline f32x16 multiply4(i32x4 w, uint32_t ws, i32x4 x, uint32_t xs, f
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, J, ws, J, xs);
 }
 
-__device__ inline bf16x8 widen(uint32_t codes, float scale) {
-  u32x4 v;
-  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
-  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
-  v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
-  v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
-  return __builtin_bit_cast(bf16x8, v);
-}
-
-__device__ inline void copy16(const uint8_t *from, uint8_t *lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                   (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
-}
-
-// 16 scale bytes of a row from block `b` on; zeros (2^-127, which takes any product to zero or
-// leaves a zero x as it is) past the row's last block. Rows start at any address.
-__device__ inline u32x4 load_scales(const uint8_t *row, int32_t b, int32_t blocks) {
-  u32x4 v = {0, 0, 0, 0};
-  if (blocks >= 16) {  // the last 16 bytes of a row that ends earlier, moved down
-    const int32_t past = max(0, b + 16 - blocks);
-    __builtin_memcpy(&v, row + b - past, 16);
-    if (past > 0) {
-      unsigned __int128 w = __builtin_bit_cast(unsigned __int128, v);
-      v = __builtin_bit_cast(u32x4, past < 16 ? w >> (8 * past) : (unsigned __int128)0);
-    }
-  } else {
-#pragma unroll 1
-    for (int i = 0; i < blocks - b; ++i) v[i / 4] |= (uint32_t)row[b + i] << (8 * (i % 4));
-  }
-  return v;
-}
-
 template <bool k4, int BT, int BN, int WT, int WN>
 struct Shape {
   static constexpr int kThreads = WT * WN * 64;
@@ -294,19 +262,7 @@ __global__ __launch_bounds__(WT *WN * 64) void mxfp4_tile_kernel(ProductArgs a, 
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += bias[j];
       if (first + row >= tile.end || col >= a.n) continue;
-      const int64_t at = (int64_t)(first + row) * a.n + col;
-      if (!quads) {
-        for (int j = 0; j < 4; ++j)
-          if (col + j < a.n) store_as(a.out, a.out_type, at + j, v[j]);
-      } else if (a.out_type == MPS_TYPE_F32) {
-        *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
-      } else {
-        uint64_t h = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          h |= (uint64_t)(a.out_type == MPS_TYPE_BF16 ? Elem<MPS_TYPE_BF16>::put(v[j]) : Elem<MPS_TYPE_F16>::put(v[j])) << (16 * j);
-        *reinterpret_cast<uint64_t *>(static_cast<uint16_t *>(a.out) + at) = h;
-      }
+      store4(a, first + row, col, v, quads);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -320,25 +276,6 @@ void launch(const ProductArgs &a, hipStream_t stream) {
                      (int32_t)tt, (int32_t)tn);
 }
 
-// Eight elements a work-item; kHalf: FP16 as hi and lo planes.
-template <bool kHalf>
-__global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride,
-                                                         int32_t k, int32_t width, uint16_t *__restrict__ out) {
-  const uint32_t pieces = (uint32_t)width / 8;
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / pieces;
-  const int32_t col = (int32_t)(unit - row * pieces) * 8;
-  if (row >= rows) return;
-  const u32x4 v = load_row8(x + row * stride, col, k, aligned16(x) && stride % 8 == 0);
-  if constexpr (kHalf) {
-    bf16x8 hi, lo;
-    split_f16(v, hi, lo);
-    *reinterpret_cast<bf16x8 *>(out + row * 2 * width + col) = hi;
-    *reinterpret_cast<bf16x8 *>(out + (row * 2 + 1) * width + col) = lo;
-  } else {
-    *reinterpret_cast<u32x4 *>(out + row * width + col) = v;
-  }
-}
-
 }  // namespace
 
 void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream) {
@@ -346,18 +283,6 @@ void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream) {
     launch<true, 256, 256, 2, 4>(a, stream);
   else
     launch<false, 256, 256, 2, 4>(a, stream);
-}
-
-void launch_pack(const void *x, int32_t x_type, int64_t rows, int64_t stride, const ProductArgs &a, void *out,
-                 hipStream_t stream) {
-  const int32_t width = (int32_t)a.x_plane;
-  const dim3 grid((unsigned)((rows * (width / 8) + 255) / 256));
-  if (x_type == MPS_TYPE_F16)
-    hipLaunchKernelGGL((mxfp4_pack_kernel<true>), grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x), rows,
-                       stride, a.k, width, static_cast<uint16_t *>(out));
-  else
-    hipLaunchKernelGGL((mxfp4_pack_kernel<false>), grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x), rows,
-                       stride, a.k, width, static_cast<uint16_t *>(out));
 }
 
 }  // namespace mps
