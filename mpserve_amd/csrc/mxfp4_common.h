@@ -14,6 +14,7 @@ constexpr int kMxBlock = 32;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -31,6 +32,11 @@ inline int64_t type_bytes(int32_t t) { return t == MPS_TYPE_F32 ? 4 : 2; }
 // The scale conversions take: only the exponent's bits count, so byte 0 is 2^-127 though its
 // bits are those of 0.0, and byte 255 makes every result NaN.
 __device__ inline float mx_scale(uint32_t s) { return __uint_as_float(s << 23); }
+
+// The scale itself, for FP32 arithmetic.
+__device__ inline float mx_scale_value(uint32_t s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
+}
 
 template <int T>
 struct Elem;

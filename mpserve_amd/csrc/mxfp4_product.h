@@ -16,8 +16,6 @@ struct ProductArgs {
   int32_t rows, x_rows, n, row_blocks, k;
   int32_t experts, top, gather;
   int32_t bias_type, out_type;
-  int32_t planes;   // BF16 rows that are added up to one row of x
-  int64_t x_plane;  // elements from one to the next
 };
 
 // The expert and the rows of tile `tile`, where every expert's rows are cut into tiles of `size`
@@ -63,15 +61,7 @@ __device__ inline u32x4 load_row8(const uint16_t *row, int64_t col, int64_t k, b
   return v;
 }
 
-// FP16 as a sum of two BF16: hi takes the first eight significant bits, lo the other three exactly.
-__device__ inline void split_f16(u32x4 v, bf16x8 &hi, bf16x8 &lo) {
-  for (int i = 0; i < 8; ++i) {
-    const float f = Elem<MPS_TYPE_F16>::get((uint16_t)(v[i / 2] >> (16 * (i % 2))));
-    hi[i] = (__bf16)f;
-    lo[i] = (__bf16)(f - (float)hi[i]);
-  }
-}
-
+// Eight codes' values in BF16, scaled: exact.
 __device__ inline bf16x8 widen(uint32_t codes, float scale) {
   u32x4 v;
   v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
@@ -81,27 +71,39 @@ __device__ inline bf16x8 widen(uint32_t codes, float scale) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
+// The codes' values in FP16, without a scale.
+__device__ inline f16x8 widen_f16(uint32_t codes) {
+  u32x4 v;
+  v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 0));
+  v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 1));
+  v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 2));
+  v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 3));
+  return __builtin_bit_cast(f16x8, v);
+}
+
 __device__ inline void copy16(const uint8_t *from, uint8_t *lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                    (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 
-// 16 scale bytes of a row from block `b` on; zeros (2^-127, which takes any product to zero or
-// leaves a zero x as it is) past the row's last block. Rows start at any address.
+// 16 scale bytes of a row from block `b` on, and zeros (2^-127, which takes any product to zero or
+// leaves a zero x as it is) past the row's last block. Rows start at any address. The load comes
+// apart from what is done to it, so that nothing waits for it where it is issued: near a row's
+// end it takes the last 16 bytes, which move_scales then moves down.
 __device__ inline u32x4 load_scales(const uint8_t *row, int32_t b, int32_t blocks) {
   u32x4 v = {0, 0, 0, 0};
-  if (blocks >= 16) {  // the last 16 bytes of a row that ends earlier, moved down
-    const int32_t past = max(0, b + 16 - blocks);
-    __builtin_memcpy(&v, row + b - past, 16);
-    if (past > 0) {
-      unsigned __int128 w = __builtin_bit_cast(unsigned __int128, v);
-      v = __builtin_bit_cast(u32x4, past < 16 ? w >> (8 * past) : (unsigned __int128)0);
-    }
+  if (blocks >= 16) {
+    __builtin_memcpy(&v, row + min(b, blocks - 16), 16);
   } else {
 #pragma unroll 1
-    for (int i = 0; i < blocks - b; ++i) v[i / 4] |= (uint32_t)row[b + i] << (8 * (i % 4));
+    for (int i = 0; i < blocks; ++i) v[i / 4] |= (uint32_t)row[i] << (8 * (i % 4));
   }
   return v;
+}
+__device__ inline u32x4 move_scales(u32x4 v, int32_t b, int32_t blocks) {
+  if (blocks < 16 || b + 16 <= blocks) return v;
+  const int32_t past = b + 16 - blocks;
+  return past < 16 ? __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * past)) : u32x4{0, 0, 0, 0};
 }
 
 // Four neighbouring columns of a row of the output; `quads`: rows are whole quads at aligned addresses.
@@ -134,8 +136,7 @@ inline int64_t product_tiles(const ProductArgs &a, int64_t size) {
 void launch_rows(const ProductArgs &a, int32_t x_type, hipStream_t stream);
 inline bool piece_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 8 == 0; }
 
-// Many rows (mxfp4_tile.hip). x is MXFP4, or BF16 in rows of whole 128-byte steps at 16-byte
-// addresses; `planes` of them, x_plane elements apart, add up to a row of x.
+// Many rows (mxfp4_tile.hip). x is MXFP4, or 16-bit rows of whole 128-byte steps at 16-byte addresses.
 void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream);
 inline bool step_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 64 == 0; }
 inline int64_t packed_width(int64_t k) { return (k + 63) / 64 * 64; }

@@ -12,36 +12,16 @@
 namespace mps {
 namespace {
 
-// Eight elements a work-item; kSplit: FP16 as BF16 planes hi and lo.
-template <bool kSplit>
+// x[rows, k] as rows of whole 128-byte steps, `width` elements wide, with zeros past column k; eight
+// elements a work-item.
 __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride,
                                                          int32_t k, int32_t width, uint16_t *__restrict__ out) {
   const uint32_t pieces = (uint32_t)width / 8;
   const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / pieces;
   const int32_t col = (int32_t)(unit - row * pieces) * 8;
   if (row >= rows) return;
-  const u32x4 v = load_row8(x + row * stride, col, k, aligned16(x) && stride % 8 == 0);
-  if constexpr (kSplit) {
-    bf16x8 hi, lo;
-    split_f16(v, hi, lo);
-    *reinterpret_cast<bf16x8 *>(out + row * 2 * width + col) = hi;
-    *reinterpret_cast<bf16x8 *>(out + (row * 2 + 1) * width + col) = lo;
-  } else {
-    *reinterpret_cast<u32x4 *>(out + row * width + col) = v;
-  }
-}
-
-// x[rows, a.k] as rows of whole steps, a.x_plane elements wide, with zeros past column k.
-void launch_pack(const void *x, bool split, int64_t rows, int64_t stride, const ProductArgs &a, void *out,
-                 hipStream_t stream) {
-  const int32_t width = (int32_t)a.x_plane;
-  const dim3 grid((unsigned)((rows * (width / 8) + 255) / 256));
-  if (split)
-    hipLaunchKernelGGL((mxfp4_pack_kernel<true>), grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x), rows,
-                       stride, a.k, width, static_cast<uint16_t *>(out));
-  else
-    hipLaunchKernelGGL((mxfp4_pack_kernel<false>), grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x), rows,
-                       stride, a.k, width, static_cast<uint16_t *>(out));
+  const bool whole = aligned16(x) && stride % 8 == 0;
+  *reinterpret_cast<u32x4 *>(out + row * width + col) = load_row8(x + row * stride, col, k, whole);
 }
 
 int check(const mps_mxfp4_product *p) {
@@ -74,20 +54,16 @@ int check(const mps_mxfp4_product *p) {
 // Which kernel takes a product, and what it needs.
 struct Way {
   bool tiles;         // mxfp4_tile.hip, else mxfp4_rows.hip
-  bool split;         // FP16 x becomes planes hi and lo
   bool packed;        // x is packed into the workspace first
-  int32_t planes;     // BF16 rows a row of x becomes
   int64_t x_rows, workspace;
 };
 Way way_of(const mps_mxfp4_product *p) {
   Way w = {};
   w.x_rows = p->gather ? p->rows / p->top : p->rows;
   w.tiles = p->rows > 64 * (p->experts > 0 ? p->experts : 1);
-  w.split = w.tiles && p->x_type == MPS_TYPE_F16;
-  w.planes = w.split ? 2 : 1;
   w.packed = p->x_type != MPS_TYPE_MXFP4 && p->k > 0 &&
-             (w.split || !(w.tiles ? step_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k)));
-  if (w.packed) w.workspace = w.x_rows * w.planes * packed_width(p->k) * 2;
+             !(w.tiles ? step_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
+  if (w.packed) w.workspace = w.x_rows * packed_width(p->k) * 2;
   return w;
 }
 
@@ -119,14 +95,16 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
   a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride;
   a.w = p->w, a.w_scales = p->w_scales, a.bias = p->bias, a.out = p->out;
   a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
-  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)way.x_rows, a.planes = 1, a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
+  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)way.x_rows, a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
   a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
   a.bias_type = p->bias_type, a.out_type = p->out_type;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (way.packed) {
-    a.x_stride = way.planes * packed_width(p->k), a.x_plane = packed_width(p->k), a.planes = way.planes;
-    launch_pack(p->x, way.split, way.x_rows, p->x_stride, a, workspace, s);
-    a.x = workspace, a.k = (int32_t)a.x_plane;
+    const int32_t width = (int32_t)packed_width(p->k);
+    const dim3 grid((unsigned)((way.x_rows * (width / 8) + 255) / 256));
+    hipLaunchKernelGGL(mxfp4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), way.x_rows,
+                       p->x_stride, a.k, width, static_cast<uint16_t *>(workspace));
+    a.x = workspace, a.x_stride = width, a.k = width;
   }
   if (way.tiles)
     launch_tiles(a, p->x_type, s);

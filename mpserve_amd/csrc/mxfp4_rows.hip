@@ -7,8 +7,14 @@
 // added up in wave order, so results do not depend on timing.
 //
 // A stage is 128 bytes of every row of x (64 elements of 16 bits, or 256 codes), in pieces of 16
-// bytes, piece p of row r at place p ^ (r & 7), and the weights of the same k: 32 bytes a row, or
-// 128 beside MXFP4 x. Lanes 16 g + r multiply pieces 2 g and 2 g + 1 of their row.
+// bytes, piece p of row r at place p ^ (r / 2 % 8), and the weights of the same k: 32 bytes a row, or
+// 128 beside MXFP4 x (their two pieces at p ^ (r / 8 % 2), their eight as x's). In a lane 16 g + r of a 16-row fragment, MXFP4 takes pieces 2 g and 2 g + 1
+// of row r, and 16-bit x piece g of one block of k after the other.
+//
+// FP16 x meets the codes' values in FP16, without their scale, which could leave FP16's range;
+// the products of a block are summed by themselves and added with the scale in FP32, exactly as
+// if it had been in the weight. (BF16 holds the scaled weight. FP16 as a sum of two BF16 took
+// twice the matrix instructions and 32 conversions a fragment: 31.7 us for 37 rows of 5000 x 3001.)
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -39,7 +45,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
   constexpr bool k4 = R::k4;
   constexpr int kFT = R::kFT;
   __shared__ __attribute__((aligned(16))) uint8_t lds[R::kLds];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   Tile tile = {0, (int32_t)blockIdx.y * R::kRows, 0};
   tile.end = min(a.rows, tile.first + R::kRows);
   if (a.offsets) tile = find_tile(a.offsets, a.experts, a.rows, R::kRows, blockIdx.y);
@@ -54,7 +60,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
     const int32_t items = ((periods - wave + W - 1) / W) * R::kSteps;
     // Where this lane's pieces come from; rows past the tile's end or the weight's are the last ones.
     const int64_t x_row_bytes = k4 ? (int64_t)blocks * 16 : a.x_stride * 2;
-    const int32_t x_piece = (lane % 8) ^ (lane / 8), x_pieces = k4 ? blocks : a.k / 8;
+    const int32_t x_piece = (lane % 8) ^ (lane / 16), x_pieces = k4 ? blocks : a.k / 8;
     const uint8_t *x_from[XL];
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
@@ -66,7 +72,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
     const uint8_t *const w_base = a.w + w_first * blocks * 16;
     const uint32_t w_row_bytes = (uint32_t)blocks * 16, w_last = (uint32_t)min(R::kBN - 1, a.n - 1 - n0) * w_row_bytes;
     const int wrow = lane / R::kWPieces;
-    const int32_t w_piece = k4 ? (lane % 8) ^ (wrow & 7) : lane % 2;
+    const int32_t w_piece = k4 ? (lane % 8) ^ (wrow >> 1) : (lane % 2) ^ (wrow >> 3 & 1);
     const uint8_t *s_from[R::kSL];
 #pragma unroll
     for (int i = 0; i < R::kSL; ++i) {
@@ -81,13 +87,16 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
     auto fetch = [&](int32_t item, int slot) {
       const int32_t step = period_of(item) * R::kSteps + item % R::kSteps;
       uint8_t *const to = mine + slot * R::kStage;
-      const int32_t x_at = min(step * 8 + x_piece, x_pieces - 1) * 16;
+      // Eight rows a load: rows of odd loads have the other half of the places' keys.
+      const int32_t x_at[2] = {min(step * 8 + x_piece, x_pieces - 1) * 16, min(step * 8 + (x_piece ^ 4), x_pieces - 1) * 16};
 #pragma unroll
-      for (int i = 0; i < XL; ++i) copy16(x_from[i] + x_at, to + i * 1024);
-      const uint32_t w_at = (uint32_t)min(step * R::kWPieces + w_piece, blocks - 1) * 16;
+      for (int i = 0; i < XL; ++i) copy16(x_from[i] + x_at[i & 1], to + i * 1024);
+      const uint32_t w_at[2] = {(uint32_t)min(step * R::kWPieces + w_piece, blocks - 1) * 16,
+                                (uint32_t)min(step * R::kWPieces + (w_piece ^ 4), blocks - 1) * 16};
 #pragma unroll
       for (int i = 0; i < R::kWL; ++i)
-        copy16(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at), to + R::kXBytes + i * 1024);
+        copy16(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at[k4 ? i & 1 : 0]),
+               to + R::kXBytes + i * 1024);
     };
     u32x4 scales[R::kSL];
     auto get_scales = [&](int32_t period) {
@@ -104,7 +113,8 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
       const int32_t in = item % R::kSteps;
       if (in == 0) {  // the lane's rows' 16 scale bytes, at its place; LDS keeps a wave's order
 #pragma unroll
-        for (int i = 0; i < R::kSL; ++i) *reinterpret_cast<u32x4 *>(ss + (i * 64 + lane) * 16) = scales[i];
+        for (int i = 0; i < R::kSL; ++i) 
+          *reinterpret_cast<u32x4 *>(ss + (i * 64 + lane) * 16) = move_scales(scales[i], 16 * period_of(item), blocks);
         if (item + R::kSteps < items) get_scales(period_of(item) + W);
       }
       if (item + S - 1 < items) {
@@ -124,7 +134,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
           sw[n] = *reinterpret_cast<const uint16_t *>(ss + (R::kRows + n * 16 + r) * 16 + in * 8 + g * 2);
         auto half = [&](auto jc) {
           constexpr int j = decltype(jc)::value;
-          const int at = ((2 * g + j) ^ (r & 7)) * 16;
+          const int at = ((2 * g + j) ^ (r >> 1)) * 16;
           i32x4 fw[FN];
 #pragma unroll
           for (int n = 0; n < FN; ++n) fw[n] = *reinterpret_cast<const i32x4 *>(wl + (n * 16 + r) * 128 + at);
@@ -133,48 +143,58 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
             const i32x4 fx = *reinterpret_cast<const i32x4 *>(xl + (t * 16 + r) % R::kRows * 128 + at);
 #pragma unroll
             for (int n = 0; n < FN; ++n) {
-              const i32x8 wa = {fw[n][0], fw[n][1], fw[n][2], fw[n][3], 0, 0, 0, 0}, xb = {fx[0], fx[1], fx[2], fx[3], 0, 0, 0, 0};
-              acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[t][n], 4, 4, j, sw[n], j, sx[t]);
+              const i32x8 wb = {fw[n][0], fw[n][1], fw[n][2], fw[n][3], 0, 0, 0, 0}, xa = {fx[0], fx[1], fx[2], fx[3], 0, 0, 0, 0};
+              acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(xa, wb, acc[t][n], 4, 4, j, sx[t], j, sw[n]);
             }
           }
         };
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
       } else {
-        uint64_t fw[FN];
-        float sw[FN];
+        u32x4 fx[kFT][2];
+        uint32_t fw[FN][2], bytes[FN];
 #pragma unroll
         for (int n = 0; n < FN; ++n) {
-          fw[n] = *reinterpret_cast<const uint64_t *>(wl + (n * 16 + r) * 32 + g * 8);
-          sw[n] = mx_scale(ss[(n * 16 + r) * 16 + in * 2 + g / 2]);
+          bytes[n] = *reinterpret_cast<const uint16_t *>(ss + (n * 16 + r) * 16 + in * 2);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) fw[n][j] = *reinterpret_cast<const uint32_t *>(wl + (n * 16 + r) * 32 + (j ^ (r >> 3)) * 16 + g * 4);
         }
+#pragma unroll
+        for (int t = 0; t < kFT; ++t)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            fx[t][j] = *reinterpret_cast<const u32x4 *>(xl + (t * 16 + r) % R::kRows * 128 + ((4 * j + g) ^ (r >> 1)) * 16);
+        __builtin_amdgcn_sched_barrier(0);
         // Pieces past the end of x's rows hold other elements: they are taken as zeros.
         const int32_t left = a.k / 8 - (period_of(item) * R::kSteps + in) * 8;
+        if (left < 8) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          bf16x8 w[FN];
+          for (int t = 0; t < kFT; ++t)
 #pragma unroll
-          for (int n = 0; n < FN; ++n) w[n] = widen((uint32_t)(fw[n] >> (32 * j)), sw[n]);
+            for (int j = 0; j < 2; ++j)
+              if (4 * j + g >= left) fx[t][j] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
-          for (int t = 0; t < kFT; ++t) {
-            u32x4 v = *reinterpret_cast<const u32x4 *>(xl + (t * 16 + r) % R::kRows * 128 + ((2 * g + j) ^ (r & 7)) * 16);
-            if (left < 8)
-              if (2 * g + j >= left) v = u32x4{0, 0, 0, 0};
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int n = 0; n < FN; ++n) {
+            const uint32_t byte = j ? bytes[n] >> 8 : bytes[n] & 255;
             if constexpr (XT == MPS_TYPE_F16) {
-              bf16x8 hi, lo;
-              split_f16(v, hi, lo);
+              const f16x8 w = widen_f16(fw[n][j]);
+              const float scale = mx_scale_value(byte);
 #pragma unroll
-              for (int n = 0; n < FN; ++n) {
-                acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[n], hi, acc[t][n], 0, 0, 0);
-                acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[n], lo, acc[t][n], 0, 0, 0);
+              for (int t = 0; t < kFT; ++t) {
+                const f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fx[t][j]), w, f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
               }
             } else {
+              const bf16x8 w = widen(fw[n][j], mx_scale(byte));
 #pragma unroll
-              for (int n = 0; n < FN; ++n)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[n], __builtin_bit_cast(bf16x8, v), acc[t][n], 0, 0, 0);
+              for (int t = 0; t < kFT; ++t)
+                acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fx[t][j]), w, acc[t][n], 0, 0, 0);
             }
           }
-        }
       }
       slot = slot == S - 1 ? 0 : slot + 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read: the next loads may take its place
@@ -188,22 +208,26 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
 #pragma unroll
     for (int n = 0; n < FN; ++n) *reinterpret_cast<f32x4 *>(sums + ((wave * kFT + t) * FN + n) * 256 + lane * 4) = acc[t][n];
   __syncthreads();
-  // A lane has row 16 t + r and columns 16 n + 4 g .. + 3 of fragment (t, n); the waves share the fragments.
+  // In fragment (t, n) lane 16 g + r has rows 16 t + 4 g .. + 3 of column 16 n + r; the waves share
+  // the fragments, a lane now taking four columns of row 16 t + lane / 4.
   const bool quads = a.n % 4 == 0 && aligned16(a.out);
   for (int f = wave; f < kFT * FN; f += W) {
-    const int t = f / FN, n = f % FN;
-    const int32_t row = tile.first + t * 16 + r, col = n0 + n * 16 + 4 * g;
-    if (t * 16 + r >= R::kRows || row >= tile.end || col >= a.n) continue;
+    const int in_row = lane / 4, in_col = lane % 4 * 4;
+    const int32_t row = tile.first + f / FN * 16 + in_row, col = n0 + f % FN * 16 + in_col;
+    if (f / FN * 16 + in_row >= R::kRows || row >= tile.end || col >= a.n) continue;
     f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < W; ++w) v += *reinterpret_cast<const f32x4 *>(sums + (w * kFT * FN + f) * 256 + lane * 4);
-    float b[4] = {0, 0, 0, 0};
+    for (int w = 0; w < W; ++w) {
+      const float *const from = sums + (w * kFT * FN + f) * 256 + (in_row / 4 * 16 + in_col) * 4 + in_row % 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += from[4 * j];
+    }
     if (a.bias && !none) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col + j < a.n) b[j] = load_as_float(a.bias, a.bias_type, (int64_t)tile.expert * a.n + col + j);
+        if (col + j < a.n) v[j] += load_as_float(a.bias, a.bias_type, (int64_t)tile.expert * a.n + col + j);
     }
-    store4(a, row, col, f32x4{v[0] + b[0], v[1] + b[1], v[2] + b[2], v[3] + b[3]}, quads);
+    store4(a, row, col, v, quads);
   }
 }
 

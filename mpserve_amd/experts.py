@@ -45,7 +45,9 @@ def expert_sort(ids: torch.Tensor, num_experts: int) -> ExpertSort:
     device, (t, top) = ids.device, ids.shape
     lib = _native.lib()
     need = ctypes.c_int64(0)
-    _native.check(lib.mps_expert_sort_workspace(t, top, num_experts, need))
+    rc = lib.mps_expert_sort_workspace(t, top, num_experts, need)
+    if rc:
+        _native.check(rc)
     order = torch.empty(t * top, dtype=torch.int32, device=device)
     positions = torch.empty((t, top), dtype=torch.int32, device=device)
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=device)
@@ -56,13 +58,20 @@ def expert_sort(ids: torch.Tensor, num_experts: int) -> ExpertSort:
 
 
 def _check_sort(sort: ExpertSort, device: torch.device) -> None:
-    for t, name in ((sort.order, "sort.order"), (sort.positions, "sort.positions"), (sort.offsets, "sort.offsets")):
+    order, positions, offsets = sort
+    i32 = torch.int32
+    if isinstance(order, torch.Tensor) and isinstance(positions, torch.Tensor) and isinstance(offsets, torch.Tensor) \
+            and order.device == positions.device == offsets.device == device \
+            and order.dtype == positions.dtype == offsets.dtype == i32 \
+            and order.is_contiguous() and positions.is_contiguous() and offsets.is_contiguous():
+        if positions.dim() != 2 or order.dim() != 1 or offsets.dim() != 1 or order.numel() != positions.numel() \
+                or offsets.numel() < 2:
+            raise ValueError("sort must be what expert_sort returns")
+        return
+    for t, name in ((order, "sort.order"), (positions, "sort.positions"), (offsets, "sort.offsets")):
         _check_cuda_contig(t, name, device)
-        if t.dtype != torch.int32:
+        if t.dtype != i32:
             raise ValueError(f"{name} must be torch.int32")
-    if sort.positions.dim() != 2 or sort.order.dim() != 1 or sort.offsets.dim() != 1 \
-            or sort.order.numel() != sort.positions.numel() or sort.offsets.numel() < 2:
-        raise ValueError("sort must be what expert_sort returns")
 
 
 def _check_rows(t: torch.Tensor, name: str, rows: int, device: Optional[torch.device] = None) -> None:
@@ -81,15 +90,19 @@ def _sum_rows(y: torch.Tensor, weights: Optional[torch.Tensor], positions: torch
     return out
 
 
+def _gather_rows(x: torch.Tensor, order: torch.Tensor, positions: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    t, top = positions.shape
+    rows = torch.empty((t * top, x.shape[1]), dtype=x.dtype, device=x.device)
+    _call(x.device, _native.lib().mps_expert_gather, x.data_ptr(), _TYPES[x.dtype], t, top, offsets.numel() - 1,
+          x.shape[1], order.data_ptr(), offsets.data_ptr(), rows.data_ptr())
+    return rows
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, positions, offsets):
         ctx.save_for_backward(positions)
-        t, top = positions.shape
-        rows = torch.empty((t * top, x.shape[1]), dtype=x.dtype, device=x.device)
-        _call(x.device, _native.lib().mps_expert_gather, x.data_ptr(), _TYPES[x.dtype], t, top, offsets.numel() - 1,
-              x.shape[1], order.data_ptr(), offsets.data_ptr(), rows.data_ptr())
-        return rows
+        return _gather_rows(x, order, positions, offsets)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -123,7 +136,9 @@ def expert_gather(x: torch.Tensor, sort: ExpertSort) -> torch.Tensor:
     _check_cuda(x, "x")
     _check_sort(sort, x.device)
     _check_rows(x, "x", sort.positions.shape[0])
-    return _Gather.apply(x.contiguous(), sort.order, sort.positions, sort.offsets)
+    if not (x.requires_grad and torch.is_grad_enabled()):
+        return _gather_rows(x.contiguous(), *sort)
+    return _Gather.apply(x.contiguous(), *sort)
 
 
 def expert_combine(y: torch.Tensor, weights: torch.Tensor, sort: ExpertSort) -> torch.Tensor:
@@ -138,7 +153,10 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, sort: ExpertSort) -> 
     _type(weights, "weights")
     if weights.shape != sort.positions.shape:
         raise ValueError(f"weights must have shape {tuple(sort.positions.shape)}, got {tuple(weights.shape)}")
-    return _Combine.apply(y.contiguous(), weights.contiguous(), sort.order, sort.positions, sort.offsets)
+    y, weights = y.contiguous(), weights.contiguous()
+    if not ((y.requires_grad or weights.requires_grad) and torch.is_grad_enabled()):
+        return _sum_rows(y, weights, sort.positions)
+    return _Combine.apply(y, weights, *sort)
 
 
 def mxfp4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, sort: ExpertSort,

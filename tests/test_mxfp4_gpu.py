@@ -212,6 +212,24 @@ def test_products_smallest_and_largest_scales():
         plain.close(mxfp4_matmul(xc, xs, codes, scales, out_dtype=torch.float32), xv @ w.T, xv.abs() @ w.abs().T, 256)
 
 
+@pytest.mark.parametrize("t", (3, 40, 200))
+def test_linear_f16_with_scales_outside_f16(t):
+    """Weights far below and far above what FP16 holds, and blocks of both in one row."""
+    g = gen(t)
+    codes, scales = plain.random_weight(g, (70,), 256, DEV, 0, 3)
+    scales[::2, 1::2] = torch.randint(60, 100, (35, 4), generator=g, device=DEV, dtype=torch.uint8)
+    scales[3] = torch.randint(150, 160, (8,), generator=g, device=DEV, dtype=torch.uint8)
+    w = plain.dequantize(codes, scales, 256)
+    x = torch.randn(t, 256, generator=g, device=DEV).to(torch.float16)
+    want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+    normal = size > 2.0 ** -100  # FP32 sums of the other columns are below its normal numbers
+    y = mxfp4_linear(x, codes, scales, out_dtype=torch.float32)
+    plain.close(torch.where(normal, y, torch.zeros_like(y)), torch.where(normal, want, torch.zeros_like(want)), size, 256)
+    assert float((y.double() - want).abs()[~normal].max()) <= 256 * 2.0 ** -149
+    scales[9, 0] = 255
+    assert bool(torch.isnan(mxfp4_linear(x, codes, scales)[:, 9]).all())
+
+
 def test_products_without_rows_columns_or_terms():
     codes, scales = torch.zeros(5, 0, dtype=torch.uint8, device=DEV), torch.zeros(5, 0, dtype=torch.uint8, device=DEV)
     bias = torch.arange(5, device=DEV).to(torch.bfloat16)
