@@ -123,6 +123,20 @@ __device__ inline void store4(const ProductArgs &a, int64_t row, int32_t col, f3
   }
 }
 
+// Two values as 16-bit ones.
+__device__ inline uint32_t pack2(float lo, float hi, int32_t type) {
+  if (type == MPS_TYPE_BF16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
+}
+
+// The biases of four neighbouring columns; zeros past the last column.
+__device__ inline f32x4 load_bias4(const ProductArgs &a, int32_t expert, int32_t col) {
+  f32x4 v = {0, 0, 0, 0};
+  for (int j = 0; j < 4; ++j)
+    if (col + j < a.n) v[j] = load_as_float(a.bias, a.bias_type, (int64_t)expert * a.n + col + j);
+  return v;
+}
+
 constexpr int32_t kMaxProductK = 1 << 24;  // offsets inside a tile fit 32 bits
 
 // Tiles of `size` rows: m ranges that are not empty have at most (rows + m (size - 1)) / size, which
@@ -136,9 +150,9 @@ inline int64_t product_tiles(const ProductArgs &a, int64_t size) {
 void launch_rows(const ProductArgs &a, int32_t x_type, hipStream_t stream);
 inline bool piece_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 8 == 0; }
 
-// Many rows (mxfp4_tile.hip). x is MXFP4, or 16-bit rows of whole 128-byte steps at 16-byte addresses.
-void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream);
-inline bool step_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 64 == 0; }
-inline int64_t packed_width(int64_t k) { return (k + 63) / 64 * 64; }
+// Many rows (mxfp4_tile.hip). x is MXFP4, or 16-bit rows of whole blocks at 16-byte addresses.
+void launch_tiles(const ProductArgs &a, int32_t x_type, int32_t cus, hipStream_t stream);
+inline bool block_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 32 == 0; }
+inline int64_t packed_width(int64_t k) { return (k + 31) / 32 * 32; }
 
 }  // namespace mps

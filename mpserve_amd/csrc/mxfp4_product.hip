@@ -7,12 +7,14 @@
 //
 // For experts, rows of x belong to experts by ranges (offsets) and each expert has weights of
 // its own; rows may be gathered from a token's row by the sorted order.
+#include <atomic>
+
 #include "mxfp4_product.h"
 
 namespace mps {
 namespace {
 
-// x[rows, k] as rows of whole 128-byte steps, `width` elements wide, with zeros past column k; eight
+// x[rows, k] as rows of whole blocks, `width` elements wide, with zeros past column k; eight
 // elements a work-item.
 __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride,
                                                          int32_t k, int32_t width, uint16_t *__restrict__ out) {
@@ -51,6 +53,18 @@ int check(const mps_mxfp4_product *p) {
   return MPS_OK;
 }
 
+// The current device's CUs; asked once a device.
+int32_t compute_units() {
+  constexpr int kDevices = 64;
+  static std::atomic<int32_t> known[kDevices];
+  int device = 0, cus = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= kDevices) return 256;
+  if (const int32_t k = known[device].load(std::memory_order_relaxed)) return k;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus < 1) return 256;
+  known[device].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
 // Which kernel takes a product, and what it needs.
 struct Way {
   bool tiles;         // mxfp4_tile.hip, else mxfp4_rows.hip
@@ -62,7 +76,7 @@ Way way_of(const mps_mxfp4_product *p) {
   w.x_rows = p->gather ? p->rows / p->top : p->rows;
   w.tiles = p->rows > 64 * (p->experts > 0 ? p->experts : 1);
   w.packed = p->x_type != MPS_TYPE_MXFP4 && p->k > 0 &&
-             !(w.tiles ? step_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
+             !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
   if (w.packed) w.workspace = w.x_rows * packed_width(p->k) * 2;
   return w;
 }
@@ -107,7 +121,7 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
     a.x = workspace, a.x_stride = width, a.k = width;
   }
   if (way.tiles)
-    launch_tiles(a, p->x_type, s);
+    launch_tiles(a, p->x_type, compute_units(), s);
   else
     launch_rows(a, p->x_type, s);
   MPS_HIP_CHECK(hipGetLastError());

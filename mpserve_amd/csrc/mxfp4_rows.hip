@@ -222,11 +222,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += from[4 * j];
     }
-    if (a.bias && !none) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < a.n) v[j] += load_as_float(a.bias, a.bias_type, (int64_t)tile.expert * a.n + col + j);
-    }
+    if (a.bias && !none) v += load_bias4(a, tile.expert, col);
     store4(a, row, col, v, quads);
   }
 }

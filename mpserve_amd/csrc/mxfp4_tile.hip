@@ -1,15 +1,19 @@
 // Products of many rows: tiles of BT rows of x times BN weight rows, with both operands' pieces of
 // k staged in LDS.
 //
-// A step covers 128 bytes of every row of x: 64 BF16 elements or 256 codes. The weights of a step
-// are 32 bytes a row beside BF16 x (written out as BF16 in registers, after LDS) and 128 beside
-// MXFP4 x, which the matrix cores multiply as it is. Pieces of 16 bytes go from memory to LDS
+// A step covers 128 bytes of every row of x, a cache line: 64 elements of 16 bits or 256 codes. The
+// weights of a step are 32 bytes a row beside 16-bit x (widened in registers, after LDS) and 128
+// beside MXFP4 x, which the matrix cores multiply as it is. Pieces of 16 bytes go from memory to LDS
 // without passing through registers; piece p of row r lies at place p ^ (r / 2 % 8) of its row's
-// eight, or p ^ (r / 8 % 2) of two, so that sixteen lanes reading one piece of sixteen rows meet
-// all 64 banks once (with r % 8, which serves eight lanes, half of all LDS cycles were conflicts). A lane of a
-// 32-row fragment reads four neighbouring pieces (one half of the row each for lanes 0-31 and
-// 32-63): k is summed in this order for both operands, so that a lane's four blocks have
-// neighbouring scale bytes.
+// eight, or p ^ (r / 8 % 2) of two: the sixteen lanes that LDS serves in a cycle (0-3, 12-15, 20-27
+// and 4-11, 16-19, 28-31, and so on) then meet all 64 banks once. With r % 8 half of LDS's cycles
+// were conflicts. (Stages of 64 bytes a row, four of them, halve the lines' use: 1177 us for 8192 x
+// 8192 x 28672 where these took 1030.)
+//
+// A step is multiplied in quarters, each from fragments read during the one before. Once the last
+// quarter's fragments are read nobody needs the buffer any more: the barrier stands there, the
+// loads of the step after next are issued behind it, and the next step's first fragments are read
+// while the last quarter is multiplied, so that the matrix cores do not wait for a new buffer.
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -24,23 +28,28 @@ __device__ inline f32x16 multiply4(i32x4 w, uint32_t ws, i32x4 x, uint32_t xs, f
 template <int XT, int BT, int BN, int WT, int WN>
 struct Shape {
   static constexpr bool k4 = XT == MPS_TYPE_MXFP4;
-  static constexpr int kThreads = WT * WN * 64;
-  static constexpr int kXPieces = 8, kWPieces = k4 ? 8 : 2;      // a row and step
-  static constexpr int kSteps = k4 ? 2 : 8;                      // steps that 16 scale bytes last
-  static constexpr int kScaleRows = k4 ? BT + BN : BN;           // x's rows, then the weight's
-  static constexpr int kXLoads = BT * kXPieces / kThreads;       // pieces a work-item and step
+  static constexpr int kWaves = WT * WN, kThreads = kWaves * 64;
+  static constexpr int kWPieces = k4 ? 8 : 2;                    // a weight row and step; x has 8
+  static constexpr int kXLoads = BT * 8 / kThreads;              // loads a wave and step, 64 pieces each
   static constexpr int kWLoads = (BN * kWPieces + kThreads - 1) / kThreads;
+  static constexpr int kWLanes = BN * kWPieces / kWaves < 64 ? BN * kWPieces / kWaves : 64;  // that load
+  static constexpr int kSteps = k4 ? 2 : 8;                      // steps a period of 16 blocks
+  static constexpr int kScaleRows = k4 ? BT + BN : BN;           // x's rows, then the weight's
+  static constexpr int kSLoads = (kScaleRows + kThreads - 1) / kThreads;
   static constexpr int kFT = BT / WT / 32, kFN = BN / WN / 32;   // 32 x 32 fragments of a wave
-  static_assert(BT * kXPieces % kThreads == 0 && kScaleRows <= kThreads, "");
+  static constexpr int kXBytes = BT * 128, kWBytes = BN * kWPieces * 16, kSBytes = kScaleRows * 16;
+  static constexpr int kPitch = kFN * 32 + 4;                    // floats of a row of sums, turned round
+  static constexpr int kStaged = 2 * (kXBytes + kWBytes + kSBytes), kTurned = kWaves * 32 * kPitch * 4;
+  static constexpr int kLds = kStaged > kTurned ? kStaged : kTurned;
+  static_assert(BT * 8 % kThreads == 0 && kThreads % 128 == 0 && kLds <= 160 * 1024, "");
 };
 
 template <int XT, int BT, int BN, int WT, int WN>
-__global__ __launch_bounds__(WT *WN * 64) void mxfp4_tile_kernel(ProductArgs a, int32_t tiles_t, int32_t tiles_n) {
+__global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_tile_kernel(ProductArgs a, int32_t tiles_t, int32_t tiles_n) {
   typedef Shape<XT, BT, BN, WT, WN> S;
   constexpr bool k4 = S::k4;
-  constexpr int kXBytes = BT * 128, kWBytes = BN * S::kWPieces * 16, kSBytes = S::kScaleRows * 16;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * (kXBytes + kWBytes + kSBytes)];
-  uint8_t *const xs = lds, *const ws = lds + 2 * kXBytes, *const ss = lds + 2 * (kXBytes + kWBytes);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLds];
+  uint8_t *const xs = lds, *const ws = lds + 2 * S::kXBytes, *const ss = ws + 2 * S::kWBytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, g = lane >> 5;
   const int wt = wave / WN, wn = wave % WN;
 
@@ -57,20 +66,21 @@ __global__ __launch_bounds__(WT *WN * 64) void mxfp4_tile_kernel(ProductArgs a, 
   if (a.offsets) tile = find_tile(a.offsets, a.experts, a.rows, BT, tile_t);
   if (tile.expert < 0) return;
   const bool none = tile.expert >= max(a.experts, 1);  // rows of no expert
-  const int32_t blocks = a.row_blocks;
-  const int32_t steps = none ? 0 : (blocks + (k4 ? 7 : 1)) / (k4 ? 8 : 2);
+  const int32_t blocks = a.row_blocks, periods = none ? 0 : (blocks + 15) / 16;
 
-  // Where this work-item's pieces come from. Rows past the tile's end or the weight's are read
-  // from the last one; what they give is not stored.
+  // Where this lane's pieces come from. Rows past the tile's end or the weight's are read from
+  // the last one (what they give is not stored), pieces past a row's end from its last one; their
+  // scales are zeros. MXFP4 x and the weights lie row by row, so an offset from the tile's
+  // first row, cut at the last, finds every piece; gathered rows need an address each.
   const int64_t x_row_bytes = k4 ? (int64_t)blocks * 16 : a.x_stride * 2;
-  const int64_t w_row_bytes = (int64_t)blocks * 16;
-  // MXFP4 x and the weights lie row by row, so an offset from the tile's first row, cut at the
-  // last, finds every piece; gathered rows need an address each.
-  const int xrow = tid / 8, wrow = tid / S::kWPieces;
-  const int32_t x_piece = (tid % 8) ^ (xrow >> 1 & 7), w_piece = k4 ? (tid % 8) ^ (wrow >> 1 & 7) : (tid % 2) ^ (wrow >> 3 & 1);
+  const uint32_t w_row_bytes = (uint32_t)blocks * 16;
+  const int w_at = wave * S::kWLanes + lane;  // of the first load's pieces
+  const int xrow = tid / 8, wrow = w_at / S::kWPieces;
+  const int32_t x_piece = (tid % 8) ^ (xrow >> 1 & 7);
+  const int32_t w_piece = k4 ? (w_at % 8) ^ (wrow >> 1 & 7) : (w_at % 2) ^ (wrow >> 3 & 1);
   const int64_t w_first = (int64_t)(none ? 0 : tile.expert) * a.n + n0;
   const uint8_t *const w_base = a.w + w_first * w_row_bytes;
-  const uint32_t w_last = (uint32_t)min(BN - 1, a.n - 1 - n0) * (uint32_t)w_row_bytes;
+  const uint32_t w_last = (uint32_t)min(BN - 1, a.n - 1 - n0) * w_row_bytes;
   const uint32_t x_last = (uint32_t)(tile.end - 1 - tile.first) * (uint32_t)x_row_bytes;
   const uint8_t *const x_base = static_cast<const uint8_t *>(a.x) + tile.first * x_row_bytes;
   const uint8_t *x_from[k4 ? 1 : S::kXLoads];
@@ -79,224 +89,243 @@ __global__ __launch_bounds__(WT *WN * 64) void mxfp4_tile_kernel(ProductArgs a, 
     for (int i = 0; i < S::kXLoads; ++i) {
       int32_t from = min(tile.first + xrow + i * (S::kThreads / 8), tile.end - 1);
       if (a.gather) from = min((uint32_t)a.order[from] / (uint32_t)a.top, (uint32_t)a.x_rows - 1);
-      x_from[i] = static_cast<const uint8_t *>(a.x) + from * x_row_bytes + x_piece * 16;
+      x_from[i] = static_cast<const uint8_t *>(a.x) + from * x_row_bytes;
     }
   }
-  const uint8_t *s_from = nullptr;
-  if (tid < S::kScaleRows) {
-    const int row = k4 ? tid - BT : tid;
+  const uint8_t *s_from[S::kSLoads];
+  const bool has_scales = S::kScaleRows % S::kThreads == 0 || tid < S::kScaleRows;
+#pragma unroll
+  for (int i = 0; i < S::kSLoads; ++i) {
+    const int at = tid + i * S::kThreads, row = k4 ? at - BT : at;
     if (k4 && row < 0)
-      s_from = a.x_scales + (int64_t)min(tile.first + tid, tile.end - 1) * blocks;
+      s_from[i] = a.x_scales + (int64_t)min(tile.first + at, tile.end - 1) * blocks;
     else
-      s_from = a.w_scales + (w_first + min(row, a.n - 1 - n0)) * blocks;
+      s_from[i] = a.w_scales + (w_first + min(min(row, BN - 1), a.n - 1 - n0)) * blocks;
   }
-
+  const int32_t x_pieces = k4 ? blocks : blocks * 4;
   auto fetch = [&](int32_t step, int buffer) {
-    if constexpr (k4) {
-      const uint32_t at = (uint32_t)min(step * 8 + x_piece, blocks - 1) * 16;
+    uint8_t *const xt = xs + buffer * S::kXBytes + wave * 1024, *const wt = ws + buffer * S::kWBytes + wave * S::kWLanes * 16;
+    const uint32_t x_at = (uint32_t)min(step * 8 + x_piece, x_pieces - 1) * 16;
 #pragma unroll
-      for (int i = 0; i < S::kXLoads; ++i)
-        copy16(x_base + (min((uint32_t)(xrow + i * (S::kThreads / 8)) * (uint32_t)x_row_bytes, x_last) + at),
-               xs + buffer * kXBytes + (i * S::kThreads + wave * 64) * 16);
-    } else {
-      const int64_t at = (int64_t)step * 128;
-#pragma unroll
-      for (int i = 0; i < S::kXLoads; ++i)
-        copy16(x_from[i] + at, xs + buffer * kXBytes + (i * S::kThreads + wave * 64) * 16);
+    for (int i = 0; i < S::kXLoads; ++i) {
+      if constexpr (k4)
+        copy16(x_base + (min((uint32_t)(xrow + i * (S::kThreads / 8)) * (uint32_t)x_row_bytes, x_last) + x_at), xt + i * S::kThreads * 16);
+      else
+        copy16(x_from[i] + x_at, xt + i * S::kThreads * 16);
     }
     const uint32_t at = (uint32_t)min(step * S::kWPieces + w_piece, blocks - 1) * 16;
+    if (S::kWLanes == 64 || lane < S::kWLanes) {
 #pragma unroll
-    for (int i = 0; i < S::kWLoads; ++i)
-      if (BN * S::kWPieces % S::kThreads == 0 || i * S::kThreads + wave * 64 < BN * S::kWPieces)
-        copy16(w_base + (min((uint32_t)(wrow + i * (S::kThreads / S::kWPieces)) * (uint32_t)w_row_bytes, w_last) + at),
-               ws + buffer * kWBytes + (i * S::kThreads + wave * 64) * 16);
+      for (int i = 0; i < S::kWLoads; ++i)
+        copy16(w_base + (min((uint32_t)(wrow + i * (S::kThreads / S::kWPieces)) * w_row_bytes, w_last) + at), wt + i * S::kThreads * 16);
+    }
   };
-  // The scales of a period (16 blocks) are fetched a period ahead.
-  auto put_scales = [&](u32x4 v, int buffer) {
-    if (s_from) *reinterpret_cast<u32x4 *>(ss + buffer * kSBytes + tid * 16) = v;
+  // Scales come 16 blocks at a time, a period ahead, through registers.
+  u32x4 scales[S::kSLoads];
+  auto get_scales = [&](int32_t period) {
+    if (has_scales) {
+#pragma unroll
+      for (int i = 0; i < S::kSLoads; ++i) scales[i] = load_scales(s_from[i], 16 * period, blocks);
+    }
+  };
+  auto put_scales = [&](int32_t period, int buffer) {
+    if (has_scales) {
+#pragma unroll
+      for (int i = 0; i < S::kSLoads; ++i)
+        *reinterpret_cast<u32x4 *>(ss + buffer * S::kSBytes + (tid + i * S::kThreads) * 16) = move_scales(scales[i], 16 * period, blocks);
+    }
   };
 
+  // Fragments of x by quarter. MXFP4: lanes 0-31 take the step's first four blocks of k, 32-63 the
+  // others, one a quarter, so that their scales are a word of neighbouring bytes. 16 bits: half a
+  // step is a block, of which lanes 0-31 take the first pieces of codes and 32-63 the others, and a quarter
+  // half of these.
+  constexpr int kBuffers = XT == MPS_TYPE_F16 ? 4 : 2;
+  u32x4 fx[kBuffers][S::kFT];
+  u32x4 fw4[2][k4 ? S::kFN : 1];               // MXFP4: by quarter
+  uint64_t fw[2][S::kFN];                      // 16 bits: by half
+  uint32_t sx[2][k4 ? S::kFT : 1], sw[2][S::kFN];  // scales: MXFP4 by step, 16 bits by half
   f32x16 acc[S::kFT][S::kFN] = {};
-  // Keeps the products of a step inside it: the compiler would read all fragments of a step first.
-  auto pin = [&]() {
+  const uint8_t *const xl = xs + (wt * S::kFT * 32 + r) * 128, *const wl = ws + (wn * S::kFN * 32 + r) * S::kWPieces * 16;
+  const uint8_t *const sl = ss + r * 16;
+  // Quarter q of the step in `buffer`, the in-th of its period.
+  auto read = [&](int q, int buffer, int in, int sbuf) {
+    const int at = ((k4 ? 4 * g + q : 4 * (q >> 1) + 2 * g + (q & 1)) ^ (r >> 1 & 7)) * 16;
+    if constexpr (k4) {
+#pragma unroll
+      for (int n = 0; n < S::kFN; ++n) fw4[q & 1][n] = *reinterpret_cast<const u32x4 *>(wl + buffer * S::kWBytes + n * 32 * 128 + at);
+      if (q == 0) {
+#pragma unroll
+        for (int t = 0; t < S::kFT; ++t)
+          sx[in & 1][t] = *reinterpret_cast<const uint32_t *>(sl + sbuf * S::kSBytes + (wt * S::kFT + t) * 32 * 16 + in * 8 + g * 4);
+#pragma unroll
+        for (int n = 0; n < S::kFN; ++n)
+          sw[in & 1][n] = *reinterpret_cast<const uint32_t *>(sl + sbuf * S::kSBytes + (BT + (wn * S::kFN + n) * 32) * 16 + in * 8 + g * 4);
+      }
+    } else if (q % 2 == 0) {
+#pragma unroll
+      for (int n = 0; n < S::kFN; ++n) {
+        fw[q >> 1][n] = *reinterpret_cast<const uint64_t *>(wl + buffer * S::kWBytes + n * 32 * 32 + ((q >> 1) ^ (r >> 3 & 1)) * 16 + g * 8);
+        sw[q >> 1][n] = sl[sbuf * S::kSBytes + (wn * S::kFN + n) * 32 * 16 + in * 2 + (q >> 1)];
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < S::kFT; ++t)
+      fx[q % kBuffers][t] = *reinterpret_cast<const u32x4 *>(xl + buffer * S::kXBytes + t * 32 * 128 + at);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](auto qc, int in, int from, int to) {
+    constexpr int q = decltype(qc)::value;
+#pragma unroll
+    for (int n = from; n < to; ++n) {
+      if constexpr (k4) {
+#pragma unroll
+        for (int t = 0; t < S::kFT; ++t)
+          acc[t][n] = multiply4<q>(__builtin_bit_cast(i32x4, fw4[q & 1][n]), sw[in & 1][n], __builtin_bit_cast(i32x4, fx[q % kBuffers][t]),
+                                   sx[in & 1][t], acc[t][n]);
+      } else if constexpr (XT == MPS_TYPE_BF16) {
+        const bf16x8 w = widen((uint32_t)(fw[q >> 1][n] >> (32 * (q & 1))), mx_scale(sw[q >> 1][n]));
+#pragma unroll
+        for (int t = 0; t < S::kFT; ++t)
+          acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, __builtin_bit_cast(bf16x8, fx[q % kBuffers][t]), acc[t][n], 0, 0, 0);
+      } else if constexpr (q % 2 == 1) {
+        // FP16: both quarters of a block, summed without the scale, which FP16 weights could not hold.
+        const f16x8 w0 = widen_f16((uint32_t)fw[q >> 1][n]), w1 = widen_f16((uint32_t)(fw[q >> 1][n] >> 32));
+        const float scale = mx_scale_value(sw[q >> 1][n]);
+#pragma unroll
+        for (int t = 0; t < S::kFT; ++t) {
+          f32x16 part = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fx[q - 1][t]), w0, f32x16{}, 0, 0, 0);
+          part = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fx[q][t]), w1, part, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
+        }
+      }
+    }
+    // The products stay where they are.
 #pragma unroll
     for (int t = 0; t < S::kFT; ++t)
 #pragma unroll
-      for (int n = 0; n < S::kFN; ++n) asm volatile("" : "+v"(acc[t][n]));
+      for (int n = from; n < to; ++n) asm volatile("" : "+v"(acc[t][n]));
+    __builtin_amdgcn_sched_barrier(0);
   };
-  const int32_t periods = (blocks + 15) / 16;
-  if (steps > 0) {
-    if (s_from) put_scales(move_scales(load_scales(s_from, 0, blocks), 0, blocks), 0);
+
+  if (periods > 0) {
     fetch(0, 0);
+    get_scales(0);
+    put_scales(0, 0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    fetch(1, 1);
+    read(0, 0, 0, 0);
+    if constexpr (XT == MPS_TYPE_F16) read(1, 0, 0, 0);
   }
-  if constexpr (k4) {
-    auto compute = [&](const uint8_t *xl, const uint8_t *wl, const uint8_t *sl) {
-      uint32_t sx[S::kFT], sw[S::kFN];
+  // 16 bits: steps past the last are left out, and so is a last block's other half; MXFP4 multiplies them
+  // by zero scales.
+  const int32_t halves = k4 ? 0 : blocks;
+  for (int32_t p = 0; p < periods; ++p) {
+    const int sbuf = p & 1;
+    if (p + 1 < periods) get_scales(p + 1);
+    for (int32_t pair = 0; pair < S::kSteps / 2; ++pair) {
 #pragma unroll
-      for (int t = 0; t < S::kFT; ++t)
-        sx[t] = *reinterpret_cast<const uint32_t *>(sl + (wt * S::kFT * 32 + t * 32 + r) * 16 + g * 4);
-#pragma unroll
-      for (int n = 0; n < S::kFN; ++n)
-        sw[n] = *reinterpret_cast<const uint32_t *>(sl + (BT + wn * S::kFN * 32 + n * 32 + r) * 16 + g * 4);
-      // The fragments of a quarter are read while the one before is multiplied.
-      i32x4 fx[2][S::kFT], fw[2][S::kFN];
-      auto read = [&](int j) {
-        const int at = ((4 * g + j) ^ (r >> 1 & 7)) * 16;
-#pragma unroll
-        for (int n = 0; n < S::kFN; ++n)
-          fw[j & 1][n] = *reinterpret_cast<const i32x4 *>(wl + (wn * S::kFN * 32 + n * 32 + r) * 128 + at);
-#pragma unroll
-        for (int t = 0; t < S::kFT; ++t)
-          fx[j & 1][t] = *reinterpret_cast<const i32x4 *>(xl + (wt * S::kFT * 32 + t * 32 + r) * 128 + at);
-      };
-      auto multiply = [&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-#pragma unroll
-        for (int t = 0; t < S::kFT; ++t)
-#pragma unroll
-          for (int n = 0; n < S::kFN; ++n) acc[t][n] = multiply4<j>(fw[j & 1][n], sw[n], fx[j & 1][t], sx[t], acc[t][n]);
-      };
-      read(0);
-      read(1);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(std::integral_constant<int, 0>{});
-      __builtin_amdgcn_sched_barrier(0);
-      read(2);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(std::integral_constant<int, 1>{});
-      __builtin_amdgcn_sched_barrier(0);
-      read(3);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(std::integral_constant<int, 2>{});
-      multiply(std::integral_constant<int, 3>{});
-      pin();
-    };
-    // Two steps a period; steps past the last block read zero scales and add nothing.
-    int sbuf = 0;
-    for (int32_t p = 0; p < (none ? 0 : periods); ++p) {
-      u32x4 scales = {0, 0, 0, 0};
-      __syncthreads();  // this step's pieces have landed, and nobody reads the other buffers any more
-      if (p + 1 < periods && s_from) scales = load_scales(s_from, 16 * (p + 1), blocks);
-      fetch(2 * p + 1, 1);
-      compute(xs, ws, ss + sbuf * kSBytes);
-      __syncthreads();
-      put_scales(move_scales(scales, 16 * (p + 1), blocks), sbuf ^ 1);
-      fetch(2 * p + 2, 0);
-      compute(xs + kXBytes, ws + kWBytes, ss + sbuf * kSBytes + 8);
-      sbuf ^= 1;
-    }
-  } else {
-    int32_t step = 0;
-    int sbuf = 0;
-    for (int32_t p = 0; p < (none ? 0 : periods); ++p) {
-      u32x4 scales = {0, 0, 0, 0};
-      const int32_t last = min(steps - p * S::kSteps, S::kSteps);
-      for (int32_t in = 0; in < last; ++in, ++step) {
-        const int buffer = step & 1;
-        __syncthreads();
-        if (in == 0 && s_from && p + 1 < periods) scales = load_scales(s_from, 16 * (p + 1), blocks);
-        if (in == last - 1) put_scales(move_scales(scales, 16 * (p + 1), blocks), sbuf ^ 1);
-        if (step + 1 < steps) fetch(step + 1, buffer ^ 1);
-        const uint8_t *xl = xs + buffer * kXBytes, *wl = ws + buffer * kWBytes, *sl = ss + sbuf * kSBytes + in * 2;
-        typedef typename std::conditional<XT == MPS_TYPE_F16, f16x8, bf16x8>::type x8;
-        auto read = [&](int piece, x8(&fx)[S::kFT]) {
-#pragma unroll
-          for (int t = 0; t < S::kFT; ++t)
-            fx[t] = *reinterpret_cast<const x8 *>(xl + (wt * S::kFT * 32 + t * 32 + r) * 128 + (piece ^ (r >> 1 & 7)) * 16);
+      for (int i = 0; i < 2; ++i) {
+        const int32_t in = 2 * pair + i, step = p * S::kSteps + in;
+        const bool has[2] = {k4 || 2 * step < halves, k4 || 2 * step + 1 < halves};
+        const int32_t next = in + 1 == S::kSteps ? 0 : in + 1;
+        const int next_sbuf = next == 0 ? sbuf ^ 1 : sbuf;
+        // The next fragments are read between the products of the weights' first fragment and the
+        // others': read before them all, they would be waited for together with these.
+        auto quarter = [&](auto qc) {
+          constexpr int q = decltype(qc)::value;
+          if (has[q >> 1]) multiply(qc, in, 0, 1);
+          if constexpr (q == 3) {
+            read(0, i ^ 1, next, next_sbuf);
+            if constexpr (XT == MPS_TYPE_F16) read(1, i ^ 1, next, next_sbuf);
+          } else if constexpr (XT == MPS_TYPE_F16) {
+            read(2, i, in, sbuf);
+            read(3, i, in, sbuf);
+          } else {
+            read(q + 1, i, in, sbuf);
+          }
+          if (has[q >> 1]) multiply(qc, in, 1, S::kFN);
         };
-        if constexpr (XT == MPS_TYPE_F16) {
-          // Lanes 0-31 have the first half of a block of k, lanes 32-63 the second.
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            x8 fx[2][S::kFT];
-            read(4 * b + 2 * g, fx[0]);
-            read(4 * b + 2 * g + 1, fx[1]);
-#pragma unroll
-            for (int n = 0; n < S::kFN; ++n) {
-              const int row = wn * S::kFN * 32 + n * 32 + r;
-              const uint64_t codes = *reinterpret_cast<const uint64_t *>(wl + row * 32 + (b ^ (r >> 3 & 1)) * 16 + g * 8);
-              const float scale = mx_scale_value(sl[row * 16 + b]);
-              const f16x8 w0 = widen_f16((uint32_t)codes), w1 = widen_f16((uint32_t)(codes >> 32));
-#pragma unroll
-              for (int t = 0; t < S::kFT; ++t) {
-                f32x16 part = __builtin_amdgcn_mfma_f32_32x32x16_f16(fx[0][t], w0, f32x16{}, 0, 0, 0);
-                part = __builtin_amdgcn_mfma_f32_32x32x16_f16(fx[1][t], w1, part, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
-              }
-            }
-          }
-        } else {
-          // Lanes 0-31 have the step's first block of k, lanes 32-63 the second.
-          u32x4 fw[S::kFN];
-          float sw[S::kFN];
-#pragma unroll
-          for (int n = 0; n < S::kFN; ++n) {
-            const int row = wn * S::kFN * 32 + n * 32 + r;
-            fw[n] = *reinterpret_cast<const u32x4 *>(wl + row * 32 + (g ^ (r >> 3 & 1)) * 16);
-            sw[n] = mx_scale(sl[row * 16 + g]);
-          }
-          x8 fx[2][S::kFT];
-          read(4 * g, fx[0]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j < 3) read(4 * g + j + 1, fx[(j + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int n = 0; n < S::kFN; ++n) {
-              const bf16x8 w = widen(fw[n][j], sw[n]);
-#pragma unroll
-              for (int t = 0; t < S::kFT; ++t)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, fx[j & 1][t], acc[t][n], 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-        pin();
+        if constexpr (XT != MPS_TYPE_F16) quarter(std::integral_constant<int, 0>{});
+        quarter(std::integral_constant<int, 1>{});
+        if constexpr (XT != MPS_TYPE_F16) quarter(std::integral_constant<int, 2>{});
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (in == S::kSteps - 2) put_scales(p + 1, sbuf ^ 1);
+        fetch(step + 2, i);
+        quarter(std::integral_constant<int, 3>{});
       }
-      sbuf ^= 1;
     }
   }
 
-  // A lane's 16 sums are places 8 i + 4 g .. + 3 of one side of a fragment, at place r of the other: columns
-  // of one row, or with FP16 x rows of one column. The wave turns 32 rows at a time round through its own
-  // part of LDS, so that stores go along the rows.
-  __syncthreads();
-  constexpr int kCols = S::kFN * 32, kPitch = kCols + 4, kLanes = kCols / 4;
-  static_assert(WT * WN * 32 * kPitch * 4 <= sizeof(lds), "");
-  float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kPitch;
-  const bool quads = a.n % 4 == 0 && aligned16(a.out);
-  const int32_t col = n0 + wn * kCols + lane % kLanes * 4;
-  float bias[4] = {0, 0, 0, 0};
-  if (a.bias && !none) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads of steps past the last
+  if constexpr (XT == MPS_TYPE_F16) {
+    // A lane's 16 sums are rows 8 i + 4 g .. + 3 of column r of a fragment. The wave turns 32 rows at a
+    // time round through its own part of LDS, so that stores go along the rows.
+    __syncthreads();
+    constexpr int kCols = S::kFN * 32, kPitch = S::kPitch, kLanes = kCols / 4;
+    float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kPitch;
+    const bool whole = a.n % 4 == 0 && aligned16(a.out);
+    const int32_t col = n0 + wn * kCols + lane % kLanes * 4;
+    f32x4 bias = {0, 0, 0, 0};
+    if (a.bias && !none) bias = load_bias4(a, tile.expert, col);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < a.n) bias[j] = load_as_float(a.bias, a.bias_type, (int64_t)tile.expert * a.n + col + j);
-  }
+    for (int t = 0; t < S::kFT; ++t) {
 #pragma unroll
-  for (int t = 0; t < S::kFT; ++t) {
+      for (int n = 0; n < S::kFN; ++n)
 #pragma unroll
-    for (int n = 0; n < S::kFN; ++n)
+        for (int i = 0; i < 16; ++i) mine[(8 * (i / 4) + 4 * g + i % 4) * kPitch + n * 32 + r] = acc[t][n][i];
+      __builtin_amdgcn_wave_barrier();
+      for (int in = lane / kLanes; in < 32; in += 64 / kLanes) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + in * kPitch + lane % kLanes * 4);
+        const int32_t row = tile.first + (wt * S::kFT + t) * 32 + in;
+        if (row < tile.end && col < a.n) store4(a, row, col, f32x4{v[0] + bias[0], v[1] + bias[1], v[2] + bias[2], v[3] + bias[3]}, whole);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  } else {
+    // A lane's 16 sums are columns 8 i + 4 g .. + 3 of row r of a fragment. For 16-bit outputs lanes r and
+    // r + 32 trade, so that each has eight neighbouring columns.
+    const bool whole = a.n % 8 == 0 && aligned16(a.out);
+    const bool wide = whole && a.out_type != MPS_TYPE_F32;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (XT == MPS_TYPE_F16) {
+    for (int n = 0; n < S::kFN; ++n) {
+      const int32_t col = n0 + (wn * S::kFN + n) * 32;
+      if (a.bias && !none) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mine[(8 * i + 4 * g + j) * kPitch + n * 32 + r] = acc[t][n][4 * i + j];
-        } else {
-          *reinterpret_cast<f32x4 *>(mine + r * kPitch + n * 32 + 8 * i + 4 * g) =
-              f32x4{acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]};
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 bias = load_bias4(a, tile.expert, col + 8 * i + 4 * g);
+#pragma unroll
+          for (int t = 0; t < S::kFT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[t][n][4 * i + j] += bias[j];
         }
       }
-    __builtin_amdgcn_wave_barrier();
-    const int32_t first = tile.first + (wt * S::kFT + t) * 32;
-    for (int row = lane / kLanes; row < 32; row += 64 / kLanes) {
-      f32x4 v = *reinterpret_cast<const f32x4 *>(mine + row * kPitch + lane % kLanes * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += bias[j];
-      if (first + row >= tile.end || col >= a.n) continue;
-      store4(a, first + row, col, v, quads);
+      for (int t = 0; t < S::kFT; ++t) {
+        const int32_t row = tile.first + (wt * S::kFT + t) * 32 + r;
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = pack2(acc[t][n][8 * i + 2 * j], acc[t][n][8 * i + 2 * j + 1], a.out_type);
+            const auto lo = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
+            const auto hi = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
+            const int32_t at = col + 16 * i + 8 * g;
+            if (row < tile.end && at < a.n)
+              *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (int64_t)row * a.n + at) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+          }
+        } else if (row < tile.end) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t at = col + 8 * i + 4 * g;
+            if (at < a.n)
+              store4(a, row, at, f32x4{acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]}, whole);
+          }
+        }
+      }
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -308,15 +337,65 @@ void launch(const ProductArgs &a, hipStream_t stream) {
                      (int32_t)tt, (int32_t)tn);
 }
 
+// The tile with the least predicted time. A CU works its tiles off two at a time (256 x 256: one);
+// `one` and `many` are the microseconds, at k = 4096, of a tile that has a CU to itself and of each of
+// several (measured: 128 x 8192 x 8192 and 1024 x 4096 x 4096 for the first, 4096 x 4096 x 14336 for
+// the second). So BF16 4096 x 4096 x 14336 takes 128 x 256 tiles, 398 us where 128 x 128 take 449,
+// and 128 x 8192 x 8192 takes 64 x 64, 52 us where 128 x 256 take 103. (BF16 in tiles of 256 x 256, one
+// workgroup of eight waves a CU: 417 us; MXFP4 in 128 x 256, 16 % slower than 256 x 256.)
+struct Choice {
+  int32_t bt, bn;
+  float one, many;
+};
+template <int N>
+int choose(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < N; ++i) {
+    const Choice &c = choices[i];
+    // Experts' ranges end in the middle of a tile, half of one each on the average.
+    const double tiles_t = a.offsets ? a.rows / (double)c.bt + 0.5 * (a.experts < a.rows ? a.experts : a.rows)
+                                     : (double)((a.rows + c.bt - 1) / c.bt);
+    const double tiles = tiles_t * (double)((a.n + c.bn - 1) / c.bn), each = tiles / cus;
+    const double time = each <= 1 ? c.one : (double)(int64_t)(each + 0.999) * c.many;
+    if (i == 0 || time < least) best = i, least = time;
+  }
+  return best;
+}
+
 }  // namespace
 
-void launch_tiles(const ProductArgs &a, int32_t x_type, hipStream_t stream) {
-  if (x_type == MPS_TYPE_MXFP4)
-    launch<MPS_TYPE_MXFP4, 256, 256, 2, 4>(a, stream);
-  else if (x_type == MPS_TYPE_BF16)
-    launch<MPS_TYPE_BF16, 256, 256, 2, 4>(a, stream);
-  else
-    launch<MPS_TYPE_F16, 256, 256, 2, 4>(a, stream);
+void launch_tiles(const ProductArgs &a, int32_t x_type, int32_t cus, hipStream_t stream) {
+  if (x_type == MPS_TYPE_MXFP4) {
+    const Choice choices[] = {{256, 256, 29.0f, 34.5f}, {128, 128, 14.0f, 10.9f}, {64, 64, 10.4f, 6.4f}};
+    const int c = choose(a, choices, cus);
+    if (c == 0)
+      launch<MPS_TYPE_MXFP4, 256, 256, 2, 4>(a, stream);
+    else if (c == 1)
+      launch<MPS_TYPE_MXFP4, 128, 128, 2, 2>(a, stream);
+    else
+      launch<MPS_TYPE_MXFP4, 64, 64, 2, 2>(a, stream);
+  } else if (x_type == MPS_TYPE_BF16) {
+    const Choice choices[] = {{128, 256, 56.0f, 57.0f}, {128, 128, 38.0f, 32.0f}, {64, 128, 28.0f, 20.5f}, {64, 64, 26.0f, 15.0f}};
+    const int c = choose(a, choices, cus);
+    if (c == 0)
+      launch<MPS_TYPE_BF16, 128, 256, 1, 4>(a, stream);
+    else if (c == 1)
+      launch<MPS_TYPE_BF16, 128, 128, 2, 2>(a, stream);
+    else if (c == 2)
+      launch<MPS_TYPE_BF16, 64, 128, 1, 4>(a, stream);
+    else
+      launch<MPS_TYPE_BF16, 64, 64, 2, 2>(a, stream);
+  } else {
+    const Choice choices[] = {{128, 128, 52.0f, 40.0f}, {64, 128, 35.0f, 23.0f}, {64, 64, 29.0f, 15.7f}};
+    const int c = choose(a, choices, cus);
+    if (c == 0)
+      launch<MPS_TYPE_F16, 128, 128, 1, 4>(a, stream);
+    else if (c == 1)
+      launch<MPS_TYPE_F16, 64, 128, 1, 4>(a, stream);
+    else
+      launch<MPS_TYPE_F16, 64, 64, 2, 2>(a, stream);
+  }
 }
 
 }  // namespace mps

@@ -141,6 +141,7 @@ EXPERT_CASES = [  # t, top, experts, k, n, dropped
     (1, 1, 1, 32, 16, 0.0), (1, 4, 64, 512, 100, 0.0), (4, 4, 64, 1024, 256, 0.2), (7, 2, 8, 100, 33, 0.3), (16, 2, 4, 160, 130, 0.0),
     (50, 4, 16, 1000, 77, 0.1), (64, 8, 128, 256, 64, 0.5), (300, 2, 4, 320, 257, 0.1), (500, 4, 8, 512, 384, 0.0),
     (1500, 6, 60, 288, 200, 0.05), (2000, 2, 3, 1056, 300, 0.0), (40, 1, 5, 64, 48, 1.0),
+    (3000, 4, 8, 96, 2100, 0.05), (9000, 2, 16, 544, 1500, 0.0),
 ]
 
 
