@@ -146,12 +146,30 @@ inline int64_t product_tiles(const ProductArgs &a, int64_t size) {
   return (a.rows + ranges * (size - 1)) / size;
 }
 
+// As many as there will be: experts' loads are unknown here, so pairs are taken to be spread evenly
+// at random; a range ends in the middle of a tile.
+inline double expected_tiles(const ProductArgs &a, int64_t size) {
+  if (!a.offsets) return (double)((a.rows + size - 1) / size);
+  const double met = a.experts * (1.0 - __builtin_exp(-(double)a.rows / a.experts));
+  const double tiles = (double)a.rows / size + 0.5 * met;
+  return tiles > met ? tiles : met;
+}
+
+// One of a kernel's shapes, and the microseconds that it is predicted to take (the launch and the first
+// loads, alike for all, are left out).
+struct Prediction {
+  int choice;
+  double us;
+};
+
 // Few rows (mxfp4_rows.hip). x is MXFP4, or 16-bit rows of whole 16-byte pieces.
-void launch_rows(const ProductArgs &a, int32_t x_type, hipStream_t stream);
+Prediction predict_rows(const ProductArgs &a, int32_t x_type, int32_t cus);
+void launch_rows(const ProductArgs &a, int32_t x_type, int choice, hipStream_t stream);
 inline bool piece_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 8 == 0; }
 
 // Many rows (mxfp4_tile.hip). x is MXFP4, or 16-bit rows of whole blocks at 16-byte addresses.
-void launch_tiles(const ProductArgs &a, int32_t x_type, int32_t cus, hipStream_t stream);
+Prediction predict_tiles(const ProductArgs &a, int32_t x_type, int32_t cus);
+void launch_tiles(const ProductArgs &a, int32_t x_type, int choice, hipStream_t stream);
 inline bool block_rows(const void *x, int64_t stride, int64_t k) { return aligned16(x) && stride % 8 == 0 && k % 32 == 0; }
 inline int64_t packed_width(int64_t k) { return (k + 31) / 32 * 32; }
 

@@ -67,17 +67,29 @@ int32_t compute_units() {
 
 // Which kernel takes a product, and what it needs.
 struct Way {
-  bool tiles;         // mxfp4_tile.hip, else mxfp4_rows.hip
-  bool packed;        // x is packed into the workspace first
-  int64_t x_rows, workspace;
+  ProductArgs args;
+  bool tiles;  // mxfp4_tile.hip, else mxfp4_rows.hip: the one predicted to be done earlier
+  int choice;
+  bool packed;  // x is packed into the workspace first
+  int64_t workspace;
 };
 Way way_of(const mps_mxfp4_product *p) {
   Way w = {};
-  w.x_rows = p->gather ? p->rows / p->top : p->rows;
-  w.tiles = p->rows > 64 * (p->experts > 0 ? p->experts : 1);
+  ProductArgs &a = w.args;
+  a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride;
+  a.w = p->w, a.w_scales = p->w_scales, a.bias = p->bias, a.out = p->out;
+  a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
+  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)(p->gather ? p->rows / p->top : p->rows);
+  a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
+  a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
+  a.bias_type = p->bias_type, a.out_type = p->out_type;
+  const int32_t cus = compute_units();
+  const Prediction rows = predict_rows(a, p->x_type, cus), tiles = predict_tiles(a, p->x_type, cus);
+  w.tiles = rows.choice < 0 || tiles.us < rows.us;
+  w.choice = w.tiles ? tiles.choice : rows.choice;
   w.packed = p->x_type != MPS_TYPE_MXFP4 && p->k > 0 &&
              !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
-  if (w.packed) w.workspace = w.x_rows * packed_width(p->k) * 2;
+  if (w.packed) w.workspace = a.x_rows * packed_width(p->k) * 2;
   return w;
 }
 
@@ -105,25 +117,19 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
   if (way.workspace > 0 && (!workspace || workspace_bytes < way.workspace || !aligned16(workspace)))
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: %lld bytes of workspace are needed, 16-byte aligned",
                 (long long)way.workspace);
-  ProductArgs a = {};
-  a.x = p->x, a.x_scales = p->x_scales, a.x_stride = p->x_stride;
-  a.w = p->w, a.w_scales = p->w_scales, a.bias = p->bias, a.out = p->out;
-  a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
-  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)way.x_rows, a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
-  a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
-  a.bias_type = p->bias_type, a.out_type = p->out_type;
+  ProductArgs a = way.args;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (way.packed) {
     const int32_t width = (int32_t)packed_width(p->k);
-    const dim3 grid((unsigned)((way.x_rows * (width / 8) + 255) / 256));
-    hipLaunchKernelGGL(mxfp4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), way.x_rows,
+    const dim3 grid((unsigned)(((int64_t)a.x_rows * (width / 8) + 255) / 256));
+    hipLaunchKernelGGL(mxfp4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), (int64_t)a.x_rows,
                        p->x_stride, a.k, width, static_cast<uint16_t *>(workspace));
     a.x = workspace, a.x_stride = width, a.k = width;
   }
   if (way.tiles)
-    launch_tiles(a, p->x_type, compute_units(), s);
+    launch_tiles(a, p->x_type, way.choice, s);
   else
-    launch_rows(a, p->x_type, s);
+    launch_rows(a, p->x_type, way.choice, s);
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
 }

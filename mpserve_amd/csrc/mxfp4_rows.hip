@@ -6,15 +6,18 @@
 // the oldest stage by the count of loads since, and multiplies it. At the end the waves' sums are
 // added up in wave order, so results do not depend on timing.
 //
-// A stage is 128 bytes of every row of x (64 elements of 16 bits, or 256 codes), in pieces of 16
-// bytes, piece p of row r at place p ^ (r / 2 % 8), and the weights of the same k: 32 bytes a row, or
-// 128 beside MXFP4 x (their two pieces at p ^ (r / 8 % 2), their eight as x's). In a lane 16 g + r of a 16-row fragment, MXFP4 takes pieces 2 g and 2 g + 1
-// of row r, and 16-bit x piece g of one block of k after the other.
+// A stage is U cache lines of every row of x (64 U elements of 16 bits, or 256 codes, U = 1) and the
+// weights of the same k, 32 U bytes a row, or 128 beside MXFP4 x: the more, the fewer instructions and
+// waits a byte (one token through 4096 x 14336: U = 1 9.1 us, U = 4 @U4@), the fewer, the more rows
+// of x fit. Pieces of 16 bytes lie in rows as in mxfp4_tile.hip: piece p of row r of x at place
+// p ^ (r / 2 % 8), of P pieces of a weight row at p ^ (r / (16 / P)).
+// In a lane 16 g + r of a 16-row fragment, MXFP4 takes pieces 2 g and 2 g + 1 of row r, and 16-bit x
+// piece g of one block of k after the other.
 //
 // FP16 x meets the codes' values in FP16, without their scale, which could leave FP16's range;
 // the products of a block are summed by themselves and added with the scale in FP32, exactly as
 // if it had been in the weight. (BF16 holds the scaled weight. FP16 as a sum of two BF16 took
-// twice the matrix instructions and 32 conversions a fragment: 31.7 us for 37 rows of 5000 x 3001.)
+// twice the matrix instructions and 32 conversions a fragment.)
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -25,23 +28,24 @@ __device__ inline void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <int XT, int XL, int FN, int W, int S>
+template <int XT, int XL, int FN, int U, int W, int S>
 struct Rows {
   static constexpr bool k4 = XT == MPS_TYPE_MXFP4;
   static constexpr int kRows = 8 * XL, kFT = XL < 2 ? 1 : XL / 2;  // rows of x; 16-row fragments
-  static constexpr int kBN = 16 * FN, kWPieces = k4 ? 8 : 2, kWL = kBN * kWPieces / 64;
-  static constexpr int kSteps = k4 ? 2 : 8;  // steps a period of 16 blocks
-  static constexpr int kXBytes = kFT * 16 * 128, kWBytes = kWL * 1024, kStage = kXBytes + kWBytes;
+  static constexpr int kBN = 16 * FN, kWPieces = k4 ? 8 : 2 * U, kWL = kBN * kWPieces / 64;
+  static constexpr int kSteps = k4 ? 2 : 8 / U;  // stages a period of 16 blocks
+  static constexpr int kLoads = XL * U + kWL;    // a stage
+  static constexpr int kLine = kRows * 128, kXBytes = U * kLine, kWBytes = kWL * 1024, kStage = kXBytes + kWBytes;
   static constexpr int kScaleRows = (k4 ? kRows : 0) + kBN, kSL = (kScaleRows + 63) / 64;
   static constexpr int kWave = S * kStage + kSL * 1024;  // LDS bytes of a wave
   static constexpr int kSums = W * kFT * FN * 1024;
   static constexpr int kLds = W * kWave > kSums ? W * kWave : kSums;
-  static_assert(kBN * kWPieces % 64 == 0 && kLds <= 160 * 1024 && (S - 1) * (XL + kWL) < 64, "");
+  static_assert(kBN * kWPieces % 64 == 0 && kLds <= 160 * 1024 && (S - 1) * kLoads < 64 && (!k4 || U == 1), "");
 };
 
-template <int XT, int XL, int FN, int W, int S>
+template <int XT, int XL, int FN, int U, int W, int S>
 __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
-  typedef Rows<XT, XL, FN, W, S> R;
+  typedef Rows<XT, XL, FN, U, W, S> R;
   constexpr bool k4 = R::k4;
   constexpr int kFT = R::kFT;
   __shared__ __attribute__((aligned(16))) uint8_t lds[R::kLds];
@@ -71,8 +75,9 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
     const int64_t w_first = (int64_t)tile.expert * a.n + n0;
     const uint8_t *const w_base = a.w + w_first * blocks * 16;
     const uint32_t w_row_bytes = (uint32_t)blocks * 16, w_last = (uint32_t)min(R::kBN - 1, a.n - 1 - n0) * w_row_bytes;
+    // A load has 64 / kWPieces weight rows; with 8 pieces a row, odd loads have the other half of the keys.
     const int wrow = lane / R::kWPieces;
-    const int32_t w_piece = k4 ? (lane % 8) ^ (wrow >> 1) : (lane % 2) ^ (wrow >> 3 & 1);
+    const int32_t w_piece = (lane % R::kWPieces) ^ (wrow % 16 / (16 / R::kWPieces));
     const uint8_t *s_from[R::kSL];
 #pragma unroll
     for (int i = 0; i < R::kSL; ++i) {
@@ -87,15 +92,17 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
     auto fetch = [&](int32_t item, int slot) {
       const int32_t step = period_of(item) * R::kSteps + item % R::kSteps;
       uint8_t *const to = mine + slot * R::kStage;
-      // Eight rows a load: rows of odd loads have the other half of the places' keys.
-      const int32_t x_at[2] = {min(step * 8 + x_piece, x_pieces - 1) * 16, min(step * 8 + (x_piece ^ 4), x_pieces - 1) * 16};
 #pragma unroll
-      for (int i = 0; i < XL; ++i) copy16(x_from[i] + x_at[i & 1], to + i * 1024);
+      for (int u = 0; u < U; ++u) {  // eight rows a load, so odd loads have the other half of the keys
+        const int32_t x_at[2] = {min((step * U + u) * 8 + x_piece, x_pieces - 1) * 16, min((step * U + u) * 8 + (x_piece ^ 4), x_pieces - 1) * 16};
+#pragma unroll
+        for (int i = 0; i < XL; ++i) copy16(x_from[i] + x_at[i & 1], to + u * R::kLine + i * 1024);
+      }
       const uint32_t w_at[2] = {(uint32_t)min(step * R::kWPieces + w_piece, blocks - 1) * 16,
                                 (uint32_t)min(step * R::kWPieces + (w_piece ^ 4), blocks - 1) * 16};
 #pragma unroll
       for (int i = 0; i < R::kWL; ++i)
-        copy16(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at[k4 ? i & 1 : 0]),
+        copy16(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at[R::kWPieces == 8 ? i & 1 : 0]),
                to + R::kXBytes + i * 1024);
     };
     u32x4 scales[R::kSL];
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
       }
       if (item + S - 1 < items) {
         fetch(item + S - 1, slot == 0 ? S - 1 : slot - 1);
-        wait_loads<(S - 1) * (XL + R::kWL)>();
+        wait_loads<(S - 1) * R::kLoads>();
       } else {
         wait_loads<0>();
       }
@@ -151,50 +158,61 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
         half(std::integral_constant<int, 0>{});
         half(std::integral_constant<int, 1>{});
       } else {
-        u32x4 fx[kFT][2];
-        uint32_t fw[FN][2], bytes[FN];
+        u32x4 fx[U][kFT][2];
+        uint32_t fw[U][FN][2];
+        uint64_t bytes[FN];
 #pragma unroll
         for (int n = 0; n < FN; ++n) {
-          bytes[n] = *reinterpret_cast<const uint16_t *>(ss + (n * 16 + r) * 16 + in * 2);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) fw[n][j] = *reinterpret_cast<const uint32_t *>(wl + (n * 16 + r) * 32 + (j ^ (r >> 3)) * 16 + g * 4);
+          const uint8_t *const at = ss + (n * 16 + r) * 16 + in * 2 * U;
+          bytes[n] = U == 4 ? *reinterpret_cast<const uint64_t *>(at) : U == 2 ? *reinterpret_cast<const uint32_t *>(at) : *reinterpret_cast<const uint16_t *>(at);
         }
 #pragma unroll
-        for (int t = 0; t < kFT; ++t)
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            fx[t][j] = *reinterpret_cast<const u32x4 *>(xl + (t * 16 + r) % R::kRows * 128 + ((4 * j + g) ^ (r >> 1)) * 16);
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int n = 0; n < FN; ++n)
+              fw[u][n][j] = *reinterpret_cast<const uint32_t *>(wl + (n * 16 + r) * R::kWPieces * 16 + ((2 * u + j) ^ (r / (16 / R::kWPieces))) * 16 + g * 4);
+#pragma unroll
+            for (int t = 0; t < kFT; ++t)
+              fx[u][t][j] = *reinterpret_cast<const u32x4 *>(xl + u * R::kLine + (t * 16 + r) % R::kRows * 128 + ((4 * j + g) ^ (r >> 1)) * 16);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
         // Pieces past the end of x's rows hold other elements: they are taken as zeros.
-        const int32_t left = a.k / 8 - (period_of(item) * R::kSteps + in) * 8;
-        if (left < 8) {
+        const int32_t left = a.k / 8 - (period_of(item) * R::kSteps + in) * 8 * U;
+        if (left < 8 * U) {
 #pragma unroll
-          for (int t = 0; t < kFT; ++t)
+          for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (4 * j + g >= left) fx[t][j] = u32x4{0, 0, 0, 0};
+            for (int t = 0; t < kFT; ++t)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (8 * u + 4 * j + g >= left) fx[u][t][j] = u32x4{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int n = 0; n < FN; ++n) {
-            const uint32_t byte = j ? bytes[n] >> 8 : bytes[n] & 255;
-            if constexpr (XT == MPS_TYPE_F16) {
-              const f16x8 w = widen_f16(fw[n][j]);
-              const float scale = mx_scale_value(byte);
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int t = 0; t < kFT; ++t) {
-                const f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fx[t][j]), w, f32x4{0, 0, 0, 0}, 0, 0, 0);
+            for (int n = 0; n < FN; ++n) {
+              const uint32_t byte = (uint32_t)(bytes[n] >> (16 * u + 8 * j)) & 255;
+              if constexpr (XT == MPS_TYPE_F16) {
+                const f16x8 w = widen_f16(fw[u][n][j]);
+                const float scale = mx_scale_value(byte);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
+                for (int t = 0; t < kFT; ++t) {
+                  const f32x4 part = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fx[u][t][j]), w, f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
+                }
+              } else {
+                const bf16x8 w = widen(fw[u][n][j], mx_scale(byte));
+#pragma unroll
+                for (int t = 0; t < kFT; ++t)
+                  acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fx[u][t][j]), w, acc[t][n], 0, 0, 0);
               }
-            } else {
-              const bf16x8 w = widen(fw[n][j], mx_scale(byte));
-#pragma unroll
-              for (int t = 0; t < kFT; ++t)
-                acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fx[t][j]), w, acc[t][n], 0, 0, 0);
             }
-          }
       }
       slot = slot == S - 1 ? 0 : slot + 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read: the next loads may take its place
@@ -227,48 +245,79 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
   }
 }
 
-template <int XT, int XL, int FN, int W, int S>
+template <int XT, int XL, int FN, int U, int W, int S>
 void launch(const ProductArgs &a, hipStream_t stream) {
-  typedef Rows<XT, XL, FN, W, S> R;
+  typedef Rows<XT, XL, FN, U, W, S> R;
   const dim3 grid((unsigned)((a.n + R::kBN - 1) / R::kBN), (unsigned)product_tiles(a, R::kRows));
-  hipLaunchKernelGGL((mxfp4_rows_kernel<XT, XL, FN, W, S>), grid, dim3(W * 64), 0, stream, a);
+  hipLaunchKernelGGL((mxfp4_rows_kernel<XT, XL, FN, U, W, S>), grid, dim3(W * 64), 0, stream, a);
 }
 
-// Rows of x a workgroup: enough for one pass over the weights, or (experts, whose rows are spread
-// unevenly) twice their share.
+// The shapes of a workgroup: 8 XL rows of x, 16 FN weight rows, U lines a stage, W waves, S stages. `resident`
+// of them fit a CU, and one takes `us` for each period of k (512 elements) that a wave has, as
+// measured with CUs full and half full (1 x 4096 x 14336, 16 x 4096 x 4096, 32 x 14336 x 4096, 64 x 8192 x
+// 8192, 64 x 4096 x 28672). More rows a workgroup spare reads of the weights, fewer fill more CUs, and more
+// waves share a long k: 64 x 8192 x 8192 in BF16 takes 16.9 us with XL 4, FN 4 and 37 with XL 1, FN 2, which
+// takes 7.5 for 1 x 4096 x 14336 where the first takes 10.0.
+struct Choice {
+  int32_t rows, cols, waves, resident;
+  float us;
+};
+constexpr Choice kChoices16[] = {{8, 32, 4, 2, 2.5f}, {8, 32, 8, 1, 2.7f}, {16, 32, 8, 1, 3.2f}, {16, 64, 4, 1, 2.8f},
+                                 {32, 32, 6, 1, 3.2f}, {32, 64, 4, 1, 3.8f}, {64, 64, 4, 1, 6.2f}};
+constexpr Choice kChoices4[] = {{8, 32, 4, 2, 1.9f}, {8, 32, 8, 1, 2.2f}, {16, 32, 4, 2, 1.9f}, {16, 32, 8, 1, 2.3f},
+                                {32, 64, 4, 1, 2.5f}, {64, 32, 6, 1, 2.7f}};
+
+template <int N>
+Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
+  Prediction best = {-1, 0};
+  const int64_t periods = (a.row_blocks + 15) / 16;
+  for (int i = 0; i < N; ++i) {
+    const Choice &c = choices[i];
+    if (product_tiles(a, c.rows) > 65535) continue;
+    const double each = expected_tiles(a, c.rows) * (double)((a.n + c.cols - 1) / c.cols) / ((double)cus * c.resident);
+    const double us = (each <= 1 ? 1.0 : __builtin_ceil(each - 0.01)) * (double)((periods + c.waves - 1) / c.waves) * c.us;
+    if (best.choice < 0 || us < best.us) best = {i, us};
+  }
+  return best;
+}
+
 template <int XT>
-void launch_type(const ProductArgs &a, hipStream_t stream) {
-  const int64_t rows = a.offsets ? 2 * (((int64_t)a.rows + a.experts - 1) / a.experts) : a.rows;
+void launch_type(const ProductArgs &a, int choice, hipStream_t stream) {
   if constexpr (XT == MPS_TYPE_MXFP4) {
-    if (rows <= 8)
-      launch<XT, 1, 2, 4, 4>(a, stream);
-    else if (rows <= 16)
-      launch<XT, 2, 2, 4, 3>(a, stream);
-    else if (rows <= 32)
-      launch<XT, 4, 2, 4, 4>(a, stream);
-    else
-      launch<XT, 8, 2, 4, 3>(a, stream);
+    switch (choice) {
+      case 0: return launch<XT, 1, 2, 1, 4, 3>(a, stream);
+      case 1: return launch<XT, 1, 2, 1, 8, 2>(a, stream);
+      case 2: return launch<XT, 2, 2, 1, 4, 3>(a, stream);
+      case 3: return launch<XT, 2, 2, 1, 8, 2>(a, stream);
+      case 4: return launch<XT, 4, 4, 1, 4, 2>(a, stream);
+      default: return launch<XT, 8, 2, 1, 6, 2>(a, stream);
+    }
   } else {
-    if (rows <= 8)
-      launch<XT, 1, 2, 8, 3>(a, stream);
-    else if (rows <= 16)
-      launch<XT, 2, 2, 8, 3>(a, stream);
-    else if (rows <= 32)
-      launch<XT, 4, 2, 8, 3>(a, stream);
-    else
-      launch<XT, 8, 2, 4, 3>(a, stream);
+    switch (choice) {
+      case 0: return launch<XT, 1, 2, 4, 4, 2>(a, stream);
+      case 1: return launch<XT, 1, 2, 4, 8, 2>(a, stream);
+      case 2: return launch<XT, 2, 2, 2, 8, 2>(a, stream);
+      case 3: return launch<XT, 2, 4, 4, 4, 2>(a, stream);
+      case 4: return launch<XT, 4, 2, 2, 6, 2>(a, stream);
+      case 5: return launch<XT, 4, 4, 2, 4, 3>(a, stream);
+      default: return launch<XT, 8, 4, 1, 4, 3>(a, stream);
+    }
   }
 }
 
 }  // namespace
 
-void launch_rows(const ProductArgs &a, int32_t x_type, hipStream_t stream) {
+Prediction predict_rows(const ProductArgs &a, int32_t x_type, int32_t cus) {
+  return x_type == MPS_TYPE_MXFP4 ? least(a, kChoices4, cus) : least(a, kChoices16, cus);
+}
+
+void launch_rows(const ProductArgs &a, int32_t x_type, int choice, hipStream_t stream) {
   if (x_type == MPS_TYPE_MXFP4)
-    launch_type<MPS_TYPE_MXFP4>(a, stream);
+    launch_type<MPS_TYPE_MXFP4>(a, choice, stream);
   else if (x_type == MPS_TYPE_BF16)
-    launch_type<MPS_TYPE_BF16>(a, stream);
+    launch_type<MPS_TYPE_BF16>(a, choice, stream);
   else
-    launch_type<MPS_TYPE_F16>(a, stream);
+    launch_type<MPS_TYPE_F16>(a, choice, stream);
 }
 
 }  // namespace mps

@@ -337,64 +337,58 @@ void launch(const ProductArgs &a, hipStream_t stream) {
                      (int32_t)tt, (int32_t)tn);
 }
 
-// The tile with the least predicted time. A CU works its tiles off two at a time (256 x 256: one);
-// `one` and `many` are the microseconds, at k = 4096, of a tile that has a CU to itself and of each of
-// several (measured: 128 x 8192 x 8192 and 1024 x 4096 x 4096 for the first, 4096 x 4096 x 14336 for
-// the second). So BF16 4096 x 4096 x 14336 takes 128 x 256 tiles, 398 us where 128 x 128 take 449,
-// and 128 x 8192 x 8192 takes 64 x 64, 52 us where 128 x 256 take 103. (BF16 in tiles of 256 x 256, one
+// The tiles. `one` and `many` are the microseconds, at k = 4096, of a tile that has a CU to itself and
+// of each of several (measured: 128 x 8192 x 8192 and 1024 x 4096 x 4096 for the first, 4096 x 4096 x
+// 14336 for the second). So BF16 4096 x 4096 x 14336 takes 128 x 256 tiles, 398 us where 128 x 128 take
+// 449, and 512 x 2048 x 1024 takes 64 x 64, 14 us where 128 x 256 take 30. (BF16 in tiles of 256 x 256, one
 // workgroup of eight waves a CU: 417 us; MXFP4 in 128 x 256, 16 % slower than 256 x 256.)
 struct Choice {
   int32_t bt, bn;
   float one, many;
 };
+constexpr Choice kChoices4[] = {{256, 256, 29.0f, 34.5f}, {128, 128, 14.0f, 10.9f}, {64, 64, 10.4f, 6.4f}};
+constexpr Choice kChoicesBf16[] = {{128, 256, 56.0f, 57.0f}, {128, 128, 38.0f, 32.0f}, {64, 128, 28.0f, 20.5f}, {64, 64, 26.0f, 15.0f}};
+constexpr Choice kChoicesF16[] = {{128, 128, 52.0f, 40.0f}, {64, 128, 35.0f, 23.0f}, {64, 64, 29.0f, 15.7f}};
+
 template <int N>
-int choose(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
-  int best = 0;
-  double least = 0;
+Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
+  Prediction best = {-1, 0};
   for (int i = 0; i < N; ++i) {
     const Choice &c = choices[i];
-    // Experts' ranges end in the middle of a tile, half of one each on the average.
-    const double tiles_t = a.offsets ? a.rows / (double)c.bt + 0.5 * (a.experts < a.rows ? a.experts : a.rows)
-                                     : (double)((a.rows + c.bt - 1) / c.bt);
-    const double tiles = tiles_t * (double)((a.n + c.bn - 1) / c.bn), each = tiles / cus;
-    const double time = each <= 1 ? c.one : (double)(int64_t)(each + 0.999) * c.many;
-    if (i == 0 || time < least) best = i, least = time;
+    const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn), each = __builtin_ceil(tiles / cus - 0.01);
+    const double us = (each <= 1 ? c.one : each * c.many) * a.row_blocks / 128;
+    if (best.choice < 0 || us < best.us) best = {i, us};
   }
   return best;
 }
 
 }  // namespace
 
-void launch_tiles(const ProductArgs &a, int32_t x_type, int32_t cus, hipStream_t stream) {
+Prediction predict_tiles(const ProductArgs &a, int32_t x_type, int32_t cus) {
+  if (x_type == MPS_TYPE_MXFP4) return least(a, kChoices4, cus);
+  return x_type == MPS_TYPE_BF16 ? least(a, kChoicesBf16, cus) : least(a, kChoicesF16, cus);
+}
+
+void launch_tiles(const ProductArgs &a, int32_t x_type, int choice, hipStream_t stream) {
   if (x_type == MPS_TYPE_MXFP4) {
-    const Choice choices[] = {{256, 256, 29.0f, 34.5f}, {128, 128, 14.0f, 10.9f}, {64, 64, 10.4f, 6.4f}};
-    const int c = choose(a, choices, cus);
-    if (c == 0)
-      launch<MPS_TYPE_MXFP4, 256, 256, 2, 4>(a, stream);
-    else if (c == 1)
-      launch<MPS_TYPE_MXFP4, 128, 128, 2, 2>(a, stream);
-    else
-      launch<MPS_TYPE_MXFP4, 64, 64, 2, 2>(a, stream);
-  } else if (x_type == MPS_TYPE_BF16) {
-    const Choice choices[] = {{128, 256, 56.0f, 57.0f}, {128, 128, 38.0f, 32.0f}, {64, 128, 28.0f, 20.5f}, {64, 64, 26.0f, 15.0f}};
-    const int c = choose(a, choices, cus);
-    if (c == 0)
-      launch<MPS_TYPE_BF16, 128, 256, 1, 4>(a, stream);
-    else if (c == 1)
-      launch<MPS_TYPE_BF16, 128, 128, 2, 2>(a, stream);
-    else if (c == 2)
-      launch<MPS_TYPE_BF16, 64, 128, 1, 4>(a, stream);
-    else
-      launch<MPS_TYPE_BF16, 64, 64, 2, 2>(a, stream);
-  } else {
-    const Choice choices[] = {{128, 128, 52.0f, 40.0f}, {64, 128, 35.0f, 23.0f}, {64, 64, 29.0f, 15.7f}};
-    const int c = choose(a, choices, cus);
-    if (c == 0)
-      launch<MPS_TYPE_F16, 128, 128, 1, 4>(a, stream);
-    else if (c == 1)
-      launch<MPS_TYPE_F16, 64, 128, 1, 4>(a, stream);
-    else
-      launch<MPS_TYPE_F16, 64, 64, 2, 2>(a, stream);
+    switch (choice) {
+      case 0: return launch<MPS_TYPE_MXFP4, 256, 256, 2, 4>(a, stream);
+      case 1: return launch<MPS_TYPE_MXFP4, 128, 128, 2, 2>(a, stream);
+      default: return launch<MPS_TYPE_MXFP4, 64, 64, 2, 2>(a, stream);
+    }
+  }
+  if (x_type == MPS_TYPE_BF16) {
+    switch (choice) {
+      case 0: return launch<MPS_TYPE_BF16, 128, 256, 1, 4>(a, stream);
+      case 1: return launch<MPS_TYPE_BF16, 128, 128, 2, 2>(a, stream);
+      case 2: return launch<MPS_TYPE_BF16, 64, 128, 1, 4>(a, stream);
+      default: return launch<MPS_TYPE_BF16, 64, 64, 2, 2>(a, stream);
+    }
+  }
+  switch (choice) {
+    case 0: return launch<MPS_TYPE_F16, 128, 128, 1, 4>(a, stream);
+    case 1: return launch<MPS_TYPE_F16, 64, 128, 1, 4>(a, stream);
+    default: return launch<MPS_TYPE_F16, 64, 64, 2, 2>(a, stream);
   }
 }
 

@@ -113,6 +113,9 @@ SHAPES = [  # t, k, n
     (16, 1000, 48), (17, 288, 257), (31, 64, 128), (33, 544, 31), (48, 2080, 300), (64, 128, 512), (65, 512, 130),
     (100, 5000, 77), (127, 736, 255), (128, 1024, 256), (130, 96, 1), (200, 1056, 513), (256, 256, 1024),
     (257, 320, 769), (300, 1500, 260), (512, 2048, 520), (1030, 672, 384),
+    # sizes at which each shape of a workgroup for few rows is the one that is taken
+    (1, 1030, 16), (130, 1030, 1030), (130, 2056, 520), (500, 1030, 520), (50, 2056, 2100), (500, 1030, 1030),
+    (130, 500, 1030), (500, 500, 520), (70, 500, 20000), (1, 500, 20000), (60, 320, 100),
     # enough tiles for each of the larger ones, ends of rows and columns inside them, one block to several periods of k
     (700, 96, 4300), (1100, 64, 8300), (2100, 32, 8300), (2300, 704, 8500), (4500, 160, 5000), (9000, 544, 2100),
 ]
