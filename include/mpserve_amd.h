@@ -368,10 +368,10 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *product, void *workspace, int64_
 int mps_expert_sort_workspace(int64_t tokens, int64_t top, int64_t experts, int64_t *bytes);
 int mps_expert_sort(const void *ids, int32_t ids_64, int64_t tokens, int64_t top, int64_t experts, int32_t *order,
                     int32_t *positions, int32_t *offsets, void *workspace, int64_t workspace_bytes, void *stream);
-/* rows[tokens * top, width]: row j is x's row order[j] / top; rows from
- * offsets[experts] on are zero. */
+/* rows[tokens * top, width]: x's row t at the place of each of its pairs; rows
+ * from offsets[experts] on are zero. */
 int mps_expert_gather(const void *x, int32_t type, int64_t tokens, int64_t top, int64_t experts, int64_t width,
-                      const int32_t *order, const int32_t *offsets, void *rows, void *stream);
+                      const int32_t *order, const int32_t *positions, const int32_t *offsets, void *rows, void *stream);
 /* out[tokens, width]: row t is the sum over its pairs' places p of
  * weights[pair] * y[p] (weights NULL: of y[p]), in FP32 and in the pairs'
  * order, without the pairs of no expert. Also the gradient of the gather. */
@@ -382,7 +382,7 @@ int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t
  * pairs of no expert. */
 int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const void *weights, int32_t weights_type,
                             int64_t tokens, int64_t top, int64_t experts, int64_t width, const int32_t *order,
-                            const int32_t *offsets, void *dy, void *dweights, void *stream);
+                            const int32_t *positions, const int32_t *offsets, void *dy, void *dweights, void *stream);
 
 #ifdef __cplusplus
 }

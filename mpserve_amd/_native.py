@@ -144,9 +144,9 @@ def lib():
     L.mps_mxfp4_multiply.argtypes = [ctypes.POINTER(MpsMxfp4Product), _p, _i64, _p]
     L.mps_expert_sort_workspace.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
     L.mps_expert_sort.argtypes = [_p, i32, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]
-    L.mps_expert_gather.argtypes = [_p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p]
+    L.mps_expert_gather.argtypes = [_p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p]
     L.mps_expert_combine.argtypes = [_p, i32, _p, i32, _i64, _i64, _i64, _p, _p, _p]
-    L.mps_expert_combine_grad.argtypes = [_p, _p, i32, _p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p]
+    L.mps_expert_combine_grad.argtypes = [_p, _p, i32, _p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]
     for name in ("mps_mxfp4_quantize", "mps_mxfp4_dequantize", "mps_mxfp4_product_workspace", "mps_mxfp4_multiply",
                  "mps_expert_sort_workspace", "mps_expert_sort", "mps_expert_gather", "mps_expert_combine",
                  "mps_expert_combine_grad"):

@@ -21,7 +21,7 @@ __device__ inline int32_t expert_of(const Id *ids, int64_t i, int32_t experts) {
 
 // Up to kOneWorkgroup pairs are sorted by one workgroup; more in chunks, a workgroup each, of which
 // each counts its pairs first, in a launch of its own. (65536 pairs of 128 experts: 78 us by one
-// workgroup, @CHUNKS@ in chunks.)
+// workgroup, 13 in chunks.)
 constexpr int32_t kOneWorkgroup = 4096, kMostChunks = 64;
 inline int32_t sort_chunk(int64_t pairs) {
   const int64_t chunk = (pairs + kMostChunks - 1) / kMostChunks;
@@ -130,89 +130,216 @@ __global__ __launch_bounds__(kSortThreads) void expert_sort_kernel(const Id *__r
   }
 }
 
-constexpr int kRowThreads = 256;
+// Rows are worked off in pieces of 16 bytes, at any alignment; the last piece of a row may be a part
+// of one. A token's pieces are shared out to a power of two of work-items (`lanes`, at most the
+// workgroup), so that narrow rows share a workgroup. A token's row is read once for all its pairs: gathered by
+// place instead, rows of x came from beyond the L2 once a pair (8192 tokens x 4096 BF16, 8 of 128 experts:
+// 171 us, by token 100).
+constexpr int kRowThreads = 256, kPairs = 4;  // pairs whose pieces are in flight together
 
-// kVec elements at a time: 16 bytes where rows are whole 16-byte pieces, else one.
-template <int T, int kVec>
+template <int T>
 struct Piece {
-  typename Elem<T>::raw v[kVec];
+  typedef typename Elem<T>::raw raw;
+  static constexpr int kVec = 16 / sizeof(raw);
+  u32x4 bits = {0, 0, 0, 0};
+
+  __device__ float get(int i) const {
+    if constexpr (T == MPS_TYPE_F32)
+      return __uint_as_float(bits[i]);
+    else
+      return Elem<T>::get((uint16_t)(bits[i / 2] >> (16 * (i % 2))));
+  }
+  __device__ void put(int i, float f) {
+    if constexpr (T == MPS_TYPE_F32)
+      bits[i] = __float_as_uint(f);
+    else
+      bits[i / 2] |= (uint32_t)Elem<T>::put(f) << (16 * (i % 2));
+  }
+  static __device__ Piece load(const raw *row, int64_t col, int64_t width) {
+    Piece p;
+    if (col + kVec <= width) {
+      p.bits = *reinterpret_cast<const u32x4_any *>(row + col);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (col + i < width) p.put(i, Elem<T>::get(row[col + i]));
+    }
+    return p;
+  }
+  __device__ void store(raw *row, int64_t col, int64_t width) const {
+    if (col + kVec <= width) {
+      *reinterpret_cast<u32x4_any *>(row + col) = bits;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (col + i < width) {
+          if constexpr (T == MPS_TYPE_F32)
+            row[col + i] = __uint_as_float(bits[i]);
+          else
+            row[col + i] = (uint16_t)(bits[i / 2] >> (16 * (i % 2)));
+        }
+    }
+  }
 };
 
-template <int T, int kVec>
-__global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(const typename Elem<T>::raw *__restrict__ x,
-                                                                    int32_t tokens, int32_t top, int64_t pairs,
-                                                                    int32_t experts, int64_t width,
-                                                                    const int32_t *__restrict__ order,
-                                                                    const int32_t *__restrict__ offsets,
-                                                                    typename Elem<T>::raw *__restrict__ rows) {
-  typedef Piece<T, kVec> P;
-  const int64_t j = blockIdx.x;
-  const bool there = j < offsets[experts];
-  const int32_t token = min((uint32_t)order[j] / (uint32_t)top, (uint32_t)tokens - 1);
-  const P *src = reinterpret_cast<const P *>(x + (int64_t)token * width);
-  P *dst = reinterpret_cast<P *>(rows + j * width);
-  const P zero = {};
-  for (int64_t c = threadIdx.x; c < width / kVec; c += kRowThreads) dst[c] = there ? src[c] : zero;
+struct RowArgs {
+  const void *in, *dout, *weights;  // x or y
+  void *out, *dweights;
+  const int32_t *order, *positions, *offsets;
+  int64_t tokens, top, pairs, width;
+  int32_t experts, weights_type, lanes;
+};
+
+// The places of pairs of no expert, and the rows there: zeros. Workgroups past the tokens' take them in turn.
+template <int T>
+__device__ inline void zero_rows(const RowArgs &a, int64_t block, int64_t blocks, bool weights) {
+  typedef Piece<T> P;
+  const int64_t first = min(max((int64_t)a.offsets[a.experts], (int64_t)0), a.pairs);
+  for (int64_t j = first + block; j < a.pairs; j += blocks) {
+    for (int64_t col = threadIdx.x * P::kVec; col < a.width; col += kRowThreads * P::kVec)
+      P{}.store(static_cast<typename Elem<T>::raw *>(a.out) + j * a.width, col, a.width);
+    if (weights && threadIdx.x == 0) {
+      const int64_t pair = a.order[j];
+      if (pair >= 0 && pair < a.pairs) store_as(a.dweights, a.weights_type, pair, 0.0f);
+    }
+  }
+}
+constexpr int kZeroBlocks = 128;
+
+template <int T, bool kWide>
+__global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(RowArgs a, int64_t token_blocks) {
+  typedef Piece<T> P;
+  typedef typename Elem<T>::raw raw;
+  if (blockIdx.x >= token_blocks) return zero_rows<T>(a, blockIdx.x - token_blocks, kZeroBlocks, false);
+  const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
+  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
+  if (t >= a.tokens) return;
+  const raw *const row = static_cast<const raw *>(a.in) + t * a.width;
+  raw *const out = static_cast<raw *>(a.out);
+  for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+    const P p = P::load(row, col, a.width);
+    for (int64_t i = 0; i < a.top; ++i) {
+      const int32_t at = a.positions[t * a.top + i];
+      if (at >= 0 && at < a.pairs) p.store(out + at * a.width, col, a.width);
+    }
+  }
 }
 
-template <int T, int kVec>
-__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(const typename Elem<T>::raw *__restrict__ y,
-                                                                     const void *__restrict__ weights, int32_t wtype,
-                                                                     int32_t top, int64_t pairs, int64_t width,
+// (The pointers stand by themselves so that the compiler may take them to be apart, and loads of the places
+// and weights, alike for all lanes, to be scalar.)
+template <int T, bool kWide>
+__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(RowArgs a, const typename Elem<T>::raw *__restrict__ y,
+                                                                     const void *__restrict__ weights,
                                                                      const int32_t *__restrict__ positions,
                                                                      typename Elem<T>::raw *__restrict__ out) {
-  typedef Piece<T, kVec> P;
-  const int64_t t = blockIdx.x;
-  for (int64_t c = threadIdx.x; c < width / kVec; c += kRowThreads) {
-    float sum[kVec] = {};
-    for (int32_t i = 0; i < top; ++i) {
-      const int64_t pair = t * top + i;
-      const int32_t at = positions[pair];
-      if (at < 0 || at >= pairs) continue;
-      const float w = weights ? load_as_float(weights, wtype, pair) : 1.0f;
-      const P p = reinterpret_cast<const P *>(y + (int64_t)at * width)[c];
-      for (int v = 0; v < kVec; ++v) sum[v] += w * Elem<T>::get(p.v[v]);
+  typedef Piece<T> P;
+  const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
+  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
+  if (t >= a.tokens) return;
+  for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+    const bool whole = col + P::kVec <= a.width;
+    float sum[P::kVec] = {};
+    for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
+      // Whole pieces without branches, so that their loads are in flight together: an absent pair reads row 0.
+      int64_t at[kPairs];
+      bool there[kPairs];
+      float w[kPairs];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const int64_t in = i0 + i < a.top ? i0 + i : 0;
+        const int32_t p = positions[t * a.top + in];
+        there[i] = i0 + i < a.top && p >= 0 && p < a.pairs;
+        at[i] = there[i] ? p : 0;
+        w[i] = 1.0f;
+      }
+      if (weights) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) w[i] = load_as_float(weights, a.weights_type, t * a.top + (i0 + i < a.top ? i0 + i : 0));
+      }
+      P p[kPairs];
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) p[i].bits = *reinterpret_cast<const u32x4_any *>(y + at[i] * a.width + col);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) p[i] = P::load(y + at[i] * a.width, col, a.width);
+      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+        for (int v = 0; v < P::kVec; ++v) sum[v] = there[i] ? __builtin_fmaf(w[i], p[i].get(v), sum[v]) : sum[v];
     }
     P o;
-    for (int v = 0; v < kVec; ++v) o.v[v] = Elem<T>::put(sum[v]);
-    reinterpret_cast<P *>(out + t * width)[c] = o;
+#pragma unroll
+    for (int v = 0; v < P::kVec; ++v) o.put(v, sum[v]);
+    o.store(out + t * a.width, col, a.width);
   }
 }
 
-// A workgroup a sorted row; the lanes' products are added up by a tree, whose order is fixed.
-template <int T, int kVec>
-__global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(
-    const typename Elem<T>::raw *__restrict__ y, const typename Elem<T>::raw *__restrict__ dout,
-    const void *__restrict__ weights, int32_t wtype, int32_t tokens, int32_t top, int64_t pairs, int32_t experts,
-    int64_t width, const int32_t *__restrict__ order, const int32_t *__restrict__ offsets,
-    typename Elem<T>::raw *__restrict__ dy, void *__restrict__ dweights) {
-  typedef Piece<T, kVec> P;
-  __shared__ float parts[kRowThreads / 64];
-  const int64_t j = blockIdx.x;
-  const bool there = j < offsets[experts];
-  const uint32_t pair = min((uint32_t)order[j], (uint32_t)(pairs - 1)), token = pair / (uint32_t)top;
-  const float w = load_as_float(weights, wtype, pair);
-  float dot = 0;
-  for (int64_t c = threadIdx.x; c < width / kVec; c += kRowThreads) {
-    P o = {};
-    if (there) {
-      const P g = reinterpret_cast<const P *>(dout + (int64_t)token * width)[c];
-      const P p = reinterpret_cast<const P *>(y + j * width)[c];
-      for (int v = 0; v < kVec; ++v) {
-        const float gv = Elem<T>::get(g.v[v]);
-        dot += gv * Elem<T>::get(p.v[v]);
-        o.v[v] = Elem<T>::put(w * gv);
-      }
+// kPairs pairs of a token at a time. A work-item's products are added up in the order of its pieces, and
+// the work-items' sums by a tree: a fixed order.
+template <int T, bool kWide>
+__global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(RowArgs a, int64_t token_blocks) {
+  typedef Piece<T> P;
+  typedef typename Elem<T>::raw raw;
+  __shared__ float parts[kPairs][kRowThreads / 64];
+  if (blockIdx.x >= token_blocks) return zero_rows<T>(a, blockIdx.x - token_blocks, kZeroBlocks, true);
+  const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
+  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
+  const bool token = t < a.tokens;
+  const raw *const y = static_cast<const raw *>(a.in), *const g = static_cast<const raw *>(a.dout) + (token ? t : 0) * a.width;
+  raw *const dy = static_cast<raw *>(a.out);
+  for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
+    float w[kPairs], dot[kPairs] = {};
+    int64_t at[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const int64_t pair = t * a.top + i0 + i;
+      at[i] = token && i0 + i < a.top ? a.positions[pair] : -1;
+      if (at[i] >= a.pairs) at[i] = -1;
+      w[i] = at[i] >= 0 ? load_as_float(a.weights, a.weights_type, pair) : 0.0f;
     }
-    reinterpret_cast<P *>(dy + j * width)[c] = o;
-  }
-  for (int d = 32; d > 0; d /= 2) dot += __shfl_xor(dot, d);
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = dot;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float sum = 0;
-    for (int i = 0; i < kRowThreads / 64; ++i) sum += parts[i];
-    store_as(dweights, wtype, pair, there ? sum : 0.0f);
+    if (token)
+      for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+        const P d = P::load(g, col, a.width);
+        P p[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (at[i] >= 0) p[i] = P::load(y + at[i] * a.width, col, a.width);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (at[i] >= 0) {
+            P o;
+#pragma unroll
+            for (int v = 0; v < P::kVec; ++v) {
+              const float gv = d.get(v);
+              dot[i] += gv * p[i].get(v);
+              o.put(v, w[i] * gv);
+            }
+            o.store(dy + at[i] * a.width, col, a.width);
+          }
+      }
+    const int in_wave = lanes < 64 ? lanes : 64;
+    for (int d = in_wave / 2; d > 0; d /= 2)
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) dot[i] += __shfl_xor(dot[i], d);
+    if (lanes > 64) {
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) parts[i][threadIdx.x >> 6] = dot[i];
+      __syncthreads();
+      const int first = threadIdx.x / lanes * (lanes / 64);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        dot[i] = 0;
+        for (int j = 0; j < lanes / 64; ++j) dot[i] += parts[i][first + j];
+      }
+      __syncthreads();
+    }
+    if ((threadIdx.x & (lanes - 1)) == 0)
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i)
+        if (at[i] >= 0) store_as(a.dweights, a.weights_type, t * a.top + i0 + i, dot[i]);
   }
 }
 
@@ -237,21 +364,22 @@ int check_sizes(const char *what, int64_t tokens, int64_t top, int64_t experts) 
   return MPS_OK;
 }
 
-// 16-byte pieces where every row starts at a 16-byte address.
-template <typename... Ptr>
-bool whole_rows(int64_t width, int32_t type, Ptr... p) {
-  return width * type_bytes(type) % 16 == 0 && (aligned16(p) && ...);
+int32_t lanes_of(int64_t width, int32_t type) {
+  const int64_t pieces = (width * type_bytes(type) + 15) / 16;
+  int32_t lanes = 1;
+  while (lanes < kRowThreads && lanes < pieces) lanes *= 2;
+  return lanes;
 }
 
-#define MPS_BY_TYPE(type, whole, CALL)                                  \
-  do {                                                                  \
-    if ((type) == MPS_TYPE_F32) {                                       \
-      if (whole) { CALL(MPS_TYPE_F32, 4); } else { CALL(MPS_TYPE_F32, 1); }     \
-    } else if ((type) == MPS_TYPE_BF16) {                               \
-      if (whole) { CALL(MPS_TYPE_BF16, 8); } else { CALL(MPS_TYPE_BF16, 1); }   \
-    } else {                                                            \
-      if (whole) { CALL(MPS_TYPE_F16, 8); } else { CALL(MPS_TYPE_F16, 1); }     \
-    }                                                                   \
+#define MPS_BY_TYPE(type, wide, CALL)                                                       \
+  do {                                                                                      \
+    if ((type) == MPS_TYPE_F32) {                                                           \
+      if (wide) { CALL(MPS_TYPE_F32, true); } else { CALL(MPS_TYPE_F32, false); }           \
+    } else if ((type) == MPS_TYPE_BF16) {                                                   \
+      if (wide) { CALL(MPS_TYPE_BF16, true); } else { CALL(MPS_TYPE_BF16, false); }         \
+    } else {                                                                                \
+      if (wide) { CALL(MPS_TYPE_F16, true); } else { CALL(MPS_TYPE_F16, false); }           \
+    }                                                                                       \
   } while (0)
 
 }  // namespace
@@ -294,20 +422,22 @@ int mps_expert_sort(const void *ids, int32_t ids_64, int64_t tokens, int64_t top
 }
 
 int mps_expert_gather(const void *x, int32_t type, int64_t tokens, int64_t top, int64_t experts, int64_t width,
-                      const int32_t *order, const int32_t *offsets, void *rows, void *stream) {
+                      const int32_t *order, const int32_t *positions, const int32_t *offsets, void *rows, void *stream) {
   last_error().clear();
   const int rc = check_sizes("expert_gather", tokens, top, experts);
   if (rc != MPS_OK) return rc;
   if (!is_float_type(type) || width < 0) return fail(MPS_ERR_INVALID_ARGUMENT, "expert_gather: bad type or width");
   const int64_t pairs = tokens * top;
   if (pairs == 0 || width == 0) return MPS_OK;
-  if (!x || !order || !offsets || !rows) return fail(MPS_ERR_INVALID_ARGUMENT, "expert_gather: null pointer");
+  if (!x || !order || !positions || !offsets || !rows) return fail(MPS_ERR_INVALID_ARGUMENT, "expert_gather: null pointer");
+  RowArgs a = {};
+  a.in = x, a.out = rows, a.order = order, a.positions = positions, a.offsets = offsets;
+  a.tokens = tokens, a.top = top, a.pairs = pairs, a.width = width, a.experts = (int32_t)experts, a.lanes = lanes_of(width, type);
+  const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define CALL(T, V)                                                                                             \
-  hipLaunchKernelGGL((expert_gather_kernel<T, V>), dim3((unsigned)pairs), dim3(kRowThreads), 0, s,            \
-                     static_cast<const Elem<T>::raw *>(x), (int32_t)tokens, (int32_t)top, pairs, (int32_t)experts, \
-                     width, order, offsets, static_cast<Elem<T>::raw *>(rows))
-  MPS_BY_TYPE(type, whole_rows(width, type, x, rows), CALL);
+#define CALL(T, W) \
+  hipLaunchKernelGGL((expert_gather_kernel<T, W>), dim3((unsigned)(blocks + kZeroBlocks)), dim3(kRowThreads), 0, s, a, blocks)
+  MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
@@ -322,13 +452,14 @@ int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine: bad type or width");
   if (tokens == 0 || width == 0) return MPS_OK;
   if (!out || (top > 0 && (!y || !positions))) return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine: null pointer");
-  const int64_t pairs = tokens * top;
+  RowArgs a = {};
+  a.in = y, a.out = out, a.weights = weights, a.weights_type = weights_type, a.positions = positions;
+  a.tokens = tokens, a.top = top, a.pairs = tokens * top, a.width = width, a.lanes = lanes_of(width, type);
+  const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define CALL(T, V)                                                                                            \
-  hipLaunchKernelGGL((expert_combine_kernel<T, V>), dim3((unsigned)tokens), dim3(kRowThreads), 0, s,         \
-                     static_cast<const Elem<T>::raw *>(y), weights, weights_type, (int32_t)top, pairs, width, \
-                     positions, static_cast<Elem<T>::raw *>(out))
-  MPS_BY_TYPE(type, whole_rows(width, type, y, out), CALL);
+#define CALL(T, W) hipLaunchKernelGGL((expert_combine_kernel<T, W>), dim3((unsigned)blocks), dim3(kRowThreads), 0, s, a, \
+                                      static_cast<const Elem<T>::raw *>(y), weights, positions, static_cast<Elem<T>::raw *>(out))
+  MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
@@ -336,7 +467,7 @@ int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t
 
 int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const void *weights, int32_t weights_type,
                             int64_t tokens, int64_t top, int64_t experts, int64_t width, const int32_t *order,
-                            const int32_t *offsets, void *dy, void *dweights, void *stream) {
+                            const int32_t *positions, const int32_t *offsets, void *dy, void *dweights, void *stream) {
   last_error().clear();
   const int rc = check_sizes("expert_combine_grad", tokens, top, experts);
   if (rc != MPS_OK) return rc;
@@ -344,15 +475,17 @@ int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine_grad: bad type or width");
   const int64_t pairs = tokens * top;
   if (pairs == 0) return MPS_OK;
-  if (!weights || !order || !offsets || !dweights || (width > 0 && (!y || !dout || !dy)))
+  if (!weights || !order || !positions || !offsets || !dweights || (width > 0 && (!y || !dout || !dy)))
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine_grad: null pointer");
+  RowArgs a = {};
+  a.in = y, a.dout = dout, a.out = dy, a.weights = weights, a.weights_type = weights_type, a.dweights = dweights;
+  a.order = order, a.positions = positions, a.offsets = offsets;
+  a.tokens = tokens, a.top = top, a.pairs = pairs, a.width = width, a.experts = (int32_t)experts, a.lanes = lanes_of(width, type);
+  const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define CALL(T, V)                                                                                                   \
-  hipLaunchKernelGGL((expert_combine_grad_kernel<T, V>), dim3((unsigned)pairs), dim3(kRowThreads), 0, s,            \
-                     static_cast<const Elem<T>::raw *>(y), static_cast<const Elem<T>::raw *>(dout), weights,         \
-                     weights_type, (int32_t)tokens, (int32_t)top, pairs, (int32_t)experts, width, order, offsets,    \
-                     static_cast<Elem<T>::raw *>(dy), dweights)
-  MPS_BY_TYPE(type, whole_rows(width, type, y, dout, dy), CALL);
+#define CALL(T, W) \
+  hipLaunchKernelGGL((expert_combine_grad_kernel<T, W>), dim3((unsigned)(blocks + kZeroBlocks)), dim3(kRowThreads), 0, s, a, blocks)
+  MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;

@@ -25,16 +25,19 @@ __device__ inline uint32_t quad_max(uint32_t v) {
   return v > b ? v : b;
 }
 
-// Eight elements of a row from column `col` on; zeros past column k.
-template <int T, bool kWhole>
+// Eight elements of a row from column `col` on, at any alignment; zeros past column k.
+template <int T>
 __device__ inline void load8(const typename Elem<T>::raw *row, int64_t col, int64_t k, uint32_t (&v)[T == MPS_TYPE_F32 ? 8 : 4]) {
-  if constexpr (kWhole) {
+  if (col + 8 <= k) {
     constexpr int n = T == MPS_TYPE_F32 ? 2 : 1;
+#pragma unroll
     for (int i = 0; i < n; ++i) {
-      const u32x4 q = reinterpret_cast<const u32x4 *>(row + col)[i];
+      const u32x4 q = reinterpret_cast<const u32x4_any *>(row + col)[i];
+#pragma unroll
       for (int j = 0; j < 4; ++j) v[4 * i + j] = q[j];
     }
   } else {
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
       typename Elem<T>::raw e = 0;
       if (col + i < k) e = row[col + i];
@@ -46,7 +49,8 @@ __device__ inline void load8(const typename Elem<T>::raw *row, int64_t col, int6
   }
 }
 
-template <int T, bool kWhole>
+// kFlat: blocks lie one after the other in x, so no row is needed.
+template <int T, bool kFlat>
 __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const typename Elem<T>::raw *__restrict__ x,
                                                                   uint32_t blocks, uint32_t row_blocks, int64_t k,
                                                                   int64_t stride, uint32_t *__restrict__ codes,
@@ -55,9 +59,9 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const typename
   const uint32_t block = (uint32_t)(unit >> 2), part = (uint32_t)unit & 3;
   if (unit >= (uint64_t)blocks * 4) return;  // whole blocks, so whole quads
   uint32_t row = 0, in_row = block;
-  if (!kWhole || stride != k) row = block / row_blocks, in_row = block - row * row_blocks;
+  if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
   uint32_t v[T == MPS_TYPE_F32 ? 8 : 4];
-  load8<T, kWhole>(x + (int64_t)row * stride, (int64_t)in_row * kMxBlock + part * 8, k, v);
+  load8<T>(x + (int64_t)row * stride, (int64_t)in_row * kMxBlock + part * 8, kFlat ? INT64_MAX : k, v);
 
   uint32_t s;
   if constexpr (T == MPS_TYPE_F32) {
@@ -100,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const typename
 }
 
 // Eight elements a lane: 4 bytes of codes in, 16 (or 32) out.
-template <int T, bool kWhole>
+template <int T, bool kFlat>
 __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const uint32_t *__restrict__ codes,
                                                                     const uint8_t *__restrict__ scales,
                                                                     uint32_t blocks, uint32_t row_blocks, int64_t k,
@@ -127,14 +131,16 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const uint32
     v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2));
     v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3));
   }
-  if constexpr (kWhole) {
+  uint32_t row = 0, in_row = block;
+  if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
+  const int64_t col = (int64_t)in_row * kMxBlock + part * 8;
+  typename Elem<T>::raw *o = out + (int64_t)row * k + col;
+  if (kFlat || col + 8 <= k) {
     constexpr int n = T == MPS_TYPE_F32 ? 2 : 1;
-    u32x4 *o = reinterpret_cast<u32x4 *>(out + unit * 8);
-    for (int i = 0; i < n; ++i) o[i] = u32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+#pragma unroll
+    for (int i = 0; i < n; ++i) reinterpret_cast<u32x4_any *>(o)[i] = u32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
   } else {
-    const uint32_t row = block / row_blocks, in_row = block - row * row_blocks;
-    const int64_t col = (int64_t)in_row * kMxBlock + part * 8;
-    typename Elem<T>::raw *o = out + (int64_t)row * k + col;
+#pragma unroll
     for (int i = 0; i < 8; ++i)
       if (col + i < k) {
         if constexpr (T == MPS_TYPE_F32)
@@ -165,8 +171,7 @@ void launch_quantize(const void *x, int64_t rows, int64_t k, int64_t stride, uin
   typedef typename Elem<T>::raw raw;
   const uint32_t row_blocks = (uint32_t)mx_blocks(k), blocks = (uint32_t)rows * row_blocks;
   const dim3 grid((unsigned)(((uint64_t)blocks * 4 + kThreads - 1) / kThreads));
-  // Rows of whole blocks at 16-byte addresses are read 16 bytes a lane, others element by element.
-  if (k % kMxBlock == 0 && aligned16(x) && (rows == 1 || stride * (int64_t)sizeof(raw) % 16 == 0))
+  if (k % kMxBlock == 0 && (rows == 1 || stride == k))
     hipLaunchKernelGGL((mxfp4_quantize_kernel<T, true>), grid, dim3(kThreads), 0, stream, static_cast<const raw *>(x),
                        blocks, row_blocks, k, stride, reinterpret_cast<uint32_t *>(codes), scales);
   else
@@ -181,7 +186,7 @@ void launch_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows
   typedef typename Elem<T>::raw raw;
   const uint32_t row_blocks = (uint32_t)mx_blocks(k), blocks = (uint32_t)rows * row_blocks;
   const dim3 grid((unsigned)(((uint64_t)blocks * 4 + kThreads - 1) / kThreads));
-  if (k % kMxBlock == 0 && aligned16(out))
+  if (k % kMxBlock == 0)
     hipLaunchKernelGGL((mxfp4_dequantize_kernel<T, true>), grid, dim3(kThreads), 0, stream,
                        reinterpret_cast<const uint32_t *>(codes), scales, blocks, row_blocks, k,
                        static_cast<raw *>(out));

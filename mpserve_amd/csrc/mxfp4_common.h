@@ -22,6 +22,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // 16-byte accesses take any alignment
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 inline int64_t mx_blocks(int64_t k) { return (k + kMxBlock - 1) / kMxBlock; }

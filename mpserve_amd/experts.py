@@ -94,7 +94,7 @@ def _gather_rows(x: torch.Tensor, order: torch.Tensor, positions: torch.Tensor, 
     t, top = positions.shape
     rows = torch.empty((t * top, x.shape[1]), dtype=x.dtype, device=x.device)
     _call(x.device, _native.lib().mps_expert_gather, x.data_ptr(), _TYPES[x.dtype], t, top, offsets.numel() - 1,
-          x.shape[1], order.data_ptr(), offsets.data_ptr(), rows.data_ptr())
+          x.shape[1], order.data_ptr(), positions.data_ptr(), offsets.data_ptr(), rows.data_ptr())
     return rows
 
 
@@ -114,19 +114,19 @@ class _Gather(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, order, positions, offsets):
-        ctx.save_for_backward(y, weights, order, offsets)
+        ctx.save_for_backward(y, weights, order, positions, offsets)
         return _sum_rows(y, weights, positions)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        y, weights, order, offsets = ctx.saved_tensors
+        y, weights, order, positions, offsets = ctx.saved_tensors
         t, top = weights.shape
         dout = dout.contiguous()
         dy, dweights = torch.empty_like(y), torch.empty_like(weights)
         _call(y.device, _native.lib().mps_expert_combine_grad, y.data_ptr(), dout.data_ptr(), _TYPES[y.dtype],
               weights.data_ptr(), _TYPES[weights.dtype], t, top, offsets.numel() - 1, y.shape[1], order.data_ptr(),
-              offsets.data_ptr(), dy.data_ptr(), dweights.data_ptr())
+              positions.data_ptr(), offsets.data_ptr(), dy.data_ptr(), dweights.data_ptr())
         return dy, dweights, None, None, None
 
 

@@ -32,9 +32,9 @@ def test_c_entries_refuse_bad_arguments():
                lib.mps_mxfp4_dequantize(p, None, 1, 32, p, 0, None), lib.mps_mxfp4_dequantize(p, p, 1, -32, p, 0, None),
                lib.mps_mxfp4_multiply(None, None, 0, None), lib.mps_expert_sort(p, 0, 2 ** 30, 4, 8, p, p, p, None, 0, None),
                lib.mps_expert_sort(p, 0, 4, 4, 0, p, p, p, None, 0, None), lib.mps_expert_sort(p, 0, 4, 4, 1025, p, p, p, None, 0, None),
-               lib.mps_expert_sort(None, 0, 4, 4, 8, p, p, p, None, 0, None), lib.mps_expert_gather(p, 3, 4, 4, 8, 32, p, p, p, None),
-               lib.mps_expert_gather(p, 0, 4, 4, 8, -1, p, p, p, None), lib.mps_expert_combine(p, 0, p, 9, 4, 4, 32, p, p, None),
-               lib.mps_expert_combine_grad(p, p, 0, None, 0, 4, 4, 8, 32, p, p, p, p, None)):
+               lib.mps_expert_sort(None, 0, 4, 4, 8, p, p, p, None, 0, None), lib.mps_expert_gather(p, 3, 4, 4, 8, 32, p, p, p, p, None),
+               lib.mps_expert_gather(p, 0, 4, 4, 8, -1, p, p, p, p, None), lib.mps_expert_combine(p, 0, p, 9, 4, 4, 32, p, p, None),
+               lib.mps_expert_combine_grad(p, p, 0, None, 0, 4, 4, 8, 32, p, p, p, p, p, None)):
         assert rc == _native.MPS_ERR_INVALID_ARGUMENT and lib.mps_last_error()
     good = dict(x=p, x_stride=32, w=p, w_scales=p, out=p, rows=4, n=8, k=32, x_type=0, out_type=0)
     for change in (dict(x_type=2), dict(out_type=3), dict(bias=p, bias_type=5), dict(rows=-1), dict(rows=2 ** 31), dict(n=2 ** 33),
