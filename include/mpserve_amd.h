@@ -339,7 +339,8 @@ int mps_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t ro
  * and the order are mps_expert_sort's (or hold its promises: offsets rise
  * from 0 to at most rows, the order's entries are below the rows of x times
  * top). Codes are 16-byte aligned; those past column k in a row's last block
- * are zero, as mps_mxfp4_quantize writes them. */
+ * are zero, as mps_mxfp4_quantize writes them. No workspace is needed for MXFP4
+ * x, nor for 16-bit x whose rows are whole blocks at 16-byte addresses. */
 typedef struct mps_mxfp4_product {
   const void *x;           /* [rows, k] with x_stride, or MXFP4 codes */
   const uint8_t *x_scales; /* MXFP4 only */

@@ -21,7 +21,7 @@ import torch
 
 from . import _native
 from ._common import _check_cuda_contig
-from .mxfp4 import BLOCK, _TYPES, _call, _check_bias, _check_cuda, _check_mx, _check_out, _multiply, _no_grad, _type
+from .mxfp4 import BLOCK, _TYPES, _call, _check_bias, _check_cuda, _check_mx, _check_out, _multiply, _no_grad, _set_x, _type
 
 
 class ExpertSort(NamedTuple):
@@ -172,7 +172,8 @@ def mxfp4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     _check_cuda(x, "x")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _no_grad("mxfp4_expert_linear", x, bias)
+    _no_grad("mxfp4_expert_linear", x)
+    _no_grad("mxfp4_expert_linear", bias)
     device = x.device
     _check_sort(sort, device)
     _check_rows(x, "x", sort.positions.shape[0] if gather else sort.order.numel())
@@ -189,11 +190,12 @@ def mxfp4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     out = _check_out(out, (rows, n), dtype, device)
     if x.stride(1) != 1:
         x = x.contiguous()
-    p.x, p.x_type, p.x_stride, p.rows = x.data_ptr(), _TYPES[x.dtype], x.stride(0), rows
+    whole = _set_x(p, x, k)
+    p.rows = rows
     p.w, p.w_scales, p.out, p.n, p.k = codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, k
     if bias is not None:
         p.bias = bias.data_ptr()
     p.experts, p.offsets, p.order = experts, sort.offsets.data_ptr(), sort.order.data_ptr()
     p.top, p.gather = max(1, sort.positions.shape[1]), bool(gather)
-    _multiply(p, device)
+    _multiply(p, whole, device)
     return out

@@ -40,8 +40,8 @@ def _type(t: torch.Tensor | torch.dtype, name: str) -> int:
     return code
 
 
-def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(name: str, t: Optional[torch.Tensor]) -> None:
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
 
 
@@ -79,11 +79,11 @@ def _check_mx(codes: torch.Tensor, scales: torch.Tensor, name: str, dims: Option
               device: Optional[torch.device] = None) -> None:
     if codes is not None and scales is not None:  # all is well in one go; what is not is named below
         c, s = codes.shape, scales.shape
-        if codes.is_cuda and scales.is_cuda and codes.dtype == scales.dtype == torch.uint8 \
-                and codes.device == scales.device and (device is None or codes.device == device) \
-                and codes.is_contiguous() and scales.is_contiguous() and len(c) == len(s) >= 1 \
-                and (dims is None or len(c) == dims) and c[:-1] == s[:-1] and c[-1] == 16 * s[-1] \
-                and codes.data_ptr() % 16 == 0:
+        n, at = len(c), codes.device
+        if codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and codes.is_cuda and at == scales.device \
+                and (device is None or at == device) and codes.is_contiguous() and scales.is_contiguous() \
+                and n == len(s) and n >= 1 and (dims is None or n == dims) and c[-1] == 16 * s[-1] \
+                and (c[0] == s[0] if n == 2 else c[:-1] == s[:-1]) and not codes.data_ptr() & 15:
             return
     for t, part in ((codes, "codes"), (scales, "scales")):
         full = f"{name}{part}"
@@ -115,16 +115,22 @@ def mxfp4_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _check_cuda(x, "x")
     t = _type(x, "x")
     _no_grad("mxfp4_quantize", x)
-    if x.dim() < 1:
+    shape, device = x.shape, x.device
+    if len(shape) < 1:
         raise ValueError("x must have at least one dimension")
-    k = x.shape[-1]
-    rows = _rows(x, k)
+    k = shape[-1]
     blocks = (k + BLOCK - 1) // BLOCK
-    lead = x.shape[:-1]
-    codes = torch.empty((*lead, 16 * blocks), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device)
-    _call(x.device, _native.lib().mps_mxfp4_quantize, rows.data_ptr(), t, rows.shape[0], k, rows.stride(0),
-          codes.data_ptr(), scales.data_ptr())
+    if len(shape) == 2:
+        n = shape[0]
+        rows = x if x.stride(1) == 1 or k <= 1 else x.contiguous()
+        codes = torch.empty((n, 16 * blocks), dtype=torch.uint8, device=device)
+        scales = torch.empty((n, blocks), dtype=torch.uint8, device=device)
+    else:
+        rows = _rows(x, k)
+        n = rows.shape[0]
+        codes = torch.empty((*shape[:-1], 16 * blocks), dtype=torch.uint8, device=device)
+        scales = torch.empty((*shape[:-1], blocks), dtype=torch.uint8, device=device)
+    _call(device, _native.lib().mps_mxfp4_quantize, rows.data_ptr(), t, n, k, rows.stride(0), codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -143,16 +149,22 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: t
     return out
 
 
-def _multiply(p: "_native.MpsMxfp4Product", device: torch.device) -> None:
+def _multiply(p: "_native.MpsMxfp4Product", x_whole: bool, device: torch.device) -> None:
+    """``x_whole``: x is MXFP4, or its rows are whole blocks at 16-byte addresses, and needs no workspace."""
+    lib = _native.lib()
+    if x_whole:
+        return _call(device, lib.mps_mxfp4_multiply, p, None, 0)
     need = ctypes.c_int64(0)
-    rc = _native.lib().mps_mxfp4_product_workspace(p, need)
-    if rc:
-        _native.check(rc)
-    if need.value:
-        work = torch.empty(need.value, dtype=torch.uint8, device=device)
-        _call(device, _native.lib().mps_mxfp4_multiply, p, work.data_ptr(), need.value)
-    else:
-        _call(device, _native.lib().mps_mxfp4_multiply, p, None, 0)
+    _native.check(lib.mps_mxfp4_product_workspace(p, need))
+    work = torch.empty(need.value, dtype=torch.uint8, device=device)
+    _call(device, lib.mps_mxfp4_multiply, p, work.data_ptr(), need.value)
+
+
+def _set_x(p: "_native.MpsMxfp4Product", x: torch.Tensor, k: int) -> bool:
+    """Rows ``x [r, k]`` of adjacent 16-bit elements; whether they need no workspace."""
+    at, stride = x.data_ptr(), x.stride(0)
+    p.x, p.x_type, p.x_stride = at, _TYPES[x.dtype], stride
+    return not (k & 31 or at & 15 or stride & 7)
 
 
 def _check_bias(bias: Optional[torch.Tensor], shape, device: torch.device) -> int:
@@ -173,24 +185,27 @@ def mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
     _check_cuda(x, "x")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _no_grad("mxfp4_linear", x, bias)
-    if x.dim() < 1:
+    _no_grad("mxfp4_linear", x)
+    _no_grad("mxfp4_linear", bias)
+    shape, device = x.shape, x.device
+    if len(shape) < 1:
         raise ValueError("x must have at least one dimension")
-    device, k = x.device, x.shape[-1]
+    k = shape[-1]
     _check_mx(codes, scales, "", 2, device)
-    if scales.shape[1] != (k + BLOCK - 1) // BLOCK:
-        raise ValueError(f"x has {k} columns, which do not fit the weight's {scales.shape[1]} blocks of {BLOCK}")
-    n = codes.shape[0]
+    n, blocks = scales.shape
+    if blocks != (k + BLOCK - 1) // BLOCK:
+        raise ValueError(f"x has {k} columns, which do not fit the weight's {blocks} blocks of {BLOCK}")
     dtype = out_dtype if out_dtype is not None else (out.dtype if out is not None else x.dtype)
     p = _native.MpsMxfp4Product()
     p.out_type, p.bias_type = _type(dtype, "out_dtype"), _check_bias(bias, (n,), device)
-    out = _check_out(out, (*x.shape[:-1], n), dtype, device)
+    out = _check_out(out, (*shape[:-1], n), dtype, device)
     rows = _rows(x, k)
-    p.x, p.x_type, p.x_stride, p.rows = rows.data_ptr(), _TYPES[x.dtype], rows.stride(0), x.numel() // k if k else out.numel() // n if n else 0
+    whole = _set_x(p, rows, k)
+    p.rows = rows.shape[0] if k else (out.numel() // n if n else 0)
     p.w, p.w_scales, p.out, p.n, p.k = codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, k
     if bias is not None:
         p.bias = bias.data_ptr()
-    _multiply(p, device)
+    _multiply(p, whole, device)
     return out
 
 
@@ -215,5 +230,5 @@ def mxfp4_matmul(x_codes: torch.Tensor, x_scales: torch.Tensor, codes: torch.Ten
     p.w, p.w_scales, p.out, p.n, p.k = codes.data_ptr(), scales.data_ptr(), out.data_ptr(), n, BLOCK * scales.shape[1]
     if bias is not None:
         p.bias = bias.data_ptr()
-    _multiply(p, device)
+    _multiply(p, True, device)
     return out
