@@ -210,17 +210,20 @@ template <int T, bool kWide>
 __global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(RowArgs a, int64_t token_blocks) {
   typedef Piece<T> P;
   typedef typename Elem<T>::raw raw;
-  if (blockIdx.x >= token_blocks) return zero_rows<T>(a, blockIdx.x - token_blocks, kZeroBlocks, false);
+  const int64_t grid = gridDim.x - kZeroBlocks;
+  if (blockIdx.x >= grid) return zero_rows<T>(a, blockIdx.x - grid, kZeroBlocks, false);
   const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
-  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
-  if (t >= a.tokens) return;
-  const raw *const row = static_cast<const raw *>(a.in) + t * a.width;
-  raw *const out = static_cast<raw *>(a.out);
-  for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
-    const P p = P::load(row, col, a.width);
-    for (int64_t i = 0; i < a.top; ++i) {
-      const int32_t at = a.positions[t * a.top + i];
-      if (at >= 0 && at < a.pairs) p.store(out + at * a.width, col, a.width);
+  for (int64_t block = blockIdx.x; block < token_blocks; block += grid) {
+    const int64_t t = kWide ? block : block * (kRowThreads / lanes) + threadIdx.x / lanes;
+    if (t >= a.tokens) continue;
+    const raw *const row = static_cast<const raw *>(a.in) + t * a.width;
+    raw *const out = static_cast<raw *>(a.out);
+    for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+      const P p = P::load(row, col, a.width);
+      for (int64_t i = 0; i < a.top; ++i) {
+        const int32_t at = a.positions[t * a.top + i];
+        if (at >= 0 && at < a.pairs) p.store(out + at * a.width, col, a.width);
+      }
     }
   }
 }
@@ -228,51 +231,54 @@ __global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(RowArgs a, i
 // (The pointers stand by themselves so that the compiler may take them to be apart, and loads of the places
 // and weights, alike for all lanes, to be scalar.)
 template <int T, bool kWide>
-__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(RowArgs a, const typename Elem<T>::raw *__restrict__ y,
+__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(RowArgs a, int64_t token_blocks,
+                                                                     const typename Elem<T>::raw *__restrict__ y,
                                                                      const void *__restrict__ weights,
                                                                      const int32_t *__restrict__ positions,
                                                                      typename Elem<T>::raw *__restrict__ out) {
   typedef Piece<T> P;
   const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
-  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
-  if (t >= a.tokens) return;
-  for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
-    const bool whole = col + P::kVec <= a.width;
-    float sum[P::kVec] = {};
-    for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
-      // Whole pieces without branches, so that their loads are in flight together: an absent pair reads row 0.
-      int64_t at[kPairs];
-      bool there[kPairs];
-      float w[kPairs];
+  for (int64_t block = blockIdx.x; block < token_blocks; block += gridDim.x) {
+    const int64_t t = kWide ? block : block * (kRowThreads / lanes) + threadIdx.x / lanes;
+    if (t >= a.tokens) continue;
+    for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+      const bool whole = col + P::kVec <= a.width;
+      float sum[P::kVec] = {};
+      for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
+        // Whole pieces without branches, so that their loads are in flight together: an absent pair reads row 0.
+        int64_t at[kPairs];
+        bool there[kPairs];
+        float w[kPairs];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        const int64_t in = i0 + i < a.top ? i0 + i : 0;
-        const int32_t p = positions[t * a.top + in];
-        there[i] = i0 + i < a.top && p >= 0 && p < a.pairs;
-        at[i] = there[i] ? p : 0;
-        w[i] = 1.0f;
+        for (int i = 0; i < kPairs; ++i) {
+          const int64_t in = i0 + i < a.top ? i0 + i : 0;
+          const int32_t p = positions[t * a.top + in];
+          there[i] = i0 + i < a.top && p >= 0 && p < a.pairs;
+          at[i] = there[i] ? p : 0;
+          w[i] = 1.0f;
+        }
+        if (weights) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) w[i] = load_as_float(weights, a.weights_type, t * a.top + (i0 + i < a.top ? i0 + i : 0));
+        }
+        P p[kPairs];
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) p[i].bits = *reinterpret_cast<const u32x4_any *>(y + at[i] * a.width + col);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) p[i] = P::load(y + at[i] * a.width, col, a.width);
+        }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+          for (int v = 0; v < P::kVec; ++v) sum[v] = there[i] ? __builtin_fmaf(w[i], p[i].get(v), sum[v]) : sum[v];
       }
-      if (weights) {
+      P o;
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) w[i] = load_as_float(weights, a.weights_type, t * a.top + (i0 + i < a.top ? i0 + i : 0));
-      }
-      P p[kPairs];
-      if (whole) {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) p[i].bits = *reinterpret_cast<const u32x4_any *>(y + at[i] * a.width + col);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) p[i] = P::load(y + at[i] * a.width, col, a.width);
-      }
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i)
-#pragma unroll
-        for (int v = 0; v < P::kVec; ++v) sum[v] = there[i] ? __builtin_fmaf(w[i], p[i].get(v), sum[v]) : sum[v];
+      for (int v = 0; v < P::kVec; ++v) o.put(v, sum[v]);
+      o.store(out + t * a.width, col, a.width);
     }
-    P o;
-#pragma unroll
-    for (int v = 0; v < P::kVec; ++v) o.put(v, sum[v]);
-    o.store(out + t * a.width, col, a.width);
   }
 }
 
@@ -283,63 +289,66 @@ __global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(RowArg
   typedef Piece<T> P;
   typedef typename Elem<T>::raw raw;
   __shared__ float parts[kPairs][kRowThreads / 64];
-  if (blockIdx.x >= token_blocks) return zero_rows<T>(a, blockIdx.x - token_blocks, kZeroBlocks, true);
+  const int64_t grid = gridDim.x - kZeroBlocks;
+  if (blockIdx.x >= grid) return zero_rows<T>(a, blockIdx.x - grid, kZeroBlocks, true);
   const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
-  const int64_t t = kWide ? blockIdx.x : (int64_t)blockIdx.x * (kRowThreads / lanes) + threadIdx.x / lanes;
-  const bool token = t < a.tokens;
-  const raw *const y = static_cast<const raw *>(a.in), *const g = static_cast<const raw *>(a.dout) + (token ? t : 0) * a.width;
-  raw *const dy = static_cast<raw *>(a.out);
-  for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
-    float w[kPairs], dot[kPairs] = {};
-    int64_t at[kPairs];
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      const int64_t pair = t * a.top + i0 + i;
-      at[i] = token && i0 + i < a.top ? a.positions[pair] : -1;
-      if (at[i] >= a.pairs) at[i] = -1;
-      w[i] = at[i] >= 0 ? load_as_float(a.weights, a.weights_type, pair) : 0.0f;
-    }
-    if (token)
-      for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
-        const P d = P::load(g, col, a.width);
-        P p[kPairs];
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i)
-          if (at[i] >= 0) p[i] = P::load(y + at[i] * a.width, col, a.width);
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i)
-          if (at[i] >= 0) {
-            P o;
-#pragma unroll
-            for (int v = 0; v < P::kVec; ++v) {
-              const float gv = d.get(v);
-              dot[i] += gv * p[i].get(v);
-              o.put(v, w[i] * gv);
-            }
-            o.store(dy + at[i] * a.width, col, a.width);
-          }
-      }
-    const int in_wave = lanes < 64 ? lanes : 64;
-    for (int d = in_wave / 2; d > 0; d /= 2)
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) dot[i] += __shfl_xor(dot[i], d);
-    if (lanes > 64) {
-      if ((threadIdx.x & 63) == 0)
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) parts[i][threadIdx.x >> 6] = dot[i];
-      __syncthreads();
-      const int first = threadIdx.x / lanes * (lanes / 64);
+  for (int64_t block = blockIdx.x; block < token_blocks; block += grid) {
+    const int64_t t = kWide ? block : block * (kRowThreads / lanes) + threadIdx.x / lanes;
+    const bool token = t < a.tokens;
+    const raw *const y = static_cast<const raw *>(a.in), *const g = static_cast<const raw *>(a.dout) + (token ? t : 0) * a.width;
+    raw *const dy = static_cast<raw *>(a.out);
+    for (int64_t i0 = 0; i0 < a.top; i0 += kPairs) {
+      float w[kPairs], dot[kPairs] = {};
+      int64_t at[kPairs];
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        dot[i] = 0;
-        for (int j = 0; j < lanes / 64; ++j) dot[i] += parts[i][first + j];
+        const int64_t pair = t * a.top + i0 + i;
+        at[i] = token && i0 + i < a.top ? a.positions[pair] : -1;
+        if (at[i] >= a.pairs) at[i] = -1;
+        w[i] = at[i] >= 0 ? load_as_float(a.weights, a.weights_type, pair) : 0.0f;
       }
-      __syncthreads();
-    }
-    if ((threadIdx.x & (lanes - 1)) == 0)
+      if (token)
+        for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
+          const P d = P::load(g, col, a.width);
+          P p[kPairs];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i)
-        if (at[i] >= 0) store_as(a.dweights, a.weights_type, t * a.top + i0 + i, dot[i]);
+          for (int i = 0; i < kPairs; ++i)
+            if (at[i] >= 0) p[i] = P::load(y + at[i] * a.width, col, a.width);
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i)
+            if (at[i] >= 0) {
+              P o;
+#pragma unroll
+              for (int v = 0; v < P::kVec; ++v) {
+                const float gv = d.get(v);
+                dot[i] += gv * p[i].get(v);
+                o.put(v, w[i] * gv);
+              }
+              o.store(dy + at[i] * a.width, col, a.width);
+            }
+        }
+      const int in_wave = lanes < 64 ? lanes : 64;
+      for (int d = in_wave / 2; d > 0; d /= 2)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) dot[i] += __shfl_xor(dot[i], d);
+      if (lanes > 64) {
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) parts[i][threadIdx.x >> 6] = dot[i];
+        __syncthreads();
+        const int first = threadIdx.x / lanes * (lanes / 64);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          dot[i] = 0;
+          for (int j = 0; j < lanes / 64; ++j) dot[i] += parts[i][first + j];
+        }
+        __syncthreads();
+      }
+      if ((threadIdx.x & (lanes - 1)) == 0)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (at[i] >= 0) store_as(a.dweights, a.weights_type, t * a.top + i0 + i, dot[i]);
+    }
   }
 }
 
@@ -436,7 +445,7 @@ int mps_expert_gather(const void *x, int32_t type, int64_t tokens, int64_t top, 
   const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define CALL(T, W) \
-  hipLaunchKernelGGL((expert_gather_kernel<T, W>), dim3((unsigned)(blocks + kZeroBlocks)), dim3(kRowThreads), 0, s, a, blocks)
+  hipLaunchKernelGGL((expert_gather_kernel<T, W>), dim3(workgroups(blocks) + kZeroBlocks), dim3(kRowThreads), 0, s, a, blocks)
   MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
   MPS_HIP_CHECK(hipGetLastError());
@@ -457,7 +466,7 @@ int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t
   a.tokens = tokens, a.top = top, a.pairs = tokens * top, a.width = width, a.lanes = lanes_of(width, type);
   const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define CALL(T, W) hipLaunchKernelGGL((expert_combine_kernel<T, W>), dim3((unsigned)blocks), dim3(kRowThreads), 0, s, a, \
+#define CALL(T, W) hipLaunchKernelGGL((expert_combine_kernel<T, W>), dim3(workgroups(blocks)), dim3(kRowThreads), 0, s, a, blocks, \
                                       static_cast<const Elem<T>::raw *>(y), weights, positions, static_cast<Elem<T>::raw *>(out))
   MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
@@ -484,7 +493,7 @@ int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const
   const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define CALL(T, W) \
-  hipLaunchKernelGGL((expert_combine_grad_kernel<T, W>), dim3((unsigned)(blocks + kZeroBlocks)), dim3(kRowThreads), 0, s, a, blocks)
+  hipLaunchKernelGGL((expert_combine_grad_kernel<T, W>), dim3(workgroups(blocks) + kZeroBlocks), dim3(kRowThreads), 0, s, a, blocks)
   MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
   MPS_HIP_CHECK(hipGetLastError());

@@ -55,52 +55,53 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const typename
                                                                   uint32_t blocks, uint32_t row_blocks, int64_t k,
                                                                   int64_t stride, uint32_t *__restrict__ codes,
                                                                   uint8_t *__restrict__ scales) {
-  const uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t block = (uint32_t)(unit >> 2), part = (uint32_t)unit & 3;
-  if (unit >= (uint64_t)blocks * 4) return;  // whole blocks, so whole quads
-  uint32_t row = 0, in_row = block;
-  if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
-  uint32_t v[T == MPS_TYPE_F32 ? 8 : 4];
-  load8<T>(x + (int64_t)row * stride, (int64_t)in_row * kMxBlock + part * 8, kFlat ? INT64_MAX : k, v);
+  for (uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x; unit < (uint64_t)blocks * 4;  // whole blocks, so whole quads
+       unit += (uint64_t)gridDim.x * kThreads) {
+    const uint32_t block = (uint32_t)(unit >> 2), part = (uint32_t)unit & 3;
+    uint32_t row = 0, in_row = block;
+    if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
+    uint32_t v[T == MPS_TYPE_F32 ? 8 : 4];
+    load8<T>(x + (int64_t)row * stride, (int64_t)in_row * kMxBlock + part * 8, kFlat ? INT64_MAX : k, v);
 
-  uint32_t s;
-  if constexpr (T == MPS_TYPE_F32) {
-    uint32_t m = 0;
-    for (int i = 0; i < 8; ++i) m = max(m, v[i] & 0x7fffffffu);
-    s = quad_max(m) >> 23;
-  } else {
-    // Magnitudes order as their bits do, NaN above infinity.
-    u16x2 m = {0, 0};
-    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
-    const uint32_t top = quad_max(max((uint32_t)m.x, (uint32_t)m.y));
-    if constexpr (T == MPS_TYPE_BF16)
-      s = top >> 7;
-    else
-      s = __float_as_uint(Elem<T>::get((uint16_t)top)) >> 23;
-  }
-  const bool finite = s != 255;
-  s = finite ? (s > 2 ? s - 2 : 0) : 255;
+    uint32_t s;
+    if constexpr (T == MPS_TYPE_F32) {
+      uint32_t m = 0;
+      for (int i = 0; i < 8; ++i) m = max(m, v[i] & 0x7fffffffu);
+      s = quad_max(m) >> 23;
+    } else {
+      // Magnitudes order as their bits do, NaN above infinity.
+      u16x2 m = {0, 0};
+      for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+      const uint32_t top = quad_max(max((uint32_t)m.x, (uint32_t)m.y));
+      if constexpr (T == MPS_TYPE_BF16)
+        s = top >> 7;
+      else
+        s = __float_as_uint(Elem<T>::get((uint16_t)top)) >> 23;
+    }
+    const bool finite = s != 255;
+    s = finite ? (s > 2 ? s - 2 : 0) : 255;
 
-  const float scale = mx_scale(s);
-  uint32_t c = 0;
-  if constexpr (T == MPS_TYPE_F32) {
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[0]), __uint_as_float(v[1]), scale, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[2]), __uint_as_float(v[3]), scale, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[4]), __uint_as_float(v[5]), scale, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[6]), __uint_as_float(v[7]), scale, 3);
-  } else if constexpr (T == MPS_TYPE_BF16) {
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[0]), scale, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[1]), scale, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[2]), scale, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[3]), scale, 3);
-  } else {
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[0]), scale, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[1]), scale, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[2]), scale, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[3]), scale, 3);
+    const float scale = mx_scale(s);
+    uint32_t c = 0;
+    if constexpr (T == MPS_TYPE_F32) {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[0]), __uint_as_float(v[1]), scale, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[2]), __uint_as_float(v[3]), scale, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[4]), __uint_as_float(v[5]), scale, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(v[6]), __uint_as_float(v[7]), scale, 3);
+    } else if constexpr (T == MPS_TYPE_BF16) {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[0]), scale, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[1]), scale, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[2]), scale, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, v[3]), scale, 3);
+    } else {
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[0]), scale, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[1]), scale, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[2]), scale, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, v[3]), scale, 3);
+    }
+    codes[unit] = finite ? c : 0;
+    if (part == 0) scales[block] = (uint8_t)s;
   }
-  codes[unit] = finite ? c : 0;
-  if (part == 0) scales[block] = (uint8_t)s;
 }
 
 // Eight elements a lane: 4 bytes of codes in, 16 (or 32) out.
@@ -109,45 +110,46 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const uint32
                                                                     const uint8_t *__restrict__ scales,
                                                                     uint32_t blocks, uint32_t row_blocks, int64_t k,
                                                                     typename Elem<T>::raw *__restrict__ out) {
-  const uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t block = (uint32_t)(unit >> 2), part = (uint32_t)unit & 3;
-  if (unit >= (uint64_t)blocks * 4) return;
-  const uint32_t c = codes[unit];
-  const float scale = mx_scale(scales[block]);
-  uint32_t v[T == MPS_TYPE_F32 ? 8 : 4];
-  if constexpr (T == MPS_TYPE_F32) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3);
-    const float f[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
-    for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(f[i]);
-  } else if constexpr (T == MPS_TYPE_BF16) {
-    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
-    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
-  } else {
-    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 0));
-    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 1));
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3));
-  }
-  uint32_t row = 0, in_row = block;
-  if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
-  const int64_t col = (int64_t)in_row * kMxBlock + part * 8;
-  typename Elem<T>::raw *o = out + (int64_t)row * k + col;
-  if (kFlat || col + 8 <= k) {
-    constexpr int n = T == MPS_TYPE_F32 ? 2 : 1;
+  for (uint64_t unit = (uint64_t)blockIdx.x * kThreads + threadIdx.x; unit < (uint64_t)blocks * 4;
+       unit += (uint64_t)gridDim.x * kThreads) {
+    const uint32_t block = (uint32_t)(unit >> 2), part = (uint32_t)unit & 3;
+    const uint32_t c = codes[unit];
+    const float scale = mx_scale(scales[block]);
+    uint32_t v[T == MPS_TYPE_F32 ? 8 : 4];
+    if constexpr (T == MPS_TYPE_F32) {
+      const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
+      const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3);
+      const float f[8] = {a.x, a.y, b.x, b.y, d.x, d.y, e.x, e.y};
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(f[i]);
+    } else if constexpr (T == MPS_TYPE_BF16) {
+      v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
+      v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
+      v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
+      v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
+    } else {
+      v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 0));
+      v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 1));
+      v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2));
+      v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3));
+    }
+    uint32_t row = 0, in_row = block;
+    if (!kFlat) row = block / row_blocks, in_row = block - row * row_blocks;
+    const int64_t col = (int64_t)in_row * kMxBlock + part * 8;
+    typename Elem<T>::raw *o = out + (int64_t)row * k + col;
+    if (kFlat || col + 8 <= k) {
+      constexpr int n = T == MPS_TYPE_F32 ? 2 : 1;
 #pragma unroll
-    for (int i = 0; i < n; ++i) reinterpret_cast<u32x4_any *>(o)[i] = u32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-  } else {
+      for (int i = 0; i < n; ++i) reinterpret_cast<u32x4_any *>(o)[i] = u32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < k) {
-        if constexpr (T == MPS_TYPE_F32)
-          o[i] = __uint_as_float(v[i]);
-        else
-          o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
-      }
+      for (int i = 0; i < 8; ++i)
+        if (col + i < k) {
+          if constexpr (T == MPS_TYPE_F32)
+            o[i] = __uint_as_float(v[i]);
+          else
+            o[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+        }
+    }
   }
 }
 
@@ -170,7 +172,7 @@ void launch_quantize(const void *x, int64_t rows, int64_t k, int64_t stride, uin
                      hipStream_t stream) {
   typedef typename Elem<T>::raw raw;
   const uint32_t row_blocks = (uint32_t)mx_blocks(k), blocks = (uint32_t)rows * row_blocks;
-  const dim3 grid((unsigned)(((uint64_t)blocks * 4 + kThreads - 1) / kThreads));
+  const dim3 grid(workgroups(((int64_t)blocks * 4 + kThreads - 1) / kThreads));
   if (k % kMxBlock == 0 && (rows == 1 || stride == k))
     hipLaunchKernelGGL((mxfp4_quantize_kernel<T, true>), grid, dim3(kThreads), 0, stream, static_cast<const raw *>(x),
                        blocks, row_blocks, k, stride, reinterpret_cast<uint32_t *>(codes), scales);
@@ -185,7 +187,7 @@ void launch_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows
                        hipStream_t stream) {
   typedef typename Elem<T>::raw raw;
   const uint32_t row_blocks = (uint32_t)mx_blocks(k), blocks = (uint32_t)rows * row_blocks;
-  const dim3 grid((unsigned)(((uint64_t)blocks * 4 + kThreads - 1) / kThreads));
+  const dim3 grid(workgroups(((int64_t)blocks * 4 + kThreads - 1) / kThreads));
   if (k % kMxBlock == 0)
     hipLaunchKernelGGL((mxfp4_dequantize_kernel<T, true>), grid, dim3(kThreads), 0, stream,
                        reinterpret_cast<const uint32_t *>(codes), scales, blocks, row_blocks, k,

@@ -25,6 +25,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // 16-byte accesses take any alignment
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
+// A grid holds fewer than 2^32 work-items: kernels over elements or rows get at most this many
+// workgroups (of 256) and go on where the grid ends.
+constexpr int64_t kMostWorkgroups = 1 << 22;
+inline unsigned workgroups(int64_t wanted) { return (unsigned)(wanted < kMostWorkgroups ? wanted : kMostWorkgroups); }
+
 inline int64_t mx_blocks(int64_t k) { return (k + kMxBlock - 1) / kMxBlock; }
 __host__ __device__ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline bool is_float_type(int32_t t) { return t == MPS_TYPE_BF16 || t == MPS_TYPE_F16 || t == MPS_TYPE_F32; }

@@ -52,10 +52,23 @@ __device__ inline Tile find_tile(const int32_t *offsets, int32_t experts, int32_
   return {-1, 0, 0};
 }
 
-// Eight elements of a 16-bit row from `col` on, as bits; zeros past column k.
-__device__ inline u32x4 load_row8(const uint16_t *row, int64_t col, int64_t k, bool whole) {
-  if (whole && col + 8 <= k) return *reinterpret_cast<const u32x4 *>(row + col);
+// How many of these tiles there are.
+__device__ inline int32_t count_tiles(const int32_t *offsets, int32_t experts, int32_t rows, int32_t size) {
+  const int lane = threadIdx.x & 63;
+  int32_t tiles = 0;
+  for (int32_t e = lane; e <= experts; e += 64) {
+    const int32_t first = min(max(offsets[e], 0), rows), end = e < experts ? max(first, min(offsets[e + 1], rows)) : rows;
+    tiles += (end - first + size - 1) / size;
+  }
+  for (int d = 32; d > 0; d /= 2) tiles += __shfl_xor(tiles, d);
+  return tiles;
+}
+
+// Eight elements of a 16-bit row from `col` on, at any alignment, as bits; zeros past column k.
+__device__ inline u32x4 load_row8(const uint16_t *row, int64_t col, int64_t k) {
+  if (col + 8 <= k) return *reinterpret_cast<const u32x4_any *>(row + col);
   u32x4 v = {0, 0, 0, 0};
+#pragma unroll
   for (int i = 0; i < 8; ++i)
     if (col + i < k) v[i / 2] |= (uint32_t)row[col + i] << (16 * (i % 2));
   return v;
@@ -155,7 +168,9 @@ inline double expected_tiles(const ProductArgs &a, int64_t size) {
   return tiles > met ? tiles : met;
 }
 
-// One of a kernel's shapes, and the microseconds that it is predicted to take (the launch and the first
+constexpr double kMostWorkItems = 4294967295.0;  // of a grid, in one direction
+
+// One of a kernel's shapes (-1: none fits a grid), and the microseconds that it is predicted to take (the launch and the first
 // loads, alike for all, are left out).
 struct Prediction {
   int choice;

@@ -19,11 +19,11 @@ namespace {
 __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride,
                                                          int32_t k, int32_t width, uint16_t *__restrict__ out) {
   const uint32_t pieces = (uint32_t)width / 8;
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / pieces;
-  const int32_t col = (int32_t)(unit - row * pieces) * 8;
-  if (row >= rows) return;
-  const bool whole = aligned16(x) && stride % 8 == 0;
-  *reinterpret_cast<u32x4 *>(out + row * width + col) = load_row8(x + row * stride, col, k, whole);
+  for (int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x; unit < rows * pieces; unit += (int64_t)gridDim.x * 256) {
+    const int64_t row = unit / pieces;
+    const int32_t col = (int32_t)(unit - row * pieces) * 8;
+    *reinterpret_cast<u32x4 *>(out + row * width + col) = load_row8(x + row * stride, col, k);
+  }
 }
 
 int check(const mps_mxfp4_product *p) {
@@ -85,7 +85,7 @@ Way way_of(const mps_mxfp4_product *p) {
   a.bias_type = p->bias_type, a.out_type = p->out_type;
   const int32_t cus = compute_units();
   const Prediction rows = predict_rows(a, p->x_type, cus), tiles = predict_tiles(a, p->x_type, cus);
-  w.tiles = rows.choice < 0 || tiles.us < rows.us;
+  w.tiles = tiles.choice >= 0 && (rows.choice < 0 || tiles.us < rows.us);
   w.choice = w.tiles ? tiles.choice : rows.choice;
   w.packed = p->x_type != MPS_TYPE_MXFP4 && p->k > 0 &&
              !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
@@ -114,6 +114,7 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
   const int rc = check(p);
   if (rc != MPS_OK || p->rows == 0 || p->n == 0) return rc;
   const Way way = way_of(p);
+  if (way.choice < 0) return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: %lld x %lld outputs are too many", (long long)p->rows, (long long)p->n);
   if (way.workspace > 0 && (!workspace || workspace_bytes < way.workspace || !aligned16(workspace)))
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: %lld bytes of workspace are needed, 16-byte aligned",
                 (long long)way.workspace);
@@ -121,7 +122,7 @@ int mps_mxfp4_multiply(const mps_mxfp4_product *p, void *workspace, int64_t work
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (way.packed) {
     const int32_t width = (int32_t)packed_width(p->k);
-    const dim3 grid((unsigned)(((int64_t)a.x_rows * (width / 8) + 255) / 256));
+    const dim3 grid(workgroups(((int64_t)a.x_rows * (width / 8) + 255) / 256));
     hipLaunchKernelGGL(mxfp4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), (int64_t)a.x_rows,
                        p->x_stride, a.k, width, static_cast<uint16_t *>(workspace));
     a.x = workspace, a.x_stride = width, a.k = width;

@@ -273,7 +273,7 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
   const int64_t periods = (a.row_blocks + 15) / 16;
   for (int i = 0; i < N; ++i) {
     const Choice &c = choices[i];
-    if (product_tiles(a, c.rows) > 65535) continue;
+    if (product_tiles(a, c.rows) > 65535 || (double)((a.n + c.cols - 1) / c.cols) * c.waves * 64 > kMostWorkItems) continue;
     const double each = expected_tiles(a, c.rows) * (double)((a.n + c.cols - 1) / c.cols) / ((double)cus * c.resident);
     const double us = (each <= 1 ? 1.0 : __builtin_ceil(each - 0.01)) * (double)((periods + c.waves - 1) / c.waves) * c.us;
     if (best.choice < 0 || us < best.us) best = {i, us};

@@ -14,6 +14,8 @@
 // quarter's fragments are read nobody needs the buffer any more: the barrier stands there, the
 // loads of the step after next are issued behind it, and the next step's first fragments are read
 // while the last quarter is multiplied, so that the matrix cores do not wait for a new buffer.
+// (Two barriers a step, one for each half of x's rows, give loads half a step more to arrive and
+// took 3 % longer.)
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -53,6 +55,7 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, g = lane >> 5;
   const int wt = wave / WN, wn = wave % WN;
 
+  if (a.offsets) tiles_t = count_tiles(a.offsets, a.experts, a.rows, BT);  // the host knows a bound only
   // Workgroups go to the 8 XCDs in turn. Each XCD takes a stretch of the tiles, in which
   // groups of 8 tiles of rows run through the weight's tiles together, so that its L2 serves both.
   const uint32_t total = (uint32_t)tiles_t * (uint32_t)tiles_n;
@@ -355,6 +358,7 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
   Prediction best = {-1, 0};
   for (int i = 0; i < N; ++i) {
     const Choice &c = choices[i];
+    if (((double)product_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) + 8) * 512 > kMostWorkItems) continue;
     const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn), each = __builtin_ceil(tiles / cus - 0.01);
     const double us = (each <= 1 ? c.one : each * c.many) * a.row_blocks / 128;
     if (best.choice < 0 || us < best.us) best = {i, us};

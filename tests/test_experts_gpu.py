@@ -242,6 +242,49 @@ def test_whole_path_in_a_graph():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_block_of_experts(dtype):
+    """The block that serves MXFP4 experts, against 64-bit arithmetic on the same MXFP4 weights. Every step
+    rounds to 16 bits: products, silu, its product with up, the weighted sum and the shared expert's
+    part, and MXFP4 activations are the quantized ones exactly. Each is off by its roundoff, amplified by
+    less than the two products' condition, which the sum of magnitudes of the last one covers."""
+    from mpserve_amd.mxfp4 import mxfp4_quantize
+    from mpserve_amd.mxfp4_experts import Mxfp4Experts, decoded_weight
+
+    t, hidden, ffn, experts, top = 45, 256, 160, 8, 3
+    g = gen(6)
+    device = torch.device(DEV, torch.cuda.current_device())
+    gu, dn = decoded_weight((experts, 2 * ffn, hidden), 1, device), decoded_weight((experts, hidden, ffn), 2, device)
+    sgu, sdn = decoded_weight((2 * ffn, hidden), 3, device), decoded_weight((hidden, ffn), 4, device)
+    block = Mxfp4Experts(gu, dn, top, shared=(sgu, sdn))
+    x = torch.randn(t, hidden, generator=g, device=DEV).to(dtype)
+    logits = torch.randn(t, experts, generator=g, device=DEV)
+    out = block(x, logits)
+    value = lambda pair, k: plain.dequantize(*pair, k)  # noqa: E731
+
+    def gated(h):
+        a, b = h.chunk(2, -1)
+        return a * torch.sigmoid(a) * b
+
+    best, ids = logits.topk(top, dim=1)
+    w = torch.softmax(best, 1).double()
+    wgu, wdn = value(block.gate_up, hidden), value(block.down, ffn)
+    want, size = torch.zeros(t, hidden, dtype=torch.float64, device=DEV), torch.zeros(t, hidden, dtype=torch.float64, device=DEV)
+    for e in range(experts):
+        token, slot = torch.where(ids == e)
+        h = gated(x[token].double() @ wgu[e].T)
+        want[token] += w[token, slot].unsqueeze(1) * (h @ wdn[e].T)
+        size[token] += w[token, slot].unsqueeze(1) * (h.abs() @ wdn[e].abs().T)
+    h = gated(value(mxfp4_quantize(x), hidden) @ value(block.shared[0], hidden).T)
+    want, size = want + h @ value(block.shared[1], ffn).T, size + h.abs() @ value(block.shared[1], ffn).abs().T
+    # gate, up, silu and their product: each rounded, silu's slope is below 1.1, so 4.1 roundoffs of h at most
+    # relative to |gate * up| (which silu's factor shrinks: twice that is taken); the products, sums and the
+    # last addition round four times more.
+    u = plain.ROUNDOFF[dtype]
+    off = (out.double() - want).abs()
+    assert bool((off <= 16 * u * size + 4 * u * want.abs() + 2.0 ** -24).all()), float((off / size).max() / u)
+
+
 def test_refusals():
     ids = routing(0, 6, 2, 4)
     sort = expert_sort(ids, 4)

@@ -259,6 +259,27 @@ def test_linear_output_past_32_bits():
         assert torch.equal(y[rows], (x[rows].double() @ w).float().to(torch.bfloat16))
 
 
+def test_quantize_past_32_bits():
+    """Over 2^32 work-items and 2^35 elements: the last rows are as right as the first."""
+    rows, k = (1 << 20) + 40, 32800
+    if torch.cuda.mem_get_info()[0] < 110 << 30:
+        pytest.skip("needs 110 GB of free memory")
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device=DEV)
+    ends = (slice(0, 2), slice(rows // 2, rows // 2 + 2), slice((1 << 20) - 2, (1 << 20) + 2), slice(rows - 2, rows))
+    for i, part in enumerate(ends):
+        x[part] = torch.randn(x[part].shape, generator=gen(i), device=DEV).to(torch.bfloat16)
+    codes, scales = mxfp4_quantize(x)
+    for part in ends:
+        want_codes, want_scales = plain.quantize(x[part])
+        assert torch.equal(codes[part].cpu(), want_codes) and torch.equal(scales[part].cpu(), want_scales)
+    back = x  # decoded over the input, which is not needed any more
+    mxfp4_dequantize(codes, scales, k, out=back)
+    for part in ends:
+        assert torch.equal(back[part], plain.dequantize(codes[part], scales[part], k).to(torch.bfloat16))
+    del x, back, codes, scales
+    torch.cuda.empty_cache()
+
+
 def test_products_repeat_bit_for_bit():
     g = gen(21)
     for t in (1, 40, 600):
