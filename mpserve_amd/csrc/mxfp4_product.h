@@ -119,27 +119,35 @@ __device__ inline u32x4 move_scales(u32x4 v, int32_t b, int32_t blocks) {
   return past < 16 ? __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (8 * past)) : u32x4{0, 0, 0, 0};
 }
 
-// Four neighbouring columns of a row of the output; `quads`: rows are whole quads at aligned addresses.
-__device__ inline void store4(const ProductArgs &a, int64_t row, int32_t col, f32x4 v, bool quads) {
-  const int64_t at = row * a.n + col;
-  if (!quads) {
-    for (int j = 0; j < 4; ++j)
-      if (col + j < a.n) store_as(a.out, a.out_type, at + j, v[j]);
-  } else if (a.out_type == MPS_TYPE_F32) {
-    *reinterpret_cast<f32x4 *>(static_cast<float *>(a.out) + at) = v;
-  } else {
-    uint64_t h = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      h |= (uint64_t)(a.out_type == MPS_TYPE_BF16 ? Elem<MPS_TYPE_BF16>::put(v[j]) : Elem<MPS_TYPE_F16>::put(v[j])) << (16 * j);
-    *reinterpret_cast<uint64_t *>(static_cast<uint16_t *>(a.out) + at) = h;
-  }
-}
-
 // Two values as 16-bit ones.
 __device__ inline uint32_t pack2(float lo, float hi, int32_t type) {
   if (type == MPS_TYPE_BF16) return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
   return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
+}
+
+// Four neighbouring columns of a row of the output, at any alignment; those past the last are left out.
+__device__ inline void store4(const ProductArgs &a, int64_t row, int32_t col, f32x4 v) {
+  const int64_t at = row * a.n + col;
+  if (col + 4 > a.n) {
+    for (int j = 0; j < 4; ++j)
+      if (col + j < a.n) store_as(a.out, a.out_type, at + j, v[j]);
+  } else if (a.out_type == MPS_TYPE_F32) {
+    *reinterpret_cast<u32x4_any *>(static_cast<float *>(a.out) + at) = __builtin_bit_cast(u32x4, v);
+  } else {
+    typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+    *reinterpret_cast<u32x2_any *>(static_cast<uint16_t *>(a.out) + at) = u32x2_any{pack2(v[0], v[1], a.out_type), pack2(v[2], v[3], a.out_type)};
+  }
+}
+
+// Eight of them.
+__device__ inline void store8(const ProductArgs &a, int64_t row, int32_t col, f32x4 v, f32x4 w) {
+  if (col + 8 > a.n || a.out_type == MPS_TYPE_F32) {
+    store4(a, row, col, v);
+    store4(a, row, col + 4, w);
+  } else {
+    *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(a.out) + row * a.n + col) =
+        u32x4{pack2(v[0], v[1], a.out_type), pack2(v[2], v[3], a.out_type), pack2(w[0], w[1], a.out_type), pack2(w[2], w[3], a.out_type)};
+  }
 }
 
 // The biases of four neighbouring columns; zeros past the last column.

@@ -228,7 +228,6 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
   __syncthreads();
   // In fragment (t, n) lane 16 g + r has rows 16 t + 4 g .. + 3 of column 16 n + r; the waves share
   // the fragments, a lane now taking four columns of row 16 t + lane / 4.
-  const bool quads = a.n % 4 == 0 && aligned16(a.out);
   for (int f = wave; f < kFT * FN; f += W) {
     const int in_row = lane / 4, in_col = lane % 4 * 4;
     const int32_t row = tile.first + f / FN * 16 + in_row, col = n0 + f % FN * 16 + in_col;
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
       for (int j = 0; j < 4; ++j) v[j] += from[4 * j];
     }
     if (a.bias && !none) v += load_bias4(a, tile.expert, col);
-    store4(a, row, col, v, quads);
+    store4(a, row, col, v);
   }
 }
 

@@ -227,7 +227,10 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   for (int32_t p = 0; p < periods; ++p) {
     const int sbuf = p & 1;
     if (p + 1 < periods) get_scales(p + 1);
-    for (int32_t pair = 0; pair < S::kSteps / 2; ++pair) {
+    const int32_t left = blocks - 16 * p;
+#pragma unroll
+    for (int32_t pair = 0; pair < S::kSteps / 2; ++pair) {  // of steps
+      if (pair * (2 * 16 / S::kSteps) >= left) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int32_t in = 2 * pair + i, step = p * S::kSteps + in;
@@ -262,35 +265,64 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   }
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads of steps past the last
-  if constexpr (XT == MPS_TYPE_F16) {
-    // A lane's 16 sums are rows 8 i + 4 g .. + 3 of column r of a fragment. The wave turns 32 rows at a
-    // time round through its own part of LDS, so that stores go along the rows.
+  if constexpr (XT != MPS_TYPE_BF16) {
+    // A lane's 16 sums are places 8 i + 4 g .. + 3 of one side of a fragment, at place r of the other: columns
+    // of one row, or with FP16 x rows of one column. The wave turns 32 rows at a time round through
+    // its own part of LDS, so that a store has whole lines (MXFP4 8192 x 512 x 8192: 56 us as below, 43 so;
+    // BF16, whose shorter tiles end at different times, 460 as below for k = 4096 and 466 so).
     __syncthreads();
-    constexpr int kCols = S::kFN * 32, kPitch = S::kPitch, kLanes = kCols / 4;
+    constexpr int kCols = S::kFN * 32, kPitch = S::kPitch, kLanes = kCols / 8, kPasses = 32 * kLanes / 64;
     float *mine = reinterpret_cast<float *>(lds) + wave * 32 * kPitch;
-    const bool whole = a.n % 4 == 0 && aligned16(a.out);
-    const int32_t col = n0 + wn * kCols + lane % kLanes * 4;
-    f32x4 bias = {0, 0, 0, 0};
-    if (a.bias && !none) bias = load_bias4(a, tile.expert, col);
+    const int32_t col = n0 + wn * kCols + lane % kLanes * 8;
+    f32x4 bias[2] = {};
+    if (a.bias && !none) bias[0] = load_bias4(a, tile.expert, col), bias[1] = load_bias4(a, tile.expert, col + 4);
 #pragma unroll
     for (int t = 0; t < S::kFT; ++t) {
 #pragma unroll
       for (int n = 0; n < S::kFN; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mine[(8 * (i / 4) + 4 * g + i % 4) * kPitch + n * 32 + r] = acc[t][n][i];
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (k4) {
+            *reinterpret_cast<f32x4 *>(mine + r * kPitch + n * 32 + 8 * i + 4 * g) =
+                f32x4{acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]};
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mine[(8 * i + 4 * g + j) * kPitch + n * 32 + r] = acc[t][n][4 * i + j];
+          }
+        }
       __builtin_amdgcn_wave_barrier();
-      for (int in = lane / kLanes; in < 32; in += 64 / kLanes) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(mine + in * kPitch + lane % kLanes * 4);
-        const int32_t row = tile.first + (wt * S::kFT + t) * 32 + in;
-        if (row < tile.end && col < a.n) store4(a, row, col, f32x4{v[0] + bias[0], v[1] + bias[1], v[2] + bias[2], v[3] + bias[3]}, whole);
+      f32x4 v[kPasses][2];
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[i][h] = *reinterpret_cast<const f32x4 *>(mine + (i * (64 / kLanes) + lane / kLanes) * kPitch + lane % kLanes * 8 + 4 * h) + bias[h];
+      __builtin_amdgcn_wave_barrier();
+      const int32_t row = tile.first + (wt * S::kFT + t) * 32 + lane / kLanes;
+      auto store = [&](auto typed) {  // whole 16-byte pieces of a known type
+        uint16_t *to = static_cast<uint16_t *>(a.out) + (int64_t)row * a.n + col;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i, to += (int64_t)(64 / kLanes) * a.n) {
+          const f32x4 lo = v[i][0], hi = v[i][1];
+          constexpr int32_t type = decltype(typed)::value;
+          const u32x4 piece = {pack2(lo[0], lo[1], type), pack2(lo[2], lo[3], type), pack2(hi[0], hi[1], type), pack2(hi[2], hi[3], type)};
+          if (row + i * (64 / kLanes) < tile.end) *reinterpret_cast<u32x4_any *>(to) = piece;
+        }
+      };
+      if (a.out_type == MPS_TYPE_BF16 && n0 + BN <= a.n) {
+        store(std::integral_constant<int32_t, MPS_TYPE_BF16>{});
+      } else if (a.out_type == MPS_TYPE_F16 && n0 + BN <= a.n) {
+        store(std::integral_constant<int32_t, MPS_TYPE_F16>{});
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i)
+          if (row + i * (64 / kLanes) < tile.end) store8(a, row + i * (64 / kLanes), col, v[i][0], v[i][1]);
       }
-      __builtin_amdgcn_wave_barrier();
     }
   } else {
     // A lane's 16 sums are columns 8 i + 4 g .. + 3 of row r of a fragment. For 16-bit outputs lanes r and
     // r + 32 trade, so that each has eight neighbouring columns.
-    const bool whole = a.n % 8 == 0 && aligned16(a.out);
-    const bool wide = whole && a.out_type != MPS_TYPE_F32;
+    const bool wide = a.out_type != MPS_TYPE_F32;
 #pragma unroll
     for (int n = 0; n < S::kFN; ++n) {
       const int32_t col = n0 + (wn * S::kFN + n) * 32;
@@ -316,15 +348,22 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
             const auto lo = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
             const auto hi = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
             const int32_t at = col + 16 * i + 8 * g;
-            if (row < tile.end && at < a.n)
-              *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (int64_t)row * a.n + at) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+            const u32x4 v = {lo[0], hi[0], lo[1], hi[1]};
+            uint16_t *const to = static_cast<uint16_t *>(a.out) + (int64_t)row * a.n + at;
+            if (row < tile.end && at + 8 <= a.n) {
+              *reinterpret_cast<u32x4_any *>(to) = v;
+            } else if (row < tile.end) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (at + j < a.n) to[j] = (uint16_t)(v[j / 2] >> (16 * (j % 2)));
+            }
           }
         } else if (row < tile.end) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int32_t at = col + 8 * i + 4 * g;
             if (at < a.n)
-              store4(a, row, at, f32x4{acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]}, whole);
+              store4(a, row, at, f32x4{acc[t][n][4 * i], acc[t][n][4 * i + 1], acc[t][n][4 * i + 2], acc[t][n][4 * i + 3]});
           }
         }
       }
@@ -340,18 +379,20 @@ void launch(const ProductArgs &a, hipStream_t stream) {
                      (int32_t)tt, (int32_t)tn);
 }
 
-// The tiles. `one` and `many` are the microseconds, at k = 4096, of a tile that has a CU to itself and
-// of each of several (measured: 128 x 8192 x 8192 and 1024 x 4096 x 4096 for the first, 4096 x 4096 x
-// 14336 for the second). So BF16 4096 x 4096 x 14336 takes 128 x 256 tiles, 398 us where 128 x 128 take
-// 449, and 512 x 2048 x 1024 takes 64 x 64, 14 us where 128 x 256 take 30. (BF16 in tiles of 256 x 256, one
-// workgroup of eight waves a CU: 417 us; MXFP4 in 128 x 256, 16 % slower than 256 x 256.)
+// The tiles, in microseconds. `start` is what a tile takes at any k, for its first loads and its stores
+// (8192 x 32 x 8192); `one` and `many` are what k = 4096 adds to a tile that has a CU to itself (128 x 8192 x
+// 8192 and 1024 x 4096 x 4096) and to each of several (4096 x 4096 x 14336). So BF16 4096 x 4096 x 14336 takes
+// 128 x 256 tiles, 398 us where 128 x 128 take 449, and 512 x 2048 x 1024 takes 64 x 64, 14 us where 128 x
+// 256 take 30. (BF16 in tiles of 256 x 256, one workgroup of eight waves a CU: 417 us; MXFP4 in 128 x
+// 256, 16 % slower than 256 x 256.)
 struct Choice {
   int32_t bt, bn;
-  float one, many;
+  float start, one, many;
 };
-constexpr Choice kChoices4[] = {{256, 256, 29.0f, 34.5f}, {128, 128, 14.0f, 10.9f}, {64, 64, 10.4f, 6.4f}};
-constexpr Choice kChoicesBf16[] = {{128, 256, 56.0f, 57.0f}, {128, 128, 38.0f, 32.0f}, {64, 128, 28.0f, 20.5f}, {64, 64, 26.0f, 15.0f}};
-constexpr Choice kChoicesF16[] = {{128, 128, 52.0f, 40.0f}, {64, 128, 35.0f, 23.0f}, {64, 64, 29.0f, 15.7f}};
+constexpr Choice kChoices4[] = {{256, 256, 10.5f, 18.0f, 27.0f}, {128, 128, 3.0f, 11.0f, 8.5f}, {64, 64, 1.5f, 8.9f, 4.2f}};
+constexpr Choice kChoicesBf16[] = {
+    {128, 256, 4.6f, 51.0f, 53.0f}, {128, 128, 2.6f, 35.0f, 30.0f}, {64, 128, 1.8f, 26.0f, 18.5f}, {64, 64, 1.45f, 24.5f, 13.4f}};
+constexpr Choice kChoicesF16[] = {{128, 128, 2.7f, 49.0f, 37.5f}, {64, 128, 1.8f, 33.0f, 21.1f}, {64, 64, 1.4f, 27.5f, 14.2f}};
 
 template <int N>
 Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
@@ -359,8 +400,14 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
   for (int i = 0; i < N; ++i) {
     const Choice &c = choices[i];
     if (((double)product_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) + 8) * 512 > kMostWorkItems) continue;
-    const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn), each = __builtin_ceil(tiles / cus - 0.01);
-    const double us = (each <= 1 ? c.one : each * c.many) * a.row_blocks / 128;
+    const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) / cus, k = a.row_blocks / 128.0;
+    // The count of experts' tiles is a guess: the mean over a tenth less and more, lest a second round of
+    // a few tiles comes unawares (468 rows of 60 experts, k = 5016, n = 896, had 264 for 256 CUs).
+    double us = 0;
+    for (int j = -1; j <= 1; ++j) {
+      const double each = __builtin_ceil(tiles * (a.offsets ? 1 + 0.1 * j : 1) - 0.01);
+      us += (each <= 1 ? c.start + c.one * k : each * (c.start + c.many * k)) / 3;
+    }
     if (best.choice < 0 || us < best.us) best = {i, us};
   }
   return best;
