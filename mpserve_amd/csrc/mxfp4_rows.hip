@@ -8,7 +8,7 @@
 //
 // A stage is U cache lines of every row of x (64 U elements of 16 bits, or 256 codes, U = 1) and the
 // weights of the same k, 32 U bytes a row, or 128 beside MXFP4 x: the more, the fewer instructions and
-// waits a byte (one token through 4096 x 14336: U = 1 9.1 us, U = 4 @U4@), the fewer, the more rows
+// waits a byte (one token through 4096 x 14336: U = 1 9.1 us, U = 4 7.5), the fewer, the more rows
 // of x fit. Pieces of 16 bytes lie in rows as in mxfp4_tile.hip: piece p of row r of x at place
 // p ^ (r / 2 % 8), of P pieces of a weight row at p ^ (r / (16 / P)).
 // In a lane 16 g + r of a 16-row fragment, MXFP4 takes pieces 2 g and 2 g + 1 of row r, and 16-bit x

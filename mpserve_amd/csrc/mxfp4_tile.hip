@@ -8,14 +8,19 @@
 // eight, or p ^ (r / 8 % 2) of two: the sixteen lanes that LDS serves in a cycle (0-3, 12-15, 20-27
 // and 4-11, 16-19, 28-31, and so on) then meet all 64 banks once. With r % 8 half of LDS's cycles
 // were conflicts. (Stages of 64 bytes a row, four of them, halve the lines' use: 1177 us for 8192 x
-// 8192 x 28672 where these took 1030.)
+// 8192 x 28672 where these took 1030 then.)
 //
 // A step is multiplied in quarters, each from fragments read during the one before. Once the last
 // quarter's fragments are read nobody needs the buffer any more: the barrier stands there, the
-// loads of the step after next are issued behind it, and the next step's first fragments are read
-// while the last quarter is multiplied, so that the matrix cores do not wait for a new buffer.
-// (Two barriers a step, one for each half of x's rows, give loads half a step more to arrive and
-// took 3 % longer.)
+// loads of the step after next are issued among that quarter's products, and the next step's first
+// fragments are read there too, so that the matrix cores do not wait for a new buffer. (All loads before
+// the quarter: BF16 4096 x 4096 x 14336 411 us where these take 403, MXFP4 alike. Two barriers a
+// step, one for each half of x's rows, give loads half a step more to arrive and took 3 % longer.)
+//
+// What bounds it: BF16 the matrix cores, at 97 % of what the library's BF16 product of that size reaches
+// beside the widening. MXFP4 8192 x 8192 x 28672 takes 955 us, 4.0 PFLOP/s: the matrix cores are
+// busy for 52 % of the cycles, at clocks that the load brings down; without any loads to LDS and barriers
+// it would take 770, without stores 870.
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -77,10 +82,10 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   // first row, cut at the last, finds every piece; gathered rows need an address each.
   const int64_t x_row_bytes = k4 ? (int64_t)blocks * 16 : a.x_stride * 2;
   const uint32_t w_row_bytes = (uint32_t)blocks * 16;
-  const int w_at = wave * S::kWLanes + lane;  // of the first load's pieces
-  const int xrow = tid / 8, wrow = w_at / S::kWPieces;
+  const int w_first_piece = wave * S::kWLanes + lane;  // of the first load's
+  const int xrow = tid / 8, wrow = w_first_piece / S::kWPieces;
   const int32_t x_piece = (tid % 8) ^ (xrow >> 1 & 7);
-  const int32_t w_piece = k4 ? (w_at % 8) ^ (wrow >> 1 & 7) : (w_at % 2) ^ (wrow >> 3 & 1);
+  const int32_t w_piece = k4 ? (w_first_piece % 8) ^ (wrow >> 1 & 7) : (w_first_piece % 2) ^ (wrow >> 3 & 1);
   const int64_t w_first = (int64_t)(none ? 0 : tile.expert) * a.n + n0;
   const uint8_t *const w_base = a.w + w_first * w_row_bytes;
   const uint32_t w_last = (uint32_t)min(BN - 1, a.n - 1 - n0) * w_row_bytes;
@@ -106,21 +111,23 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
       s_from[i] = a.w_scales + (w_first + min(min(row, BN - 1), a.n - 1 - n0)) * blocks;
   }
   const int32_t x_pieces = k4 ? blocks : blocks * 4;
-  auto fetch = [&](int32_t step, int buffer) {
+  // Loads `from` to `to` of a step, x's before the weights'.
+  constexpr int kLoads = S::kXLoads + S::kWLoads;
+  auto fetch = [&](int32_t step, int buffer, int from, int to) {
     uint8_t *const xt = xs + buffer * S::kXBytes + wave * 1024, *const wt = ws + buffer * S::kWBytes + wave * S::kWLanes * 16;
     const uint32_t x_at = (uint32_t)min(step * 8 + x_piece, x_pieces - 1) * 16;
+    const uint32_t w_at = (uint32_t)min(step * S::kWPieces + w_piece, blocks - 1) * 16;
 #pragma unroll
-    for (int i = 0; i < S::kXLoads; ++i) {
-      if constexpr (k4)
+    for (int l = from; l < to; ++l) {
+      const int i = l < S::kXLoads ? l : l - S::kXLoads;
+      if (l >= S::kXLoads) {
+        if (S::kWLanes == 64 || lane < S::kWLanes)
+          copy16(w_base + (min((uint32_t)(wrow + i * (S::kThreads / S::kWPieces)) * w_row_bytes, w_last) + w_at), wt + i * S::kThreads * 16);
+      } else if constexpr (k4) {
         copy16(x_base + (min((uint32_t)(xrow + i * (S::kThreads / 8)) * (uint32_t)x_row_bytes, x_last) + x_at), xt + i * S::kThreads * 16);
-      else
+      } else {
         copy16(x_from[i] + x_at, xt + i * S::kThreads * 16);
-    }
-    const uint32_t at = (uint32_t)min(step * S::kWPieces + w_piece, blocks - 1) * 16;
-    if (S::kWLanes == 64 || lane < S::kWLanes) {
-#pragma unroll
-      for (int i = 0; i < S::kWLoads; ++i)
-        copy16(w_base + (min((uint32_t)(wrow + i * (S::kThreads / S::kWPieces)) * w_row_bytes, w_last) + at), wt + i * S::kThreads * 16);
+      }
     }
   };
   // Scales come 16 blocks at a time, a period ahead, through registers.
@@ -213,11 +220,11 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   };
 
   if (periods > 0) {
-    fetch(0, 0);
+    fetch(0, 0, 0, kLoads);
     get_scales(0);
     put_scales(0, 0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    fetch(1, 1);
+    fetch(1, 1, 0, kLoads);
     read(0, 0, 0, 0);
     if constexpr (XT == MPS_TYPE_F16) read(1, 0, 0, 0);
   }
@@ -251,14 +258,18 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
           } else {
             read(q + 1, i, in, sbuf);
           }
+          if constexpr (q == 3) {
+            fetch(step + 2, i, 0, kLoads / 2);
+            __builtin_amdgcn_sched_barrier(0);
+          }
           if (has[q >> 1]) multiply(qc, in, 1, S::kFN);
+          if constexpr (q == 3) fetch(step + 2, i, kLoads / 2, kLoads);
         };
         if constexpr (XT != MPS_TYPE_F16) quarter(std::integral_constant<int, 0>{});
         quarter(std::integral_constant<int, 1>{});
         if constexpr (XT != MPS_TYPE_F16) quarter(std::integral_constant<int, 2>{});
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (in == S::kSteps - 2) put_scales(p + 1, sbuf ^ 1);
-        fetch(step + 2, i);
         quarter(std::integral_constant<int, 3>{});
       }
     }
