@@ -98,6 +98,17 @@ def _gather_rows(x: torch.Tensor, order: torch.Tensor, positions: torch.Tensor, 
     return rows
 
 
+def _first_gradient(backward):
+    """``once_differentiable``, whose wrapper costs 5 us of a small backward's 45, only where a graph of the
+    gradients is being made."""
+    once = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, grad):
+        return once(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+
+    return run
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, positions, offsets):
@@ -105,7 +116,7 @@ class _Gather(torch.autograd.Function):
         return _gather_rows(x, order, positions, offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_gradient
     def backward(ctx, drows):
         (positions,) = ctx.saved_tensors
         return _sum_rows(drows.contiguous(), None, positions), None, None, None
@@ -118,7 +129,7 @@ class _Combine(torch.autograd.Function):
         return _sum_rows(y, weights, positions)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_gradient
     def backward(ctx, dout):
         y, weights, order, positions, offsets = ctx.saved_tensors
         t, top = weights.shape

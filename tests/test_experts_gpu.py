@@ -202,6 +202,19 @@ def test_bad_orders_and_offsets_stay_in_bounds():
     torch.cuda.synchronize()
 
 
+def test_no_second_gradient():
+    """A graph of the gradients may be asked for; a gradient through it is refused."""
+    sort = expert_sort(torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device=DEV), 3)
+    x = torch.randn(2, 8, device=DEV, requires_grad=True)
+    weights = torch.rand(2, 2, device=DEV, requires_grad=True)
+    out = expert_combine(expert_gather(x, sort), weights, sort)
+    once = torch.autograd.grad(out.square().sum(), (x, weights), retain_graph=True)
+    again = torch.autograd.grad(out.square().sum(), (x, weights), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, again))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        again[0].sum().backward()
+
+
 def test_whole_path_in_a_graph():
     """Sort, product, weighted sum and gradients, captured once and replayed on new routings and tokens."""
     t, top, experts, k, n = 50, 4, 16, 256, 136
