@@ -261,8 +261,11 @@ struct Choice {
   int32_t rows, cols, waves, resident;
   float us;
 };
-constexpr Choice kChoices16[] = {{8, 32, 4, 2, 2.5f}, {8, 32, 8, 1, 2.7f}, {16, 32, 8, 1, 3.2f}, {16, 64, 4, 1, 2.8f},
-                                 {32, 32, 6, 1, 3.2f}, {32, 64, 4, 1, 3.8f}, {64, 64, 4, 1, 6.2f}};
+constexpr Choice kChoicesBf16[] = {{8, 32, 4, 2, 2.5f}, {8, 32, 8, 1, 2.7f}, {16, 32, 8, 1, 3.2f}, {16, 64, 4, 1, 2.8f},
+                                   {32, 32, 6, 1, 3.2f}, {32, 64, 4, 1, 3.8f}, {64, 64, 4, 1, 6.2f}};
+// FP16's scaled sums cost more, the more rows (64 x 2048 x 8192 with XL 4, FN 4 7.1 us in BF16, 9.8 in FP16).
+constexpr Choice kChoicesF16[] = {{8, 32, 4, 2, 3.1f}, {8, 32, 8, 1, 3.4f}, {16, 32, 8, 1, 3.8f}, {16, 64, 4, 1, 3.6f},
+                                  {32, 32, 6, 1, 3.8f}, {32, 64, 4, 1, 5.6f}, {64, 64, 4, 1, 9.6f}};
 constexpr Choice kChoices4[] = {{8, 32, 4, 2, 1.9f}, {8, 32, 8, 1, 2.2f}, {16, 32, 4, 2, 1.9f}, {16, 32, 8, 1, 2.3f},
                                 {32, 64, 4, 1, 2.5f}, {64, 32, 6, 1, 2.7f}};
 
@@ -307,7 +310,8 @@ void launch_type(const ProductArgs &a, int choice, hipStream_t stream) {
 }  // namespace
 
 Prediction predict_rows(const ProductArgs &a, int32_t x_type, int32_t cus) {
-  return x_type == MPS_TYPE_MXFP4 ? least(a, kChoices4, cus) : least(a, kChoices16, cus);
+  if (x_type == MPS_TYPE_MXFP4) return least(a, kChoices4, cus);
+  return x_type == MPS_TYPE_BF16 ? least(a, kChoicesBf16, cus) : least(a, kChoicesF16, cus);
 }
 
 void launch_rows(const ProductArgs &a, int32_t x_type, int choice, hipStream_t stream) {

@@ -118,7 +118,7 @@ SHAPES = [  # t, k, n
     (130, 500, 1030), (500, 500, 520), (70, 500, 20000), (1, 500, 20000), (60, 320, 100),
     # enough tiles for each of the larger ones, ends of rows and columns inside them, one block to several periods of k
     (700, 96, 4300), (1100, 64, 8300), (2100, 32, 8300), (2300, 704, 8500), (4500, 160, 5000), (9000, 544, 2100),
-    (200, 608, 5000), (250, 1030, 4101), (1000, 1030, 8195), (2000, 1030, 4101),
+    (200, 608, 5000), (250, 1030, 4101), (1000, 1030, 8195), (2000, 1030, 4101), (130, 4100, 5000),
 ]
 
 
