@@ -18,7 +18,7 @@
 // step, one for each half of x's rows, give loads half a step more to arrive and took 3 % longer.)
 //
 // What bounds it: BF16 the matrix cores, at 97 % of what the library's BF16 product of that size reaches
-// beside the widening. MXFP4 8192 x 8192 x 28672 takes 955 us, 4.0 PFLOP/s: the matrix cores are
+// beside the widening. MXFP4 8192 x 8192 x 28672 takes 955 to 985 us, 4.0 PFLOP/s: the matrix cores are
 // busy for 52 % of the cycles, at clocks that the load brings down; without any loads to LDS and barriers
 // it would take 770, without stores 870.
 #include "mxfp4_product.h"
