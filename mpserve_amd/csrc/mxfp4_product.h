@@ -176,6 +176,15 @@ inline double expected_tiles(const ProductArgs &a, int64_t size) {
   return tiles > met ? tiles : met;
 }
 
+// The share of these tiles that have rows in their first half only: an expert's last tile is one or not, but
+// where experts have less than half a tile each, all are.
+inline double expected_halves(const ProductArgs &a, int64_t size) {
+  if (!a.offsets || a.rows == 0) return 0;
+  const double met = a.experts * (1.0 - __builtin_exp(-(double)a.rows / a.experts)), fill = a.rows / met / (double)size;
+  const double share = fill <= 0.4 ? 1.0 : fill >= 0.6 ? 0.5 : 1.0 - 2.5 * (fill - 0.4);
+  return share * met / expected_tiles(a, size);
+}
+
 constexpr double kMostWorkItems = 4294967295.0;  // of a grid, in one direction
 
 // One of a kernel's shapes (-1: none fits a grid), and the microseconds that it is predicted to take (the launch and the first

@@ -259,15 +259,17 @@ void launch(const ProductArgs &a, hipStream_t stream) {
 // takes 7.5 for 1 x 4096 x 14336 where the first takes 10.0.
 struct Choice {
   int32_t rows, cols, waves, resident;
-  float us;
+  float us, start;
 };
-constexpr Choice kChoicesBf16[] = {{8, 32, 4, 2, 2.5f}, {8, 32, 8, 1, 2.7f}, {16, 32, 8, 1, 3.2f}, {16, 64, 4, 1, 2.8f},
-                                   {32, 32, 6, 1, 3.2f}, {32, 64, 4, 1, 3.8f}, {64, 64, 4, 1, 6.2f}};
+// Workgroups past the first on a CU cost `start` each beside (1200 to 8000 rows of 60 and 64 experts; 1200 rows of
+// 64 experts, 4096 x 2048, in BF16: 93 us with XL 4, FN 4, and 81 in tiles of 128 x 256, which are taken).
+constexpr Choice kChoicesBf16[] = {{8, 32, 4, 2, 2.5f, 1.3f}, {8, 32, 8, 1, 2.7f, 1.9f}, {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 4, 1, 2.8f, 2.1f},
+                                   {32, 32, 6, 1, 3.2f, 1.2f}, {32, 64, 4, 1, 3.8f, 2.7f}, {64, 64, 4, 1, 6.2f, 3.5f}};
 // FP16's scaled sums cost more, the more rows (64 x 2048 x 8192 with XL 4, FN 4 7.1 us in BF16, 9.8 in FP16).
-constexpr Choice kChoicesF16[] = {{8, 32, 4, 2, 3.1f}, {8, 32, 8, 1, 3.4f}, {16, 32, 8, 1, 3.8f}, {16, 64, 4, 1, 3.6f},
-                                  {32, 32, 6, 1, 3.8f}, {32, 64, 4, 1, 5.6f}, {64, 64, 4, 1, 9.6f}};
-constexpr Choice kChoices4[] = {{8, 32, 4, 2, 1.9f}, {8, 32, 8, 1, 2.2f}, {16, 32, 4, 2, 1.9f}, {16, 32, 8, 1, 2.3f},
-                                {32, 64, 4, 1, 2.5f}, {64, 32, 6, 1, 2.7f}};
+constexpr Choice kChoicesF16[] = {{8, 32, 4, 2, 3.1f, 1.3f}, {8, 32, 8, 1, 3.4f, 1.9f}, {16, 32, 8, 1, 3.8f, 2.5f}, {16, 64, 4, 1, 3.6f, 2.1f},
+                                  {32, 32, 6, 1, 3.8f, 1.2f}, {32, 64, 4, 1, 5.6f, 2.7f}, {64, 64, 4, 1, 9.6f, 3.5f}};
+constexpr Choice kChoices4[] = {{8, 32, 4, 2, 1.9f, 0}, {8, 32, 8, 1, 2.2f, 0}, {16, 32, 4, 2, 1.9f, 0}, {16, 32, 8, 1, 2.3f, 0},
+                                {32, 64, 4, 1, 2.5f, 0}, {64, 32, 6, 1, 2.7f, 0}};
 
 template <int N>
 Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
@@ -277,7 +279,8 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
     const Choice &c = choices[i];
     if (product_tiles(a, c.rows) > 65535 || (double)((a.n + c.cols - 1) / c.cols) * c.waves * 64 > kMostWorkItems) continue;
     const double each = expected_tiles(a, c.rows) * (double)((a.n + c.cols - 1) / c.cols) / ((double)cus * c.resident);
-    const double us = (each <= 1 ? 1.0 : __builtin_ceil(each - 0.01)) * (double)((periods + c.waves - 1) / c.waves) * c.us;
+    const double rounds = each <= 1 ? 1.0 : __builtin_ceil(each - 0.01);
+    const double us = rounds * (double)((periods + c.waves - 1) / c.waves) * c.us + (each > 1 ? each - 1 : 0) * c.start;
     if (best.choice < 0 || us < best.us) best = {i, us};
   }
   return best;
