@@ -409,17 +409,16 @@ void launch(const ProductArgs &a, hipStream_t stream) {
 // 8192 and 1024 x 4096 x 4096) and to each of several (4096 x 4096 x 14336). So BF16 4096 x 4096 x 14336 takes
 // 128 x 256 tiles, 398 us where 128 x 128 take 449, and 512 x 2048 x 1024 takes 64 x 64, 14 us where 128 x
 // 256 take 30. (BF16 in tiles of 256 x 256, one workgroup of eight waves a CU: 417 us; MXFP4 in 128 x
-// 256, 16 % slower than 256 x 256.) `half` is the share that one of several tiles spares if its rows are in its first half only
-// (2400 rows of 64 experts, 4096 x 2048, in BF16: 86 us in 128 x 256, 100 in 64 x 128, which
-// would be taken without it).
+// 256, 16 % slower than 256 x 256.) `half` is the share that one of several tiles spares if its rows are in
+// its first half only (2400 rows of 64 experts, 4096 x 2048, in BF16: 85 us in 128 x 256, 100 in 64 x 128).
 struct Choice {
   int32_t bt, bn;
   float start, one, many, half;
 };
 constexpr Choice kChoices4[] = {{256, 256, 10.5f, 18.0f, 27.0f, 0}, {128, 128, 3.0f, 11.0f, 8.5f, 0}, {64, 64, 1.5f, 8.9f, 4.2f, 0}};
 constexpr Choice kChoicesBf16[] = {
-    {128, 256, 4.6f, 51.0f, 53.0f, 0.25f}, {128, 128, 2.6f, 35.0f, 30.0f, 0}, {64, 128, 1.8f, 26.0f, 18.5f, 0}, {64, 64, 1.45f, 24.5f, 13.4f, 0}};
-constexpr Choice kChoicesF16[] = {{128, 128, 2.7f, 49.0f, 37.5f, 0.25f}, {64, 128, 1.8f, 33.0f, 21.1f, 0}, {64, 64, 1.4f, 27.5f, 14.2f, 0}};
+    {128, 256, 4.6f, 51.0f, 53.0f, 0.35f}, {128, 128, 2.6f, 35.0f, 30.0f, 0}, {64, 128, 1.8f, 26.0f, 18.5f, 0}, {64, 64, 1.45f, 24.5f, 13.4f, 0}};
+constexpr Choice kChoicesF16[] = {{128, 128, 2.7f, 49.0f, 37.5f, 0.35f}, {64, 128, 1.8f, 33.0f, 21.1f, 0}, {64, 64, 1.4f, 27.5f, 14.2f, 0}};
 
 template <int N>
 Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) {
@@ -428,13 +427,17 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
     const Choice &c = choices[i];
     if (((double)product_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) + 8) * 512 > kMostWorkItems) continue;
     const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) / cus, k = a.row_blocks / 128.0;
-    // The count of experts' tiles is a guess: the mean over a tenth less and more, lest a second round of
-    // a few tiles comes unawares (468 rows of 60 experts, k = 5016, n = 896, had 264 for 256 CUs).
+    // The count of experts' tiles is a guess, unless most have one: the mean over a tenth less and more, lest a
+    // second round of a few tiles comes unawares (1872 rows of 60 experts, k = 5016, n = 896, had 264 for 256
+    // CUs). Experts' weights are no other tile's, and come later (`start` by 3.5 us: 64 x 64 and 64 x 128
+    // took 147 and 95 us for 1200 rows of 64 experts, 4096 x 2048, where 119 and 81 would follow).
+    const bool sure = a.rows >= 4.0 * a.experts && a.rows <= 0.6 * c.bt * a.experts;
+    const double start = c.start + (a.offsets ? 3.5 : 0), spread = a.offsets && !sure ? 0.1 : 0;
     const double whole = 1 - c.half * expected_halves(a, c.bt);
     double us = 0;
     for (int j = -1; j <= 1; ++j) {
-      const double each = __builtin_ceil(tiles * (a.offsets ? 1 + 0.1 * j : 1) - 0.01);
-      us += (each <= 1 ? c.start + c.one * k : each * (c.start + c.many * k) * whole) / 3;
+      const double each = __builtin_ceil(tiles * (1 + spread * j) - 0.01);
+      us += (each <= 1 ? start + c.one * k : each * (start + c.many * k) * whole) / 3;
     }
     if (best.choice < 0 || us < best.us) best = {i, us};
   }
