@@ -334,8 +334,9 @@ int mps_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t ro
  * w in MXFP4 and x in BF16, FP16 or MXFP4; FP32 sums, one rounding to
  * out_type. With experts > 0, w is [experts, n, k] and bias [experts, n]:
  * rows offsets[e] .. offsets[e + 1] are multiplied by expert e's weight and
- * rows from offsets[experts] on are set to zero. With `gather`, row j of the
- * product is made of x's row order[j] / top instead of its row j. The offsets
+ * rows from offsets[experts] on are set to zero. With `gather`, for 16-bit x
+ * only, row j of the product is made of x's row order[j] / top instead of its
+ * row j; MXFP4 x comes in the sorted order. The offsets
  * and the order are mps_expert_sort's (or hold its promises: offsets rise
  * from 0 to at most rows, the order's entries are below the rows of x times
  * top). Codes are 16-byte aligned; those past column k in a row's last block

@@ -44,6 +44,17 @@ def test_c_entries_refuse_bad_arguments():
         assert lib.mps_mxfp4_multiply(args, None, 0, None) == _native.MPS_ERR_INVALID_ARGUMENT, change
 
 
+def test_gather_of_mxfp4_rows_is_refused():
+    """MXFP4 x has rows / top rows where it is gathered, but is read by sorted place: none of it may be launched."""
+    lib = _native.lib()
+    p = ctypes.c_void_p(4096)  # never read
+    args = _native.MpsMxfp4Product(x=p, x_scales=p, w=p, w_scales=p, out=p, offsets=p, order=p, rows=8, n=8, k=32, experts=2, top=2,
+                                   gather=1, x_type=_native.MPS_TYPE_MXFP4)
+    need = ctypes.c_int64(0)
+    for rc in (lib.mps_mxfp4_multiply(args, None, 0, None), lib.mps_mxfp4_product_workspace(args, need)):
+        assert rc == _native.MPS_ERR_INVALID_ARGUMENT and b"16-bit" in lib.mps_last_error()
+
+
 def test_plain_quantization_known_answers():
     """The oracle of these tests against a block worked out by hand: the largest element 5 has floor(log2) 2, so the
     scale is 2^0; 5 is halfway between 4 (code 6, even) and 6, 0.75 between 0.5 and 1 (code 2, even)."""
