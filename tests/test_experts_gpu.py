@@ -174,6 +174,36 @@ def test_expert_linear_whole_numbers_are_exact(dtype, t, top, experts, k, n, dro
     assert torch.equal(out.double(), want)
 
 
+@pytest.mark.parametrize("t,top,experts,k,n,dropped", EXPERT_CASES)
+def test_mxfp4_rows_of_experts_are_exact(t, top, experts, k, n, dropped):
+    """MXFP4 x in the sorted order, which the C entry takes: the same products with whole numbers, through
+    the kernels of few and of many rows, uneven loads and pairs of no expert."""
+    import ctypes
+
+    from mpserve_amd import _native
+
+    g = gen(t + k)
+    ids = routing(t + n, t, top, experts, 2.0 * dropped)
+    rows = ids.numel()
+    sort = expert_sort(ids, experts)
+    xc, xs = plain.random_weight(g, (rows,), k, DEV, 126, 129)
+    codes, scales = plain.random_weight(g, (experts, n), k, DEV, 126, 129)
+    bias = torch.randint(-64, 65, (experts, n), generator=g, device=DEV).float()
+    x = plain.dequantize(xc, xs, k)
+    offsets = plain.sort(ids, experts)[2].tolist()
+    want = torch.zeros(rows, n, dtype=torch.float64, device=DEV)
+    for e in range(experts):
+        a, b = offsets[e], offsets[e + 1]
+        if b > a:
+            want[a:b] = x[a:b] @ plain.dequantize(codes[e], scales[e], k).T + bias[e].double()
+    out = torch.full((rows, n), float("nan"), device=DEV)
+    p = _native.MpsMxfp4Product(x=xc.data_ptr(), x_scales=xs.data_ptr(), w=codes.data_ptr(), w_scales=scales.data_ptr(), bias=bias.data_ptr(),
+                                out=out.data_ptr(), offsets=sort.offsets.data_ptr(), rows=rows, n=n, k=k, experts=experts, top=ids.shape[1],
+                                x_type=_native.MPS_TYPE_MXFP4, bias_type=_native.MPS_TYPE_F32, out_type=_native.MPS_TYPE_F32)
+    _native.check(_native.lib().mps_mxfp4_multiply(p, None, 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert torch.equal(out.double(), want)
+
+
 def test_expert_linear_without_rows_or_terms():
     sort = expert_sort(torch.empty(0, 2, dtype=torch.int32, device=DEV), 4)
     codes, scales = plain.random_weight(gen(0), (4, 8), 64, DEV)
