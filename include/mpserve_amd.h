@@ -336,7 +336,7 @@ int mps_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t ro
  * rows offsets[e] .. offsets[e + 1] are multiplied by expert e's weight and
  * rows from offsets[experts] on are set to zero. With `gather`, for 16-bit x
  * only, row j of the product is made of x's row order[j] / top instead of its
- * row j; MXFP4 x comes in the sorted order. The offsets
+ * row j, of x's rows / top rows; MXFP4 x comes in the sorted order. The offsets
  * and the order are mps_expert_sort's (or hold its promises: offsets rise
  * from 0 to at most rows, the order's entries are below the rows of x times
  * top). Codes are 16-byte aligned; those past column k in a row's last block

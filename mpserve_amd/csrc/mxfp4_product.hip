@@ -50,6 +50,9 @@ int check(const mps_mxfp4_product *p) {
   if (p->experts > 0 && !p->offsets) return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: experts need offsets");
   if (p->gather && (p->experts == 0 || !p->order || p->top <= 0))
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: a gather needs experts, the sorted order and top > 0");
+  // x has rows / top rows, of which the kernels take none past the last: there has to be one.
+  if (p->gather && p->rows % p->top != 0)
+    return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: a gather's %lld rows are no multiple of top (%lld)", (long long)p->rows, (long long)p->top);
   // The kernels find MXFP4 rows by an offset from their tile's first one.
   if (p->gather && p->x_type == MPS_TYPE_MXFP4)
     return fail(MPS_ERR_INVALID_ARGUMENT, "mxfp4 product: a gather needs 16-bit x");

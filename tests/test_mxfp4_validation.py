@@ -55,6 +55,15 @@ def test_gather_of_mxfp4_rows_is_refused():
         assert rc == _native.MPS_ERR_INVALID_ARGUMENT and b"16-bit" in lib.mps_last_error()
 
 
+@pytest.mark.parametrize("rows,top", [(3, 4), (1, 2 ** 31 + 1), (9, 2)])
+def test_gather_of_parts_of_tokens_is_refused(rows, top):
+    """x has rows / top rows: with fewer rows than top there would be none to keep bad orders within."""
+    lib = _native.lib()
+    p = ctypes.c_void_p(4096)  # never read
+    args = _native.MpsMxfp4Product(x=p, x_stride=32, w=p, w_scales=p, out=p, offsets=p, order=p, rows=rows, n=8, k=32, experts=2, top=top, gather=1)
+    assert lib.mps_mxfp4_multiply(args, None, 0, None) == _native.MPS_ERR_INVALID_ARGUMENT and b"multiple of top" in lib.mps_last_error()
+
+
 def test_plain_quantization_known_answers():
     """The oracle of these tests against a block worked out by hand: the largest element 5 has floor(log2) 2, so the
     scale is 2^0; 5 is halfway between 4 (code 6, even) and 6, 0.75 between 0.5 and 1 (code 2, even)."""
