@@ -27,6 +27,14 @@ inline int32_t sort_chunk(int64_t pairs) {
   const int64_t chunk = (pairs + kMostChunks - 1) / kMostChunks;
   return pairs <= kOneWorkgroup ? kOneWorkgroup : (int32_t)(chunk < 2048 ? 2048 : (chunk + 1023) / 1024 * 1024);
 }
+inline int64_t sort_chunks(int64_t pairs) {  // in 64 bits: near 2^31 pairs the sum passes 32
+  const int64_t chunk = sort_chunk(pairs);
+  return pairs > 0 ? (pairs + chunk - 1) / chunk : 1;
+}
+inline int64_t sort_bytes(int64_t pairs, int64_t experts) {
+  const int64_t chunks = sort_chunks(pairs);
+  return chunks > 1 ? chunks * (experts + 1) * 4 : 0;
+}
 
 template <typename Id>
 __global__ __launch_bounds__(kSortThreads) void expert_count_kernel(const Id *__restrict__ ids, int32_t pairs,
@@ -403,8 +411,7 @@ int mps_expert_sort_workspace(int64_t tokens, int64_t top, int64_t experts, int6
   const int rc = check_sizes("expert_sort", tokens, top, experts);
   if (rc != MPS_OK) return rc;
   if (!bytes) return fail(MPS_ERR_INVALID_ARGUMENT, "expert_sort: null pointer");
-  const int64_t pairs = tokens * top, chunk = sort_chunk(pairs), chunks = (pairs + chunk - 1) / chunk;
-  *bytes = chunks > 1 ? chunks * (experts + 1) * 4 : 0;
+  *bytes = sort_bytes(tokens * top, experts);
   return MPS_OK;
 }
 
@@ -416,12 +423,12 @@ int mps_expert_sort(const void *ids, int32_t ids_64, int64_t tokens, int64_t top
   const int32_t pairs = (int32_t)(tokens * top);
   if (!offsets || (pairs > 0 && (!ids || !order || !positions)))
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_sort: null pointer");
-  const int32_t chunk = sort_chunk(pairs), chunks = pairs > 0 ? (pairs + chunk - 1) / chunk : 1;
-  if (chunks > 1 && (!workspace || workspace_bytes < (int64_t)chunks * (experts + 1) * 4))
-    return fail(MPS_ERR_INVALID_ARGUMENT, "expert_sort: %lld bytes of workspace are needed",
-                (long long)chunks * (experts + 1) * 4);
+  const int32_t chunk = sort_chunk(pairs), chunks = (int32_t)sort_chunks(pairs);
+  const int64_t need = sort_bytes(pairs, experts);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(MPS_ERR_INVALID_ARGUMENT, "expert_sort: %lld bytes of workspace are needed", (long long)need);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  int32_t *const counts = chunks > 1 ? static_cast<int32_t *>(workspace) : nullptr;
+  int32_t *const counts = need > 0 ? static_cast<int32_t *>(workspace) : nullptr;
   if (ids_64)
     launch_sort(static_cast<const int64_t *>(ids), pairs, chunk, chunks, (int32_t)experts, counts, order, positions, offsets, s);
   else

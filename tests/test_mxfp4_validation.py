@@ -64,6 +64,18 @@ def test_gather_of_parts_of_tokens_is_refused(rows, top):
     assert lib.mps_mxfp4_multiply(args, None, 0, None) == _native.MPS_ERR_INVALID_ARGUMENT and b"multiple of top" in lib.mps_last_error()
 
 
+@pytest.mark.parametrize("pairs", (4097, 65536, 2113929216, 2113930241, 2 ** 31 - 1025))
+def test_sort_asks_for_its_workspace(pairs):
+    """Up to the most pairs there may be, both entries want the same: chunks of 2^25 pairs, counted in 64 bits."""
+    lib = _native.lib()
+    p = ctypes.c_void_p(4096)  # never read
+    need = ctypes.c_int64(0)
+    assert lib.mps_expert_sort_workspace(pairs, 1, 8, need) == 0 and need.value > 0 and need.value <= 64 * 9 * 4
+    for work, size in ((None, 0), (p, need.value - 1)):
+        rc = lib.mps_expert_sort(p, 0, pairs, 1, 8, p, p, p, work, size, None)
+        assert rc == _native.MPS_ERR_INVALID_ARGUMENT and b"%d bytes of workspace" % need.value in lib.mps_last_error()
+
+
 def test_plain_quantization_known_answers():
     """The oracle of these tests against a block worked out by hand: the largest element 5 has floor(log2) 2, so the
     scale is 2^0; 5 is halfway between 4 (code 6, even) and 6, 0.75 between 0.5 and 1 (code 2, even)."""
