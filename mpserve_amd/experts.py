@@ -10,7 +10,8 @@ A router gives each of ``t`` tokens ``top`` experts; an expert id outside ``[0, 
 
 Shapes do not depend on the routing, so nothing synchronises and all of it can be captured
 into a graph. The calls run on the current stream of their tensors' device; results do not
-depend on the order in which the GPU ran anything.
+depend on the order in which the GPU ran anything. Gradients are those of backward mode; tensors
+that carry a tangent are refused.
 """
 from __future__ import annotations
 
@@ -21,7 +22,7 @@ import torch
 
 from . import _native
 from ._common import _check_cuda_contig
-from .mxfp4 import BLOCK, _TYPES, _call, _check_bias, _check_cuda, _check_mx, _check_out, _multiply, _no_grad, _set_x, _type
+from .mxfp4 import BLOCK, _TYPES, _call, _check_bias, _check_cuda, _check_mx, _check_out, _multiply, _no_grad, _no_tangent, _set_x, _type
 
 
 class ExpertSort(NamedTuple):
@@ -147,6 +148,7 @@ def expert_gather(x: torch.Tensor, sort: ExpertSort) -> torch.Tensor:
     _check_cuda(x, "x")
     _check_sort(sort, x.device)
     _check_rows(x, "x", sort.positions.shape[0])
+    _no_tangent("expert_gather", x)
     if not (x.requires_grad and torch.is_grad_enabled()):
         return _gather_rows(x.contiguous(), *sort)
     return _Gather.apply(x.contiguous(), *sort)
@@ -164,6 +166,7 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, sort: ExpertSort) -> 
     _type(weights, "weights")
     if weights.shape != sort.positions.shape:
         raise ValueError(f"weights must have shape {tuple(sort.positions.shape)}, got {tuple(weights.shape)}")
+    _no_tangent("expert_combine", y, weights)
     y, weights = y.contiguous(), weights.contiguous()
     if not ((y.requires_grad or weights.requires_grad) and torch.is_grad_enabled()):
         return _sum_rows(y, weights, sort.positions)

@@ -13,7 +13,7 @@ A row's last block is filled up with zero codes.
 The weights that the decode ops rebuild (``huffman_decode_fp8``, ``DecodePlan``) go straight
 into ``mxfp4_quantize``; a weight's codes and scales are kept as they are. All calls run on
 the current stream of their tensors' device, do not synchronise, and can be captured into a
-graph. They have no gradients, and refuse tensors that ask for one. The work is done by the
+graph. They have no gradients, and refuse tensors that ask for one or carry a tangent. The work is done by the
 HIP kernels of libmpserve_amd.so; there is no CPU path.
 """
 from __future__ import annotations
@@ -22,6 +22,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._common import _check_cuda_contig
@@ -40,7 +41,16 @@ def _type(t: torch.Tensor | torch.dtype, name: str) -> int:
     return code
 
 
+def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors, which need not require a gradient: their tangents would be lost."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: call it with the primal tensors")
+
+
 def _no_grad(name: str, t: Optional[torch.Tensor]) -> None:
+    _no_tangent(name, t)
     if t is not None and t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
 

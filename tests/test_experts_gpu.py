@@ -245,6 +245,28 @@ def test_no_second_gradient():
         again[0].sum().backward()
 
 
+def test_no_forward_mode():
+    """A dual tensor requires no gradient, but a result without its tangent would be wrong."""
+    from torch.autograd import forward_ad
+
+    from mpserve_amd.mxfp4 import mxfp4_linear, mxfp4_matmul, mxfp4_quantize
+
+    sort = expert_sort(torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device=DEV), 3)
+    x, y, w, bias = torch.randn(2, 32, device=DEV), torch.randn(4, 32, device=DEV), torch.rand(2, 2, device=DEV), torch.randn(8, device=DEV)
+    half = x.to(torch.bfloat16)
+    codes, scales = plain.random_weight(gen(0), (8,), 32, DEV)
+    codes3, scales3 = plain.random_weight(gen(0), (3, 8), 32, DEV)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: expert_gather(dual(x), sort), lambda: expert_combine(dual(y), w, sort), lambda: expert_combine(y, dual(w), sort),
+                     lambda: mxfp4_quantize(dual(x)), lambda: mxfp4_linear(dual(half), codes, scales),
+                     lambda: mxfp4_linear(half, codes, scales, dual(bias)), lambda: mxfp4_matmul(codes, scales, codes, scales, dual(bias)),
+                     lambda: mxfp4_expert_linear(dual(half), codes3, scales3, sort, gather=True)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+        assert expert_combine(expert_gather(x, sort), w, sort).shape == (2, 32)
+
+
 def test_whole_path_in_a_graph():
     """Sort, product, weighted sum and gradients, captured once and replayed on new routings and tokens."""
     t, top, experts, k, n = 50, 4, 16, 256, 136

@@ -76,6 +76,24 @@ def test_sort_asks_for_its_workspace(pairs):
         assert rc == _native.MPS_ERR_INVALID_ARGUMENT and b"%d bytes of workspace" % need.value in lib.mps_last_error()
 
 
+def test_dual_tensors_are_told():
+    from torch.autograd import forward_ad
+
+    from mpserve_amd.mxfp4 import _no_grad, _no_tangent
+
+    x = torch.zeros(2, 32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not dual.requires_grad
+        for call in (lambda: _no_tangent("op", None, x, dual), lambda: _no_grad("op", dual)):
+            with pytest.raises(RuntimeError, match="op has no forward-mode derivative"):
+                call()
+        _no_tangent("op", None, x, forward_ad.unpack_dual(dual).primal)
+        with torch.inference_mode():  # no derivative is being taken
+            _no_tangent("op", dual)
+    _no_tangent("op", x)
+
+
 def test_plain_quantization_known_answers():
     """The oracle of these tests against a block worked out by hand: the largest element 5 has floor(log2) 2, so the
     scale is 2^0; 5 is halfway between 4 (code 6, even) and 6, 0.75 between 0.5 and 1 (code 2, even)."""
