@@ -74,7 +74,7 @@ __device__ inline u32x4 load_row8(const uint16_t *row, int64_t col, int64_t k) {
   return v;
 }
 
-// Eight codes' values in BF16, scaled: exact.
+// Eight codes' values in BF16, scaled: exact but for scales 253 and 254, where 2^128 and more are infinite.
 __device__ inline bf16x8 widen(uint32_t codes, float scale) {
   u32x4 v;
   v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
@@ -82,6 +82,27 @@ __device__ inline bf16x8 widen(uint32_t codes, float scale) {
   v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
   v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
   return __builtin_bit_cast(bf16x8, v);
+}
+
+// A quarter of eight codes' values in BF16, exact for every scale (1.5 * 2^127 down to 2^-130, of which BF16 still has
+// the last bit). Where `widen` could overflow, x meets it four times: no product is infinite that need not be,
+// and a zero of x stays one. That takes four times the matrix instructions and more, so the kernels go on as
+// if nothing could overflow, note whether a scale was 2^65 or more, which no weight in use has, and if so
+// make the sums again this way.
+__device__ inline bf16x8 widen_quarter(uint32_t codes, uint32_t s) {
+  const float scale = __uint_as_float(s == 255 ? 0x7fc00000u : s > 2 ? (s - 2) << 23 : 0x00100000u << s);
+  const f32x2 f[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1),
+                      __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3)};
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(f[i].x * scale) >> 16 | (__float_as_uint(f[i].y * scale) & 0xffff0000u);
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+// Has bits of kLargeScale if one of 16 scale bytes is 192 or more.
+constexpr uint32_t kLargeScale = 0x80808080u;
+__device__ inline uint32_t large_scales(u32x4 s) {
+  return (s[0] & s[0] << 1) | (s[1] & s[1] << 1) | (s[2] & s[2] << 1) | (s[3] & s[3] << 1);
 }
 
 // The codes' values in FP16, without a scale.

@@ -16,7 +16,7 @@
 //
 // FP16 x meets the codes' values in FP16, without their scale, which could leave FP16's range;
 // the products of a block are summed by themselves and added with the scale in FP32, exactly as
-// if it had been in the weight. (BF16 holds the scaled weight. FP16 as a sum of two BF16 took
+// if it had been in the weight. (BF16 holds the scaled weight; for scales near 2^127 a quarter of it. FP16 as a sum of two BF16 took
 // twice the matrix instructions and 32 conversions a fragment.)
 #include "mxfp4_product.h"
 
@@ -111,25 +111,17 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
       for (int i = 0; i < R::kSL; ++i) scales[i] = load_scales(s_from[i], 16 * period, blocks);
     };
 
-    get_scales(wave);
+    uint32_t large = 0;  // BF16: whether this lane has met a large scale
+    auto put_scales = [&](int32_t period) {  // the lane's rows' 16 scale bytes, at its place; LDS keeps a wave's order
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-      if (i < items) fetch(i, i);
-    int slot = 0;
-    for (int32_t item = 0; item < items; ++item) {
+      for (int i = 0; i < R::kSL; ++i) {
+        const u32x4 moved = move_scales(scales[i], 16 * period, blocks);
+        *reinterpret_cast<u32x4 *>(ss + (i * 64 + lane) * 16) = moved;
+        if constexpr (XT == MPS_TYPE_BF16) large |= large_scales(moved);
+      }
+    };
+    auto multiply = [&](int32_t item, int slot, auto quartered) {
       const int32_t in = item % R::kSteps;
-      if (in == 0) {  // the lane's rows' 16 scale bytes, at its place; LDS keeps a wave's order
-#pragma unroll
-        for (int i = 0; i < R::kSL; ++i) 
-          *reinterpret_cast<u32x4 *>(ss + (i * 64 + lane) * 16) = move_scales(scales[i], 16 * period_of(item), blocks);
-        if (item + R::kSteps < items) get_scales(period_of(item) + W);
-      }
-      if (item + S - 1 < items) {
-        fetch(item + S - 1, slot == 0 ? S - 1 : slot - 1);
-        wait_loads<(S - 1) * R::kLoads>();
-      } else {
-        wait_loads<0>();
-      }
       const uint8_t *const xl = mine + slot * R::kStage, *const wl = xl + R::kXBytes;
       if constexpr (k4) {
         uint32_t sx[kFT], sw[FN];
@@ -207,15 +199,56 @@ __global__ __launch_bounds__(W * 64) void mxfp4_rows_kernel(ProductArgs a) {
                   for (int i = 0; i < 4; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[i], acc[t][n][i]);
                 }
               } else {
-                const bf16x8 w = widen(fw[u][n][j], mx_scale(byte));
+                constexpr bool quarters = decltype(quartered)::value;
+                const bf16x8 w = quarters ? widen_quarter(fw[u][n][j], byte) : widen(fw[u][n][j], mx_scale(byte));
 #pragma unroll
-                for (int t = 0; t < kFT; ++t)
-                  acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fx[u][t][j]), w, acc[t][n], 0, 0, 0);
+                for (int i = 0; i < (quarters ? 4 : 1); ++i)
+#pragma unroll
+                  for (int t = 0; t < kFT; ++t)
+                    acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fx[u][t][j]), w, acc[t][n], 0, 0, 0);
               }
             }
       }
+    };
+
+    get_scales(wave);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      if (i < items) fetch(i, i);
+    int slot = 0;
+    for (int32_t item = 0; item < items; ++item) {
+      if (item % R::kSteps == 0) {
+        put_scales(period_of(item));
+        if (item + R::kSteps < items) get_scales(period_of(item) + W);
+      }
+      if (item + S - 1 < items) {
+        fetch(item + S - 1, slot == 0 ? S - 1 : slot - 1);
+        wait_loads<(S - 1) * R::kLoads>();
+      } else {
+        wait_loads<0>();
+      }
+      multiply(item, slot, std::false_type{});
       slot = slot == S - 1 ? 0 : slot + 1;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read: the next loads may take its place
+    }
+    if constexpr (XT == MPS_TYPE_BF16) {
+      if (__builtin_expect(__any(large & kLargeScale), 0)) {  // a weight may have overflowed: all again, one at a time
+#pragma unroll
+        for (int t = 0; t < kFT; ++t)
+#pragma unroll
+          for (int n = 0; n < FN; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+        for (int32_t item = 0; item < items; ++item) {
+          if (item % R::kSteps == 0) {
+            get_scales(period_of(item));
+            put_scales(period_of(item));
+          }
+          fetch(item, 0);
+          wait_loads<0>();
+          multiply(item, 0, std::true_type{});
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+      }
     }
   }
 

@@ -47,7 +47,8 @@ struct Shape {
   static constexpr int kXBytes = BT * 128, kWBytes = BN * kWPieces * 16, kSBytes = kScaleRows * 16;
   static constexpr int kPitch = kFN * 32 + 4;                    // floats of a row of sums, turned round
   static constexpr int kStaged = 2 * (kXBytes + kWBytes + kSBytes), kTurned = kWaves * 32 * kPitch * 4;
-  static constexpr int kLds = kStaged > kTurned ? kStaged : kTurned;
+  static constexpr int kFlags = kStaged > kTurned ? kStaged : kTurned;  // a word a wave
+  static constexpr int kLds = kFlags + (XT == MPS_TYPE_BF16 ? kWaves * 4 : 0);
   static_assert(BT * 8 % kThreads == 0 && kThreads % 128 == 0 && kLds <= 160 * 1024, "");
 };
 
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
     }
   };
   // Scales come 16 blocks at a time, a period ahead, through registers.
-  u32x4 scales[S::kSLoads];
+  u32x4 scales[S::kSLoads] = {};
   auto get_scales = [&](int32_t period) {
     if (has_scales) {
 #pragma unroll
@@ -143,6 +144,20 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
       for (int i = 0; i < S::kSLoads; ++i)
         *reinterpret_cast<u32x4 *>(ss + buffer * S::kSBytes + (tid + i * S::kThreads) * 16) = move_scales(scales[i], 16 * period, blocks);
+    }
+    if constexpr (XT == MPS_TYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < S::kSLoads; ++i) asm volatile("" : "+v"(scales[i]));  // are there, for all waves: waited for here, not below
+    }
+  };
+  // BF16: a wave that meets a large scale says so in LDS, by the next barrier.
+  uint32_t *const flags = reinterpret_cast<uint32_t *>(lds + S::kFlags);
+  auto note_scales = [&]() {
+    if constexpr (XT == MPS_TYPE_BF16) {
+      uint32_t large = 0;
+#pragma unroll
+      for (int i = 0; i < S::kSLoads; ++i) large |= large_scales(scales[i]);
+      if (__builtin_expect(__any(large & kLargeScale), 0)) flags[wave] = 1;
     }
   };
 
@@ -224,7 +239,9 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
     if (periods > 0) {
       fetch(0, 0, 0, kLoads);
       get_scales(0);
+      if constexpr (XT == MPS_TYPE_BF16) flags[wave] = 0;
       put_scales(0, 0);
+      note_scales();
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       fetch(1, 1, 0, kLoads);
       read(tc, 0, 0, 0, 0);
@@ -273,6 +290,7 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
           if (in == S::kSteps - 2) put_scales(p + 1, sbuf ^ 1);
           quarter(std::integral_constant<int, 3>{});
+          if (in == S::kSteps - 2) note_scales();
         }
       }
     }
@@ -290,6 +308,43 @@ __global__ __launch_bounds__(WT *WN * 64) __attribute__((amdgpu_waves_per_eu(2, 
   }
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads of steps past the last
+  if constexpr (XT == MPS_TYPE_BF16) {
+    uint32_t any = 0;
+    if (periods > 0)
+      for (int w = 0; w < S::kWaves; ++w) any |= flags[w];
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) != 0, 0)) {  // alike in all waves: a product could have overflowed
+#pragma unroll
+      for (int t = 0; t < S::kFT; ++t)
+#pragma unroll
+        for (int n = 0; n < S::kFN; ++n) acc[t][n] = f32x16{};
+#pragma unroll 1
+      for (int32_t step = 0; 2 * step < blocks; ++step) {  // all again, one at a time, with scales from memory
+        __syncthreads();
+        fetch(step, 0, 0, kLoads);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int32_t block = 2 * step + (q >> 1);
+          if (block >= blocks) break;
+          read(std::integral_constant<int, S::kFT>{}, q, 0, 0, 0);
+          if (q % 2 == 0) {
+#pragma unroll
+            for (int n = 0; n < S::kFN; ++n)
+              sw[q >> 1][n] = a.w_scales[(w_first + min((wn * S::kFN + n) * 32 + r, a.n - 1 - n0)) * blocks + block];
+          }
+#pragma unroll
+          for (int n = 0; n < S::kFN; ++n) {
+            const bf16x8 w = widen_quarter((uint32_t)(fw[q >> 1][n] >> (32 * (q & 1))), sw[q >> 1][n]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int t = 0; t < S::kFT; ++t)
+                acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, __builtin_bit_cast(bf16x8, fx[q % kBuffers][t]), acc[t][n], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
   if constexpr (XT != MPS_TYPE_BF16) {
     // A lane's 16 sums are places 8 i + 4 g .. + 3 of one side of a fragment, at place r of the other: columns
     // of one row, or with FP16 x rows of one column. The wave turns 32 rows at a time round through

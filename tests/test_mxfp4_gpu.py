@@ -218,6 +218,49 @@ def test_products_smallest_and_largest_scales():
         plain.close(mxfp4_matmul(xc, xs, codes, scales, out_dtype=torch.float32), xv @ w.T, xv.abs() @ w.abs().T, 256)
 
 
+LARGEST = [(1, 1030, 16), (1, 4096, 512), (8, 160, 33), (16, 1000, 48), (50, 2056, 2100), (64, 128, 512), (130, 1030, 1030), (130, 2056, 520),
+           (500, 1030, 520), (70, 500, 20000), (60, 320, 100), (250, 1030, 4101), (700, 96, 4300), (1100, 64, 8300), (2300, 704, 8500)]
+
+
+@pytest.mark.parametrize("kind", (torch.bfloat16, torch.float16, "mxfp4"))
+@pytest.mark.parametrize("t,k,n", LARGEST)
+def test_products_with_the_largest_scales_are_exact(kind, t, k, n):
+    """Weights of 2^128 and more in every second column, ordinary ones beside them, and small x, zeros among them:
+    whole numbers times powers of two, so that FP32 holds all products and sums (in quarters of halves, below 2^24)."""
+    g = gen(t + k + n)
+    codes, scales = plain.random_weight(g, (n,), k, DEV, 126, 129)
+    scales[::2] = torch.randint(252, 255, scales[::2].shape, generator=g, device=DEV, dtype=torch.uint8)
+    if kind == "mxfp4":
+        xc, xs = plain.random_weight(g, (t,), k, DEV, 66, 69)
+        x, got = plain.dequantize(xc, xs, k), mxfp4_matmul(xc, xs, codes, scales, out_dtype=torch.float32)
+    else:
+        x = (whole_numbers(g, t, k, torch.float32) * (2.0 ** -60 if kind is torch.bfloat16 else 2.0 ** -20)).to(kind)
+        got = mxfp4_linear(x, codes, scales, out_dtype=torch.float32)
+    want = x.double() @ plain.dequantize(codes, scales, k).T
+    assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("t", (3, 300))
+def test_linear_bf16_largest_scales_beside_others(t):
+    """NaN scales, the smallest ones, and infinite x, in tiles with the largest scales. Two terms a sum, of powers of two."""
+    g = gen(t)
+    codes, scales = plain.random_weight(g, (300,), 320, DEV, 250, 255)
+    tiny = torch.zeros(300, dtype=torch.bool, device=DEV)
+    tiny[1::3] = True
+    scales[tiny] = torch.randint(0, 4, scales[tiny].shape, generator=g, device=DEV, dtype=torch.uint8)
+    scales[36, 4] = 255
+    x = torch.zeros(t, 320, dtype=torch.bfloat16, device=DEV)
+    x[0, 7], x[0, 300], x[1, 319], x[2, 7], x[2, 300] = 2.0 ** -10, -2.0 ** -9, float("inf"), 2.0 ** 30, 2.0 ** 31
+    y = mxfp4_linear(x, codes, scales, out_dtype=torch.float32)
+    assert bool(torch.isnan(y[:, 36]).all()) and not bool(torch.isfinite(y[1]).any())
+    want = x.double() @ plain.dequantize(codes, scales, 320).T
+    large = ~tiny
+    large[36] = False
+    assert torch.equal(y[0, large].double(), want[0, large])
+    assert torch.equal(y[2, tiny].double(), want[2, tiny])
+    assert bool((y[3:, tiny | large] == 0).all())
+
+
 @pytest.mark.parametrize("t", (3, 40, 200))
 def test_linear_f16_with_scales_outside_f16(t):
     """Weights far below and far above what FP16 holds, and blocks of both in one row."""
