@@ -111,8 +111,12 @@ def _check_mx(codes: torch.Tensor, scales: torch.Tensor, name: str, dims: Option
 def _check_out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("out must not require a gradient: the calls have none for it")
+    _no_tangent("a call with out", out)
     if out.dtype != dtype or out.device != device or not out.is_contiguous() or tuple(out.shape) != tuple(shape):
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+    torch.autograd.graph.increment_version(out)  # so that autograd knows if it had saved what is there now
     return out
 
 

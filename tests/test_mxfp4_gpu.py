@@ -384,3 +384,28 @@ def test_refusals():
             call()
     with torch.no_grad():
         assert mxfp4_linear(x.detach().requires_grad_(), codes, scales).shape == (4, 8)
+
+
+def test_out_and_autograd():
+    """A tensor that autograd follows is not written behind its back."""
+    from mpserve_amd.experts import expert_sort, mxfp4_expert_linear
+
+    x = torch.randn(4, 64, device=DEV).to(torch.bfloat16)
+    codes, scales = plain.random_weight(gen(0), (8,), 64, DEV)
+    sort = expert_sort(torch.zeros(4, 1, dtype=torch.int32, device=DEV), 1)
+    calls = (lambda out: mxfp4_linear(x, codes, scales, out=out), lambda out: mxfp4_matmul(*mxfp4_quantize(x), codes, scales, out=out),
+             lambda out: mxfp4_expert_linear(x, codes[None], scales[None], sort, out=out))
+    for call in calls + (lambda out: mxfp4_dequantize(codes[:4, :16].contiguous(), scales[:4, :1].contiguous(), 8, torch.bfloat16, out=out),):
+        out = torch.zeros(4, 8, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(RuntimeError, match="out must not require a gradient"):
+            call(out.requires_grad_())
+        with torch.no_grad():
+            assert call(out) is out
+        out, factor = torch.zeros(4, 8, dtype=torch.bfloat16, device=DEV), torch.ones(4, 8, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+        product = out * factor  # autograd keeps `out`
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+        with torch.inference_mode():
+            out = torch.zeros(4, 8, dtype=torch.bfloat16, device=DEV)
+            assert call(out) is out
