@@ -381,7 +381,8 @@ int mps_expert_combine(const void *y, int32_t type, const void *weights, int32_t
                        int64_t top, int64_t width, const int32_t *positions, void *out, void *stream);
 /* Gradients of mps_expert_combine: dy[j] = weights[pair] * dout[token] and
  * dweights[pair] = <y[j], dout[token]> for the pair at place j; zero for the
- * pairs of no expert. */
+ * pairs of no expert. dy or dweights may be NULL, if that gradient is not
+ * wanted; y may be NULL without dweights. */
 int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const void *weights, int32_t weights_type,
                             int64_t tokens, int64_t top, int64_t experts, int64_t width, const int32_t *order,
                             const int32_t *positions, const int32_t *offsets, void *dy, void *dweights, void *stream);

@@ -199,14 +199,15 @@ struct RowArgs {
 };
 
 // The places of pairs of no expert, and the rows there: zeros. Workgroups past the tokens' take them in turn.
-template <int T>
-__device__ inline void zero_rows(const RowArgs &a, int64_t block, int64_t blocks, bool weights) {
+template <int T, bool kRows, bool kWeights>
+__device__ inline void zero_rows(const RowArgs &a, int64_t block, int64_t blocks) {
   typedef Piece<T> P;
   const int64_t first = min(max((int64_t)a.offsets[a.experts], (int64_t)0), a.pairs);
   for (int64_t j = first + block; j < a.pairs; j += blocks) {
-    for (int64_t col = threadIdx.x * P::kVec; col < a.width; col += kRowThreads * P::kVec)
-      P{}.store(static_cast<typename Elem<T>::raw *>(a.out) + j * a.width, col, a.width);
-    if (weights && threadIdx.x == 0) {
+    if constexpr (kRows)
+      for (int64_t col = threadIdx.x * P::kVec; col < a.width; col += kRowThreads * P::kVec)
+        P{}.store(static_cast<typename Elem<T>::raw *>(a.out) + j * a.width, col, a.width);
+    if (kWeights && threadIdx.x == 0) {
       const int64_t pair = a.order[j];
       if (pair >= 0 && pair < a.pairs) store_as(a.dweights, a.weights_type, pair, 0.0f);
     }
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(RowArgs a, i
   typedef Piece<T> P;
   typedef typename Elem<T>::raw raw;
   const int64_t grid = gridDim.x - kZeroBlocks;
-  if (blockIdx.x >= grid) return zero_rows<T>(a, blockIdx.x - grid, kZeroBlocks, false);
+  if (blockIdx.x >= grid) return zero_rows<T, true, false>(a, blockIdx.x - grid, kZeroBlocks);
   const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
   for (int64_t block = blockIdx.x; block < token_blocks; block += grid) {
     const int64_t t = kWide ? block : block * (kRowThreads / lanes) + threadIdx.x / lanes;
@@ -291,14 +292,15 @@ __global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(RowArgs a, 
 }
 
 // kPairs pairs of a token at a time. A work-item's products are added up in the order of its pieces, and
-// the work-items' sums by a tree: a fixed order.
-template <int T, bool kWide>
+// the work-items' sums by a tree: a fixed order. kDy and kDw: which gradients are asked for; the weights' alone
+// write no rows, those of y alone read none.
+template <int T, bool kWide, bool kDy, bool kDw>
 __global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(RowArgs a, int64_t token_blocks) {
   typedef Piece<T> P;
   typedef typename Elem<T>::raw raw;
   __shared__ float parts[kPairs][kRowThreads / 64];
   const int64_t grid = gridDim.x - kZeroBlocks;
-  if (blockIdx.x >= grid) return zero_rows<T>(a, blockIdx.x - grid, kZeroBlocks, true);
+  if (blockIdx.x >= grid) return zero_rows<T, kDy, kDw>(a, blockIdx.x - grid, kZeroBlocks);
   const int32_t lanes = kWide ? kRowThreads : a.lanes;  // a token a workgroup: its places are scalars
   for (int64_t block = blockIdx.x; block < token_blocks; block += grid) {
     const int64_t t = kWide ? block : block * (kRowThreads / lanes) + threadIdx.x / lanes;
@@ -313,28 +315,32 @@ __global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(RowArg
         const int64_t pair = t * a.top + i0 + i;
         at[i] = token && i0 + i < a.top ? a.positions[pair] : -1;
         if (at[i] >= a.pairs) at[i] = -1;
-        w[i] = at[i] >= 0 ? load_as_float(a.weights, a.weights_type, pair) : 0.0f;
+        w[i] = kDy && at[i] >= 0 ? load_as_float(a.weights, a.weights_type, pair) : 0.0f;
       }
       if (token)
         for (int64_t col = (threadIdx.x & (lanes - 1)) * P::kVec; col < a.width; col += lanes * P::kVec) {
           const P d = P::load(g, col, a.width);
           P p[kPairs];
+          if constexpr (kDw) {
 #pragma unroll
-          for (int i = 0; i < kPairs; ++i)
-            if (at[i] >= 0) p[i] = P::load(y + at[i] * a.width, col, a.width);
+            for (int i = 0; i < kPairs; ++i)
+              if (at[i] >= 0) p[i] = P::load(y + at[i] * a.width, col, a.width);
+          }
 #pragma unroll
           for (int i = 0; i < kPairs; ++i)
             if (at[i] >= 0) {
+#pragma clang fp contract(off)  // one multiply-add each, whichever gradients are asked for (FP16 pairs became dot products in one form)
               P o;
 #pragma unroll
               for (int v = 0; v < P::kVec; ++v) {
                 const float gv = d.get(v);
-                dot[i] += gv * p[i].get(v);
-                o.put(v, w[i] * gv);
+                if constexpr (kDw) dot[i] = __builtin_fmaf(gv, p[i].get(v), dot[i]);
+                if constexpr (kDy) o.put(v, w[i] * gv);
               }
-              o.store(dy + at[i] * a.width, col, a.width);
+              if constexpr (kDy) o.store(dy + at[i] * a.width, col, a.width);
             }
         }
+      if constexpr (!kDw) continue;
       const int in_wave = lanes < 64 ? lanes : 64;
       for (int d = in_wave / 2; d > 0; d /= 2)
 #pragma unroll
@@ -490,8 +496,8 @@ int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const
   if (!is_float_type(type) || !is_float_type(weights_type) || width < 0)
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine_grad: bad type or width");
   const int64_t pairs = tokens * top;
-  if (pairs == 0) return MPS_OK;
-  if (!weights || !order || !positions || !offsets || !dweights || (width > 0 && (!y || !dout || !dy)))
+  if (pairs == 0 || (width == 0 && !dweights)) return MPS_OK;
+  if (!weights || !order || !positions || !offsets || (!dy && !dweights) || (width > 0 && (!dout || (dweights && !y))))
     return fail(MPS_ERR_INVALID_ARGUMENT, "expert_combine_grad: null pointer");
   RowArgs a = {};
   a.in = y, a.dout = dout, a.out = dy, a.weights = weights, a.weights_type = weights_type, a.dweights = dweights;
@@ -499,10 +505,15 @@ int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const
   a.tokens = tokens, a.top = top, a.pairs = pairs, a.width = width, a.experts = (int32_t)experts, a.lanes = lanes_of(width, type);
   const int64_t per = kRowThreads / a.lanes, blocks = (tokens + per - 1) / per;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define CALL(T, W) \
-  hipLaunchKernelGGL((expert_combine_grad_kernel<T, W>), dim3(workgroups(blocks) + kZeroBlocks), dim3(kRowThreads), 0, s, a, blocks)
+#define LAUNCH(T, W, DY, DW) \
+  hipLaunchKernelGGL((expert_combine_grad_kernel<T, W, DY, DW>), dim3(workgroups(blocks) + kZeroBlocks), dim3(kRowThreads), 0, s, a, blocks)
+#define CALL(T, W)                                    \
+  if (!dy) { LAUNCH(T, W, false, true); }             \
+  else if (!dweights) { LAUNCH(T, W, true, false); }  \
+  else { LAUNCH(T, W, true, true); }
   MPS_BY_TYPE(type, a.lanes == kRowThreads, CALL);
 #undef CALL
+#undef LAUNCH
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
 }

@@ -126,7 +126,8 @@ class _Gather(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, order, positions, offsets):
-        ctx.save_for_backward(y, weights, order, positions, offsets)
+        # y is needed for the weights' gradient only
+        ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, weights, order, positions, offsets)
         return _sum_rows(y, weights, positions)
 
     @staticmethod
@@ -135,10 +136,15 @@ class _Combine(torch.autograd.Function):
         y, weights, order, positions, offsets = ctx.saved_tensors
         t, top = weights.shape
         dout = dout.contiguous()
-        dy, dweights = torch.empty_like(y), torch.empty_like(weights)
-        _call(y.device, _native.lib().mps_expert_combine_grad, y.data_ptr(), dout.data_ptr(), _TYPES[y.dtype],
-              weights.data_ptr(), _TYPES[weights.dtype], t, top, offsets.numel() - 1, y.shape[1], order.data_ptr(),
-              positions.data_ptr(), offsets.data_ptr(), dy.data_ptr(), dweights.data_ptr())
+        width, dy, dweights = dout.shape[1], None, None
+        if ctx.needs_input_grad[0]:
+            dy = torch.empty((t * top, width), dtype=dout.dtype, device=dout.device)
+        if ctx.needs_input_grad[1]:
+            dweights = torch.empty_like(weights)
+        _call(dout.device, _native.lib().mps_expert_combine_grad, y.data_ptr() if y is not None else None, dout.data_ptr(), _TYPES[dout.dtype],
+              weights.data_ptr(), _TYPES[weights.dtype], t, top, offsets.numel() - 1, width, order.data_ptr(),
+              positions.data_ptr(), offsets.data_ptr(), dy.data_ptr() if dy is not None else None,
+              dweights.data_ptr() if dweights is not None else None)
         return dy, dweights, None, None, None
 
 

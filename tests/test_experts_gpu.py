@@ -114,6 +114,35 @@ def test_gradients_match_formulas(dtype, t, top, experts, width):
         plain.close(dw, terms.sum(1).view(t, top), terms.abs().sum(1).view(t, top), width + 1)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,top,experts,width", CASES + [(300, 4, 16, 4096)])
+def test_one_gradient_alone(dtype, t, top, experts, width):
+    """The gradient of y or of the weights alone is what it is beside the other one; the weights' makes no rows
+    for y, and that of y keeps no y."""
+    g = gen(t + 2)
+    sort = expert_sort(routing(t, t, top, experts), experts)
+    top = sort.positions.shape[1]
+    y, dout = torch.randn(t * top, width, generator=g, device=DEV).to(dtype), torch.randn(t, width, generator=g, device=DEV).to(dtype)
+    weights = torch.rand(t, top, generator=g, device=DEV)
+    both = [v.clone().requires_grad_() for v in (y, weights)]
+    dy, dw = torch.autograd.grad(expert_combine(*both, sort), both, dout)
+    w = weights.clone().requires_grad_()
+    out = expert_combine(y, w, sort)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    (alone,) = torch.autograd.grad(out, w, dout)
+    assert torch.equal(alone, dw)
+    if y.numel() * y.element_size() >= 1 << 20:
+        assert torch.cuda.max_memory_allocated() - before < y.numel() * y.element_size()
+    leaf = y.clone().requires_grad_()
+    other = leaf * 1
+    out = expert_combine(other, weights, sort)
+    other.zero_()  # not kept for this gradient
+    (alone,) = torch.autograd.grad(out, leaf, dout)
+    assert torch.equal(alone, dy)
+
+
 def test_gradients_match_differences():
     """The combine is linear in y and in the weights, so a difference is exact but for rounding: with whole
     numbers it is exact."""

@@ -94,6 +94,14 @@ def test_dual_tensors_are_told():
     _no_tangent("op", x)
 
 
+def test_combine_grad_wants_something_to_write():
+    lib = _native.lib()
+    p = ctypes.c_void_p(4096)  # never read
+    for y, dy, dw in ((p, None, None), (None, p, p), (None, None, p)):
+        rc = lib.mps_expert_combine_grad(y, p, 0, p, 0, 4, 4, 8, 32, p, p, p, dy, dw, None)
+        assert rc == _native.MPS_ERR_INVALID_ARGUMENT and b"null pointer" in lib.mps_last_error()
+
+
 def test_plain_quantization_known_answers():
     """The oracle of these tests against a block worked out by hand: the largest element 5 has floor(log2) 2, so the
     scale is 2^0; 5 is halfway between 4 (code 6, even) and 6, 0.75 between 0.5 and 1 (code 2, even)."""
