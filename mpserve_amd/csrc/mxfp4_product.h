@@ -44,6 +44,7 @@ __device__ inline Tile find_tile(const int32_t *offsets, int32_t experts, int32_
     if (hit) {
       const int at = __ffsll((unsigned long long)hit) - 1;
       const int32_t in = tile - before - (__shfl(upto, at) - __shfl(tiles, at));
+      if ((uint32_t)in >= (uint32_t)__shfl(tiles, at)) return {-1, 0, 0};  // bad offsets whose tiles add up to 2^31 and more
       const int32_t f = __shfl(first, at) + in * size;
       return {e0 + at, f, min(f + size, __shfl(end, at))};
     }

@@ -261,6 +261,21 @@ def test_bad_orders_and_offsets_stay_in_bounds():
     torch.cuda.synchronize()
 
 
+def test_bad_offsets_of_many_rows_stay_in_bounds():
+    """Every second expert has all of 4e8 rows, so that the counts of tiles pass 2^31: no tile may come out of
+    what is left of them."""
+    rows, experts = 400_000_000, 1024
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GB of free memory")
+    offsets = torch.tensor([0, 2 ** 31 - 1], dtype=torch.int32, device=DEV).repeat(experts // 2 + 1)[:experts + 1].contiguous()
+    order = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    codes, scales = plain.random_weight(gen(0), (experts, 1), 32, DEV)
+    x = torch.zeros(1, 32, dtype=torch.bfloat16, device=DEV).expand(rows, 32)
+    y = mxfp4_expert_linear(x, codes, scales, ExpertSort(order, order.view(rows, 1), offsets))
+    torch.cuda.synchronize()
+    assert y.shape == (rows, 1)
+
+
 def test_no_second_gradient():
     """A graph of the gradients may be asked for; a gradient through it is refused."""
     sort = expert_sort(torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device=DEV), 3)
