@@ -97,7 +97,7 @@ def _check_mx(codes: torch.Tensor, scales: torch.Tensor, name: str, dims: Option
             return
     for t, part in ((codes, "codes"), (scales, "scales")):
         full = f"{name}{part}"
-        _check_cuda_contig(t, full, device if device is not None else codes.device)
+        _check_cuda_contig(t, full, device if device is not None or codes is None else codes.device)
         if t.dtype != torch.uint8:
             raise ValueError(f"{full} must be torch.uint8")
         if t.dim() < 1 or (dims is not None and t.dim() != dims):

@@ -22,6 +22,15 @@ def test_host_tensors_are_refused():
             call()
 
 
+def test_missing_tensors_are_refused():
+    codes, scales = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)
+    for call, name in ((lambda: mxfp4_quantize(None), "x"), (lambda: mxfp4_dequantize(None, scales, 32), "codes"),
+                       (lambda: mxfp4_matmul(None, scales, codes, scales), "x_codes"), (lambda: mxfp4_linear(None, codes, scales), "x"),
+                       (lambda: expert_sort(None, 1), "ids")):
+        with pytest.raises(ValueError, match=f"^{name} must be defined"):
+            call()
+
+
 def test_c_entries_refuse_bad_arguments():
     lib = _native.lib()
     p = ctypes.c_void_p(4096)  # never read: each call is refused before any work
