@@ -12,6 +12,11 @@ Shapes do not depend on the routing, so nothing synchronises and all of it can b
 into a graph. The calls run on the current stream of their tensors' device; results do not
 depend on the order in which the GPU ran anything. Gradients are those of backward mode; tensors
 that carry a tangent are refused.
+
+Experts' rows are rounded to the type of ``x`` between the product and the weighted sum, and the sum once more:
+a relative error of 0.0023 in BF16 where one rounding has 0.0017. Rows of ``out_dtype=torch.float32``, whose
+sum is FP32 too and is rounded by the caller's ``.to``, spare the first: 8192 tokens, four of 64 experts each, 4096 ->
+2048, then take 612 us in place of 548, four tokens 32 in place of 28.
 """
 from __future__ import annotations
 

@@ -1,7 +1,8 @@
 """A mixture-of-experts block over MXFP4 weights: the MXFP4 and expert operators as a serving program uses them.
 
 ``Mxfp4Experts`` holds the experts' gate/up and down projections in MXFP4, and optionally a
-shared expert's, whose gate/up product takes its activations in MXFP4 too. The weights may come
+shared expert's, whose gate/up product takes its activations in MXFP4 too. It rounds to the type of ``x``
+after each step, or with ``rounded=False`` as little as it can. The weights may come
 from anywhere in BF16, for instance from a checkpoint's FP8 bytes and sidecars through
 ``DecodePlan``, which is what the command does with small synthetic ones:
 
@@ -25,11 +26,13 @@ def _gated(h: torch.Tensor) -> torch.Tensor:
 
 class Mxfp4Experts:
     """``gate_up [experts, 2 * ffn, hidden]`` and ``down [experts, hidden, ffn]`` in BF16, FP16 or FP32;
-    ``shared``: the same pair of a shared expert, ``[2 * ffn, hidden]`` and ``[hidden, ffn]``."""
+    ``shared``: the same pair of a shared expert, ``[2 * ffn, hidden]`` and ``[hidden, ffn]``.
+    ``rounded=False``: the down products stay FP32 until they are added up, and the shared expert takes its
+    activations as they are, not in MXFP4."""
 
     def __init__(self, gate_up: torch.Tensor, down: torch.Tensor, top: int,
-                 shared: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
-        self.experts, self.top = gate_up.shape[0], int(top)
+                 shared: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, rounded: bool = True):
+        self.experts, self.top, self.rounded = gate_up.shape[0], int(top), bool(rounded)
         self.gate_up, self.down = mxfp4_quantize(gate_up), mxfp4_quantize(down)
         self.shared = None if shared is None else tuple(mxfp4_quantize(w) for w in shared)
 
@@ -40,12 +43,13 @@ class Mxfp4Experts:
         weights = torch.softmax(best, dim=-1)
         sort = expert_sort(ids, self.experts)
         h = _gated(mxfp4_expert_linear(x, *self.gate_up, sort, gather=True))
-        out = expert_combine(mxfp4_expert_linear(h, *self.down, sort), weights, sort)
+        rows = x.dtype if self.rounded else torch.float32
+        out = expert_combine(mxfp4_expert_linear(h, *self.down, sort, out_dtype=rows), weights, sort)
         if self.shared is not None:
             gate_up, down = self.shared
-            h = _gated(mxfp4_matmul(*mxfp4_quantize(x), *gate_up, out_dtype=x.dtype))
-            out = out + mxfp4_linear(h, *down)
-        return out
+            h = mxfp4_matmul(*mxfp4_quantize(x), *gate_up, out_dtype=x.dtype) if self.rounded else mxfp4_linear(x, *gate_up)
+            out = out + mxfp4_linear(_gated(h), *down, out_dtype=rows)
+        return out.to(x.dtype)
 
 
 def decoded_weight(shape, seed: int, device: torch.device) -> torch.Tensor:

@@ -394,6 +394,45 @@ def test_block_of_experts(dtype):
     assert bool((off <= 16 * u * size + 4 * u * want.abs() + 2.0 ** -24).all()), float((off / size).max() / u)
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_block_of_experts_that_rounds_less(dtype):
+    """With ``rounded=False`` the only roundings to 16 bits are those of gate and up, of silu (whose slope is below
+    1.1) and of its product with up, 4.1 roundoffs of |gate * up|, and that of the answer. FP32 sums of n terms are
+    off by n * 2^-23 of their terms' magnitudes. The default, which rounds the shared expert's activations to
+    4 bits, is far outside."""
+    from mpserve_amd.mxfp4_experts import Mxfp4Experts
+
+    t, hidden, ffn, experts, top = 45, 256, 160, 8, 3
+    g = gen(16)
+    weights = [0.05 * torch.randn(s, generator=g, device=DEV) for s in ((experts, 2 * ffn, hidden), (experts, hidden, ffn), (2 * ffn, hidden), (hidden, ffn))]
+    block = Mxfp4Experts(weights[0], weights[1], top, shared=(weights[2], weights[3]), rounded=False)
+    x = torch.randn(t, hidden, generator=g, device=DEV).to(dtype)
+    logits = torch.randn(t, experts, generator=g, device=DEV)
+    best, ids = logits.topk(top, dim=1)
+    w = torch.softmax(best, 1).double()
+    u, step = plain.ROUNDOFF[dtype], 2.0 ** -23
+
+    def expert(rows, gate_up, down):
+        """(answer, bound of its error before it is rounded)"""
+        (a, b), (big_a, big_b) = (rows @ gate_up.T).chunk(2, -1), (rows.abs() @ gate_up.abs().T).chunk(2, -1)
+        h = a * torch.sigmoid(a) * b
+        off = 4.2 * u * (a * b).abs() + 1.2 * hidden * step * (big_a * b.abs() + big_b * a.abs() + hidden * step * big_a * big_b)
+        return h @ down.T, (off + (ffn + top + 2) * step * (h.abs() + off)) @ down.abs().T
+
+    gu, dn = plain.dequantize(*block.gate_up, hidden), plain.dequantize(*block.down, ffn)
+    want, bound = expert(x.double(), plain.dequantize(*block.shared[0], hidden), plain.dequantize(*block.shared[1], ffn))
+    for e in range(experts):
+        token, slot = torch.where(ids == e)
+        y, off = expert(x[token].double(), gu[e], dn[e])
+        want[token] += w[token, slot].unsqueeze(1) * y
+        bound[token] += w[token, slot].unsqueeze(1) * off
+    bound = bound + u * (want.abs() + bound) + 2.0 ** -25
+    out = block(x, logits)
+    assert out.dtype == dtype and bool(((out.double() - want).abs() <= bound).all())
+    block.rounded = True
+    assert not bool(((block(x, logits).double() - want).abs() <= bound).all())
+
+
 def test_refusals():
     ids = routing(0, 6, 2, 4)
     sort = expert_sort(ids, 4)
