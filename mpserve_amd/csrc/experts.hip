@@ -170,7 +170,12 @@ struct Piece {
     } else {
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        if (col + i < width) p.put(i, Elem<T>::get(row[col + i]));
+        if (col + i < width) {  // bits as they are, those of a NaN too
+          if constexpr (T == MPS_TYPE_F32)
+            p.bits[i] = __float_as_uint(row[col + i]);
+          else
+            p.bits[i / 2] |= (uint32_t)row[col + i] << (16 * (i % 2));
+        }
     }
     return p;
   }

@@ -86,6 +86,14 @@ def test_gather_and_combine(dtype, t, top, experts, width):
         plain.close(expert_combine(y, weights, sort), exact, size, 2 * top)
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+def test_gather_copies_bits(dtype):
+    """Every value of 16 bits, signalling NaN too, in a row's whole pieces and in the part at its end."""
+    x = torch.arange(65536, dtype=torch.int32, device=DEV).to(torch.uint16).view(-1, 1).repeat(1, 11).view(dtype)
+    sort = expert_sort(torch.zeros(65536, 1, dtype=torch.int32, device=DEV), 1)
+    assert torch.equal(expert_gather(x, sort).view(torch.int16), x.view(torch.int16))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("t,top,experts,width", CASES)
 def test_gradients_match_formulas(dtype, t, top, experts, width):
