@@ -24,6 +24,7 @@ import ctypes
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._common import _check_cuda_contig
@@ -159,7 +160,8 @@ def expert_gather(x: torch.Tensor, sort: ExpertSort) -> torch.Tensor:
     _check_cuda(x, "x")
     _check_sort(sort, x.device)
     _check_rows(x, "x", sort.positions.shape[0])
-    _no_tangent("expert_gather", x)
+    if forward_ad._current_level >= 0:
+        _no_tangent("expert_gather", x)
     if not (x.requires_grad and torch.is_grad_enabled()):
         return _gather_rows(x.contiguous(), *sort)
     return _Gather.apply(x.contiguous(), *sort)
@@ -177,7 +179,8 @@ def expert_combine(y: torch.Tensor, weights: torch.Tensor, sort: ExpertSort) -> 
     _type(weights, "weights")
     if weights.shape != sort.positions.shape:
         raise ValueError(f"weights must have shape {tuple(sort.positions.shape)}, got {tuple(weights.shape)}")
-    _no_tangent("expert_combine", y, weights)
+    if forward_ad._current_level >= 0:
+        _no_tangent("expert_combine", y, weights)
     y, weights = y.contiguous(), weights.contiguous()
     if not ((y.requires_grad or weights.requires_grad) and torch.is_grad_enabled()):
         return _sum_rows(y, weights, sort.positions)
@@ -197,8 +200,7 @@ def mxfp4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     _check_cuda(x, "x")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _no_grad("mxfp4_expert_linear", x)
-    _no_grad("mxfp4_expert_linear", bias)
+    _no_grad("mxfp4_expert_linear", x, bias)
     device = x.device
     _check_sort(sort, device)
     _check_rows(x, "x", sort.positions.shape[0] if gather else sort.order.numel())

@@ -49,10 +49,13 @@ def _no_tangent(name: str, *tensors: Optional[torch.Tensor]) -> None:
                 raise RuntimeError(f"{name} has no forward-mode derivative: call it with the primal tensors")
 
 
-def _no_grad(name: str, t: Optional[torch.Tensor]) -> None:
-    _no_tangent(name, t)
-    if t is not None and t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
+def _no_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if forward_ad._current_level >= 0:
+        _no_tangent(name, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
 
 
 def _check_cuda(t: torch.Tensor, name: str, device: Optional[torch.device] = None) -> None:
@@ -113,7 +116,8 @@ def _check_out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: t
         return torch.empty(shape, dtype=dtype, device=device)
     if out.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("out must not require a gradient: the calls have none for it")
-    _no_tangent("a call with out", out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("a call with out", out)
     if out.dtype != dtype or out.device != device or not out.is_contiguous() or tuple(out.shape) != tuple(shape):
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
     torch.autograd.graph.increment_version(out)  # so that autograd knows if it had saved what is there now
@@ -199,8 +203,7 @@ def mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bia
     _check_cuda(x, "x")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
-    _no_grad("mxfp4_linear", x)
-    _no_grad("mxfp4_linear", bias)
+    _no_grad("mxfp4_linear", x, bias)
     shape, device = x.shape, x.device
     if len(shape) < 1:
         raise ValueError("x must have at least one dimension")
