@@ -20,7 +20,8 @@ struct ProductArgs {
 
 // The expert and the rows of tile `tile`, where every expert's rows are cut into tiles of `size`
 // rows and the rows past the last expert's into more tiles, as those of expert `experts`.
-// All lanes get the same answer; {-1, 0, 0} past the last tile.
+// All lanes get the same answer, and the compiler knows it (lanes are read, not shuffled), so that it stays in
+// scalar registers; {-1, 0, 0} past the last tile.
 struct Tile {
   int32_t expert, first, end;
 };
@@ -43,12 +44,12 @@ __device__ inline Tile find_tile(const int32_t *offsets, int32_t experts, int32_
     const uint64_t hit = __ballot(before + upto > tile);
     if (hit) {
       const int at = __ffsll((unsigned long long)hit) - 1;
-      const int32_t in = tile - before - (__shfl(upto, at) - __shfl(tiles, at));
-      if ((uint32_t)in >= (uint32_t)__shfl(tiles, at)) return {-1, 0, 0};  // bad offsets whose tiles add up to 2^31 and more
-      const int32_t f = __shfl(first, at) + in * size;
-      return {e0 + at, f, min(f + size, __shfl(end, at))};
+      const int32_t here = __builtin_amdgcn_readlane(tiles, at), in = tile - before - (__builtin_amdgcn_readlane(upto, at) - here);
+      if ((uint32_t)in >= (uint32_t)here) break;  // bad offsets whose tiles add up to 2^31 and more
+      const int32_t f = __builtin_amdgcn_readlane(first, at) + in * size;
+      return {e0 + at, f, min(f + size, __builtin_amdgcn_readlane(end, at))};
     }
-    before += __shfl(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return {-1, 0, 0};
 }
@@ -62,7 +63,7 @@ __device__ inline int32_t count_tiles(const int32_t *offsets, int32_t experts, i
     tiles += (end - first + size - 1) / size;
   }
   for (int d = 32; d > 0; d /= 2) tiles += __shfl_xor(tiles, d);
-  return tiles;
+  return __builtin_amdgcn_readfirstlane(tiles);
 }
 
 // Eight elements of a 16-bit row from `col` on, at any alignment, as bits; zeros past column k.
