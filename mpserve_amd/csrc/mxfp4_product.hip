@@ -1,9 +1,9 @@
 // Products with MXFP4 weights: y[t, n] = sum over k of x[t, k] * w[n, k], plus a bias.
 //
 // x is BF16, FP16 or MXFP4; w is MXFP4; sums are FP32 in the matrix cores and are rounded once, to
-// the output's type. With 16-bit x the weights' values are written out as BF16, which holds each
-// exactly (two significant bits and the exponent of the scale), and FP16 x as a BF16 sum
-// hi + lo, also exact: eight significant bits each, and FP16 has eleven.
+// the output's type. Products are exact: beside BF16 x the weights' values are widened to BF16, which holds
+// each (two significant bits and the exponent of the scale; near 2^127 a quarter of it), beside FP16 x
+// the codes' to FP16, a block's sum getting its scale in FP32, and MXFP4 x is multiplied as it is.
 //
 // For experts, rows of x belong to experts by ranges (offsets) and each expert has weights of
 // its own; rows may be gathered from a token's row by the sorted order.

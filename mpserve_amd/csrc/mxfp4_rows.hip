@@ -288,17 +288,17 @@ void launch(const ProductArgs &a, hipStream_t stream) {
 // of them fit a CU, and one takes `us` for each period of k (512 elements) that a wave has, as
 // measured with CUs full and half full (1 x 4096 x 14336, 16 x 4096 x 4096, 32 x 14336 x 4096, 64 x 8192 x
 // 8192, 64 x 4096 x 28672). More rows a workgroup spare reads of the weights, fewer fill more CUs, and more
-// waves share a long k: 64 x 8192 x 8192 in BF16 takes 16.9 us with XL 4, FN 4 and 37 with XL 1, FN 2, which
-// takes 7.5 for 1 x 4096 x 14336 where the first takes 10.0.
+// waves share a long k: 64 x 8192 x 8192 in BF16 takes 17.0 us with XL 4, FN 4 and 41 with XL 1, FN 2, which
+// takes 6.7 to 7.5 for 1 x 4096 x 14336 where the first takes 9.3 to 10.5.
 struct Choice {
   int32_t rows, cols, waves, resident;
   float us, start;
 };
-// Workgroups past the first on a CU cost `start` each beside (1200 to 8000 rows of 60 and 64 experts; 1200 rows of
-// 64 experts, 4096 x 2048, in BF16: 93 us with XL 4, FN 4, and 81 in tiles of 128 x 256, which are taken).
+// Workgroups past the first on a CU cost `start` each beside (1200 to 8000 rows of 60 and 64 experts; 1200 rows spread
+// evenly over 64 experts, 4096 x 2048, in BF16: 97 us with XL 4, FN 4, and 82 to 88 in tiles of 128 x 256, which are taken).
 constexpr Choice kChoicesBf16[] = {{8, 32, 4, 2, 2.5f, 1.3f}, {8, 32, 8, 1, 2.7f, 1.9f}, {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 4, 1, 2.8f, 2.1f},
                                    {32, 32, 6, 1, 3.2f, 1.2f}, {32, 64, 4, 1, 3.8f, 2.7f}, {64, 64, 4, 1, 6.2f, 3.5f}};
-// FP16's scaled sums cost more, the more rows (64 x 2048 x 8192 with XL 4, FN 4 7.1 us in BF16, 9.8 in FP16).
+// FP16's scaled sums cost more, the more rows (64 x 2048 x 8192 with XL 4, FN 4 7.2 us in BF16, 9.7 in FP16).
 constexpr Choice kChoicesF16[] = {{8, 32, 4, 2, 3.1f, 1.3f}, {8, 32, 8, 1, 3.4f, 1.9f}, {16, 32, 8, 1, 3.8f, 2.5f}, {16, 64, 4, 1, 3.6f, 2.1f},
                                   {32, 32, 6, 1, 3.8f, 1.2f}, {32, 64, 4, 1, 5.6f, 2.7f}, {64, 64, 4, 1, 9.6f, 3.5f}};
 constexpr Choice kChoices4[] = {{8, 32, 4, 2, 1.9f, 0}, {8, 32, 8, 1, 2.2f, 0}, {16, 32, 4, 2, 1.9f, 0}, {16, 32, 8, 1, 2.3f, 0},

@@ -17,10 +17,11 @@
 // the quarter: BF16 4096 x 4096 x 14336 411 us where these take 403, MXFP4 alike. Two barriers a
 // step, one for each half of x's rows, give loads half a step more to arrive and took 3 % longer.)
 //
-// What bounds it: BF16 the matrix cores, at 97 % of what the library's BF16 product of that size reaches
-// beside the widening. MXFP4 8192 x 8192 x 28672 takes 955 to 985 us, 4.0 PFLOP/s: the matrix cores are
-// busy for 52 % of the cycles, at clocks that the load brings down; without any loads to LDS and barriers
-// it would take 770, without stores 870.
+// What bounds it: the matrix cores, at clocks that the load brings down. BF16 4096 x 4096 x 14336 takes 391 to
+// 417 us, 1.15 to 1.23 PFLOP/s, with the matrix cores busy for 64 % of the cycles; the library's product with a BF16
+// weight [n, k] takes 326 to 368 on the same cards, with one [k, n] 395 where this took 391. MXFP4 8192 x 8192 x
+// 28672 takes 970 to 1010 us, 3.8 to 4.0 PFLOP/s, busy for 56 %; at 955, no loads to LDS and no barriers would have
+// made it 770, no stores 870.
 #include "mxfp4_product.h"
 
 namespace mps {
@@ -462,10 +463,11 @@ void launch(const ProductArgs &a, hipStream_t stream) {
 // The tiles, in microseconds. `start` is what a tile takes at any k, for its first loads and its stores
 // (8192 x 32 x 8192); `one` and `many` are what k = 4096 adds to a tile that has a CU to itself (128 x 8192 x
 // 8192 and 1024 x 4096 x 4096) and to each of several (4096 x 4096 x 14336). So BF16 4096 x 4096 x 14336 takes
-// 128 x 256 tiles, 398 us where 128 x 128 take 449, and 512 x 2048 x 1024 takes 64 x 64, 14 us where 128 x
-// 256 take 30. (BF16 in tiles of 256 x 256, one workgroup of eight waves a CU: 417 us; MXFP4 in 128 x
+// 128 x 256 tiles, 395 us where 128 x 128 take 450, and for 512 x 2048 x 1024 the least of the tiles are 64 x 64, 13 us
+// where 128 x 256 take 31 and the kernel of few rows, which is taken, 7. (BF16 in tiles of 256 x 256, one workgroup of eight waves a CU: 417 us; MXFP4 in 128 x
 // 256, 16 % slower than 256 x 256.) `half` is the share that one of several tiles spares if its rows are in
-// its first half only (2400 rows of 64 experts, 4096 x 2048, in BF16: 85 us in 128 x 256, 100 in 64 x 128).
+// its first half only (2400 rows spread evenly over 64 experts, 4096 x 2048, in BF16: 86 to 95 us in 128 x 256, 108 in
+// 64 x 128; a router that likes some experts more, which the host cannot know, makes it 147 to 160 and 132).
 struct Choice {
   int32_t bt, bn;
   float start, one, many, half;
@@ -485,7 +487,7 @@ Prediction least(const ProductArgs &a, const Choice (&choices)[N], int32_t cus) 
     // The count of experts' tiles is a guess, unless most have one: the mean over a tenth less and more, lest a
     // second round of a few tiles comes unawares (1872 rows of 60 experts, k = 5016, n = 896, had 264 for 256
     // CUs). Experts' weights are no other tile's, and come later (`start` by 3.5 us: 64 x 64 and 64 x 128
-    // took 147 and 95 us for 1200 rows of 64 experts, 4096 x 2048, where 119 and 81 would follow).
+    // take 151 and 96 us for 1200 rows spread evenly over 64 experts, 4096 x 2048, where 119 and 81 would follow).
     const bool sure = a.rows >= 4.0 * a.experts && a.rows <= 0.6 * c.bt * a.experts;
     const double start = c.start + (a.offsets ? 3.5 : 0), spread = a.offsets && !sure ? 0.1 : 0;
     const double whole = 1 - c.half * expected_halves(a, c.bt);
