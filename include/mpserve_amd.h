@@ -387,6 +387,62 @@ int mps_expert_combine_grad(const void *y, const void *dout, int32_t type, const
                             int64_t tokens, int64_t top, int64_t experts, int64_t width, const int32_t *order,
                             const int32_t *positions, const int32_t *offsets, void *dy, void *dweights, void *stream);
 
+/* ------------------------------------------------------ int4 products and the experts' router
+ * As above: asynchronous on `stream`, nothing allocated, capturable. */
+
+/* out[rows, n] = x[rows, k] times the transpose of w[n, k], plus bias[n]; x in BF16 or FP16,
+ * w[n, k] = scales[n, k / group] * (q[n, k] - zeros[n, k / group]) with whole numbers q below 16, and zeros
+ * up to 16 (their low five bits count; NULL: 8). Sums are FP32, with one rounding to out_type. Codes: blocks of 32 elements, 16
+ * bytes each, ceil(k / 32) a row, 16-byte aligned; byte b of each 4 bytes holds element b of eight in its
+ * low half and element b + 4 in its high half. What the last block holds past column k does not matter.
+ * `group` is a power of two, at least 32; scales (BF16 or FP16) and zeros have ceil(k / group) columns.
+ * Experts, offsets, order, top and gather are as in mps_mxfp4_product. */
+typedef struct mps_int4_product {
+  const void *x;
+  int64_t x_stride; /* elements from row to row */
+  const uint8_t *w;
+  const void *scales;
+  const uint8_t *zeros; /* may be NULL */
+  const void *bias;     /* may be NULL */
+  void *out;
+  const int32_t *offsets; /* [experts + 1] */
+  const int32_t *order;   /* [rows], gather only */
+  int64_t rows, n, k, group;
+  int64_t experts; /* 0: one weight for all rows */
+  int64_t top;
+  int32_t gather;
+  int32_t x_type, scale_type, bias_type, out_type;
+} mps_int4_product;
+int mps_int4_product_workspace(const mps_int4_product *product, int64_t *bytes);
+int mps_int4_multiply(const mps_int4_product *product, void *workspace, int64_t workspace_bytes, void *stream);
+
+#define MPS_SCORES_SOFTMAX 0
+#define MPS_SCORES_SIGMOID 1
+
+/* The `top` experts of each row of logits[tokens, experts] (`stride` elements from row to row) and their weights:
+ * ids and weights are [tokens, top], by falling key, ties to the lower expert. The key is the logit, or with
+ * bias[experts] score + bias in 64 bits; a score is the row's softmax or the logit's sigmoid. Experts whose logit or key is -inf
+ * or NaN are not taken: where fewer than `top` are left, ids are -1 and weights 0. A weight is scale * share; a share is the
+ * expert's score, with `normalize` divided by the sum of the row's chosen scores. shares[tokens, top] may be NULL. */
+int mps_expert_route(const void *logits, int32_t type, int64_t tokens, int64_t experts, int64_t stride, int64_t top,
+                     int32_t scores, const float *bias, int32_t normalize, float scale, int32_t *ids, float *weights,
+                     float *shares, void *stream);
+/* dlogits[tokens, experts], of the type of the logits, from dweights[tokens, top] and what the call above gave. */
+int mps_expert_route_grad(const void *logits, int32_t type, int64_t tokens, int64_t experts, int64_t stride, int64_t top,
+                          int32_t scores, int32_t normalize, float scale, const int32_t *ids, const float *shares,
+                          const float *dweights, void *dlogits, void *stream);
+/* counts[e]: the pairs of ids[tokens, top] (int32, or int64 with ids_64) of expert e. kept[experts + 1]: the same, and
+ * the tokens T that have a logit above -inf, for the gradient. Both may be NULL. loss = experts * sum over e of counts[e] / N * P[e], with N the sum of the counts and
+ * P[e] the mean over these T tokens of p[t, e], the softmax of the logits or their sigmoids divided by the sigmoids' sum;
+ * 0 if N or T is 0. */
+int mps_expert_balance_workspace(int64_t tokens, int64_t experts, int64_t top, int64_t *bytes);
+int mps_expert_balance(const void *logits, int32_t type, int64_t tokens, int64_t experts, int64_t stride, int32_t scores,
+                       const void *ids, int32_t ids_64, int64_t top, float *loss, int32_t *counts, int32_t *kept,
+                       void *workspace, int64_t workspace_bytes, void *stream);
+/* dlogits[tokens, experts], of the type of the logits, from *dloss (device memory) and `kept`; 0 where a logit is -inf. */
+int mps_expert_balance_grad(const void *logits, int32_t type, int64_t tokens, int64_t experts, int64_t stride, int32_t scores,
+                            const int32_t *kept, const float *dloss, void *dlogits, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

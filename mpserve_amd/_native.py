@@ -92,6 +92,20 @@ class MpsMxfp4Product(ctypes.Structure):
     ]
 
 
+class MpsInt4Product(ctypes.Structure):
+    """mps_int4_product: operands of a product with int4 weights, device pointers."""
+
+    _fields_ = [
+        ("x", _p), ("x_stride", _i64), ("w", _p), ("scales", _p), ("zeros", _p), ("bias", _p), ("out", _p),
+        ("offsets", _p), ("order", _p), ("rows", _i64), ("n", _i64), ("k", _i64), ("group", _i64), ("experts", _i64),
+        ("top", _i64), ("gather", ctypes.c_int32), ("x_type", ctypes.c_int32), ("scale_type", ctypes.c_int32),
+        ("bias_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+    ]
+
+
+#: what a router makes of its logits
+MPS_SCORES_SOFTMAX, MPS_SCORES_SIGMOID = 0, 1
+
 #: mps_encode_alloc: (ctx, slot, bytes) -> device pointer, or None for no memory
 ENCODE_ALLOC = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, _i64)
 
@@ -147,6 +161,17 @@ def lib():
     L.mps_expert_gather.argtypes = [_p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p]
     L.mps_expert_combine.argtypes = [_p, i32, _p, i32, _i64, _i64, _i64, _p, _p, _p]
     L.mps_expert_combine_grad.argtypes = [_p, _p, i32, _p, i32, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]
+    f32 = ctypes.c_float
+    L.mps_int4_product_workspace.argtypes = [ctypes.POINTER(MpsInt4Product), ctypes.POINTER(_i64)]
+    L.mps_int4_multiply.argtypes = [ctypes.POINTER(MpsInt4Product), _p, _i64, _p]
+    L.mps_expert_route.argtypes = [_p, i32, _i64, _i64, _i64, _i64, i32, _p, i32, f32, _p, _p, _p, _p]
+    L.mps_expert_route_grad.argtypes = [_p, i32, _i64, _i64, _i64, _i64, i32, i32, f32, _p, _p, _p, _p, _p]
+    L.mps_expert_balance_workspace.argtypes = [_i64, _i64, _i64, ctypes.POINTER(_i64)]
+    L.mps_expert_balance.argtypes = [_p, i32, _i64, _i64, _i64, i32, _p, i32, _i64, _p, _p, _p, _p, _i64, _p]
+    L.mps_expert_balance_grad.argtypes = [_p, i32, _i64, _i64, _i64, i32, _p, _p, _p, _p]
+    for name in ("mps_int4_product_workspace", "mps_int4_multiply", "mps_expert_route", "mps_expert_route_grad",
+                 "mps_expert_balance_workspace", "mps_expert_balance", "mps_expert_balance_grad"):
+        getattr(L, name).restype = ctypes.c_int
     for name in ("mps_mxfp4_quantize", "mps_mxfp4_dequantize", "mps_mxfp4_product_workspace", "mps_mxfp4_multiply",
                  "mps_expert_sort_workspace", "mps_expert_sort", "mps_expert_gather", "mps_expert_combine",
                  "mps_expert_combine_grad"):

@@ -1,11 +1,14 @@
-"""Mixtures of experts: tokens to their experts and back, and products with MXFP4 experts.
+"""Mixtures of experts: the router, tokens to their experts and back, and products with MXFP4 and int4 experts.
 
 A router gives each of ``t`` tokens ``top`` experts; an expert id outside ``[0, experts)`` (say
 -1) means none here: the pair was dropped, or its expert is on another rank.
 
+* :func:`expert_route` — from a router's logits to experts and weights (differentiable);
+* :func:`expert_balance` — the loss that keeps experts' loads alike, and their counts (differentiable);
 * :func:`expert_sort` — the pairs of tokens and experts ordered by expert;
 * :func:`expert_gather` — the tokens' rows in that order (differentiable);
 * :func:`mxfp4_expert_linear` — each row times its expert's MXFP4 weight;
+* :func:`int4_expert_linear` — each row times its expert's int4 weight;
 * :func:`expert_combine` — the weighted sum of each token's rows (differentiable).
 
 Shapes do not depend on the routing, so nothing synchronises and all of it can be captured
@@ -28,7 +31,20 @@ from torch.autograd import forward_ad
 
 from . import _native
 from ._common import _check_cuda_contig
+from .int4 import _check_int4, _HALVES, _int4_multiply, _int4_product
 from .mxfp4 import BLOCK, _TYPES, _call, _check_bias, _check_cuda, _check_mx, _check_out, _multiply, _no_grad, _no_tangent, _set_x, _type
+
+
+class ExpertRoute(NamedTuple):
+    """Each token's experts, by falling score."""
+    ids: torch.Tensor      # int32 [t, top]: -1 where no expert was left
+    weights: torch.Tensor  # FP32 [t, top]: 0 there
+
+
+class ExpertBalance(NamedTuple):
+    """A batch's balance loss and loads."""
+    loss: torch.Tensor    # FP32, no dimensions
+    counts: torch.Tensor  # int32 [experts]: pairs of each expert
 
 
 class ExpertSort(NamedTuple):
@@ -226,3 +242,209 @@ def mxfp4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     p.top, p.gather = max(1, sort.positions.shape[1]), bool(gather)
     _multiply(p, whole, device)
     return out
+
+
+def int4_expert_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, sort: ExpertSort,
+                       zeros: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *, group: int = 128,
+                       gather: bool = False, out_dtype: Optional[torch.dtype] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[j] = x[j] @ w[e].T + bias[e]`` for the rows ``j`` of expert ``e`` in the sorted order.
+
+    As :func:`mxfp4_expert_linear`, with the experts' weights in int4: ``codes [experts, n, 16 * ceil(k / 32)]``,
+    ``scales [experts, n, ceil(k / group)]`` and ``zeros`` of that shape or None, as ``int4_linear`` takes
+    them. Returns ``y [t * top, n]``; the places of pairs of no expert are zero."""
+    _check_cuda(x, "x")
+    if x.dtype not in _HALVES:
+        raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
+    _no_grad("int4_expert_linear", x, scales, bias)
+    device, group = x.device, int(group)
+    _check_sort(sort, device)
+    _check_rows(x, "x", sort.positions.shape[0] if gather else sort.order.numel())
+    k = x.shape[1]
+    _check_int4(codes, scales, zeros, k, group, 3, device)
+    experts, n = codes.shape[0], codes.shape[1]
+    if sort.offsets.numel() != experts + 1:
+        raise ValueError(f"sort has {sort.offsets.numel() - 1} experts and codes {experts}")
+    dtype = out_dtype if out_dtype is not None else (out.dtype if out is not None else x.dtype)
+    out_type, bias_type, rows = _type(dtype, "out_dtype"), _check_bias(bias, (experts, n), device), sort.order.numel()
+    out = _check_out(out, (rows, n), dtype, device)
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    p = _int4_product(x, codes, scales, zeros, bias, group, k, n)
+    p.rows, p.out, p.out_type, p.bias_type = rows, out.data_ptr(), out_type, bias_type
+    p.experts, p.offsets, p.order = experts, sort.offsets.data_ptr(), sort.order.data_ptr()
+    p.top, p.gather = max(1, sort.positions.shape[1]), bool(gather)
+    _int4_multiply(p, device)
+    return out
+
+
+_SCORES = {"softmax": _native.MPS_SCORES_SOFTMAX, "sigmoid": _native.MPS_SCORES_SIGMOID}
+
+
+def _check_logits(logits: torch.Tensor, scores: str) -> int:
+    _check_cuda(logits, "logits")
+    _type(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must have 2 dimensions")
+    if not 1 <= logits.shape[1] <= _native.MPS_MAX_EXPERTS:
+        raise ValueError(f"logits must have 1 to {_native.MPS_MAX_EXPERTS} columns, got {logits.shape[1]}")
+    code = _SCORES.get(scores)
+    if code is None:
+        raise ValueError(f"scores must be 'softmax' or 'sigmoid', got {scores!r}")
+    return code
+
+
+def _adjacent(logits: torch.Tensor) -> torch.Tensor:
+    return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+
+
+def _route(logits, top, code, bias, normalize, scale, shares):
+    (t, experts), device = logits.shape, logits.device
+    ids = torch.empty((t, top), dtype=torch.int32, device=device)
+    weights = torch.empty((t, top), dtype=torch.float32, device=device)
+    kept = torch.empty_like(weights) if shares else None
+    _call(device, _native.lib().mps_expert_route, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0), top, code,
+          bias.data_ptr() if bias is not None else None, normalize, scale, ids.data_ptr(), weights.data_ptr(),
+          kept.data_ptr() if shares else None)
+    return ids, weights, kept
+
+
+class _NoSecond(torch.autograd.Function):
+    """A gradient that has none itself: of a tensor that hangs on ``sources``, so that one is refused, not left out."""
+
+    @staticmethod
+    def forward(ctx, gradient, name, *sources):
+        ctx.name = name
+        return gradient
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"the gradient of {ctx.name} has no gradient")
+
+
+def _only_gradient(gradient, name, ctx, grad):
+    if not torch.is_grad_enabled():
+        return gradient(ctx, grad)
+    with torch.no_grad():
+        d = gradient(ctx, grad)
+    return _NoSecond.apply(d, name, grad, ctx.saved_tensors[0])
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top, code, bias, normalize, scale):
+        ids, weights, shares = _route(logits, top, code, bias, normalize, scale, scale != 1.0)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, ids, weights if shares is None else shares)
+        ctx.how = code, normalize, scale
+        return ids, weights
+
+    @staticmethod
+    def backward(ctx, _, dweights):
+        return None if dweights is None else _only_gradient(_route_grad, "expert_route", ctx, dweights), None, None, None, None, None
+
+
+def _route_grad(ctx, dweights):
+    logits, ids, shares = ctx.saved_tensors
+    (t, experts), (code, normalize, scale) = logits.shape, ctx.how
+    dweights = dweights.contiguous()
+    dlogits = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
+    _call(logits.device, _native.lib().mps_expert_route_grad, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0),
+          ids.shape[1], code, normalize, scale, ids.data_ptr(), shares.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
+    return dlogits
+
+
+
+def expert_route(logits: torch.Tensor, top: int, *, scores: str = "softmax", bias: Optional[torch.Tensor] = None,
+                 normalize: bool = True, scale: float = 1.0) -> ExpertRoute:
+    """The ``top`` experts of each token, by falling score, and their weights.
+
+    ``logits [t, experts]`` are BF16, FP16 or FP32; ``scores`` is ``"softmax"`` (over a token's logits) or
+    ``"sigmoid"``. The experts of the largest logits are taken, or with ``bias [experts]`` (FP32) those of the largest
+    ``score + bias``, compared in FP64; ties go to the lower expert. The bias counts for the choice only. A weight is the expert's score,
+    with ``normalize`` divided by the sum of the token's chosen scores, times ``scale``. An expert whose logit or
+    bias is -inf (or whose logit is NaN) is not taken: where fewer than ``top`` are left, as in a row of padding, ids are
+    -1 and weights 0, which :func:`expert_sort` and :func:`expert_combine` take for no expert. The gradient is that of the
+    weights; the choice has none."""
+    code = _check_logits(logits, scores)
+    top = int(top)
+    (t, experts), device = logits.shape, logits.device
+    if not 0 <= top <= experts:
+        raise ValueError(f"top must be in [0, {experts}], got {top}")
+    if bias is not None:
+        _check_cuda_contig(bias, "bias", device)
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (experts,):
+            raise ValueError(f"bias must be torch.float32 of shape {(experts,)}, got {bias.dtype} {tuple(bias.shape)}")
+        _no_grad("the bias of expert_route", bias)
+    if forward_ad._current_level >= 0:
+        _no_tangent("expert_route", logits)
+    logits, normalize, scale = _adjacent(logits), bool(normalize), float(scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return ExpertRoute(*_Route.apply(logits, top, code, bias, normalize, scale))
+    return ExpertRoute(*_route(logits, top, code, bias, normalize, scale, False)[:2])
+
+
+def _balance(logits, ids, code, keep):
+    (t, experts), device = logits.shape, logits.device
+    lib = _native.lib()
+    need = ctypes.c_int64(0)
+    rc = lib.mps_expert_balance_workspace(t, experts, ids.shape[1], need)
+    if rc:
+        _native.check(rc)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    counts = torch.empty(experts, dtype=torch.int32, device=device)
+    kept = torch.empty(experts + 1, dtype=torch.int32, device=device) if keep else None
+    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    _call(device, lib.mps_expert_balance, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0), code, ids.data_ptr(),
+          ids.dtype == torch.int64, ids.shape[1], loss.data_ptr(), counts.data_ptr(), kept.data_ptr() if keep else None,
+          work.data_ptr() if need.value else None, need.value)
+    return loss, counts, kept
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, code):
+        loss, counts, kept = _balance(logits, ids, code, True)
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, kept)  # not the counts: a program may add up its ranks' in place
+        ctx.code = code
+        return loss, counts
+
+    @staticmethod
+    def backward(ctx, dloss, _):
+        return None if dloss is None else _only_gradient(_balance_grad, "expert_balance", ctx, dloss), None, None
+
+
+def _balance_grad(ctx, dloss):
+    logits, kept = ctx.saved_tensors
+    t, experts = logits.shape
+    dloss = dloss.contiguous()
+    dlogits = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
+    _call(logits.device, _native.lib().mps_expert_balance_grad, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0),
+          ctx.code, kept.data_ptr(), dloss.data_ptr(), dlogits.data_ptr())
+    return dlogits
+
+
+
+def expert_balance(logits: torch.Tensor, ids: torch.Tensor, *, scores: str = "softmax") -> ExpertBalance:
+    """The balance loss of a batch, ``experts * sum over e of f[e] * P[e]``, and each expert's count of pairs.
+
+    ``f[e]`` is the share of the pairs of ``ids [t, top]`` (int32 or int64; an id outside ``[0, experts)`` is no expert's)
+    that are expert ``e``'s, ``P[e]`` the mean over the tokens of ``p[t, e]``, the softmax of ``logits [t, experts]``
+    (BF16, FP16 or FP32) or, for ``"sigmoid"``, their sigmoids divided by the token's sum of them. The loss is 1 where either is alike for
+    all experts. Tokens whose logits are all -inf, as padding's are, count for nothing; without pairs or tokens the loss is
+    0. Sums are in a fixed order. The gradient is that of ``P``: the counts have none."""
+    code = _check_logits(logits, scores)
+    _check_cuda_contig(ids, "ids", logits.device)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be torch.int32 or torch.int64, got {ids.dtype}")
+    if ids.dim() != 2 or ids.shape[0] != logits.shape[0]:
+        raise ValueError(f"ids must have shape [{logits.shape[0]}, top], got {tuple(ids.shape)}")
+    if forward_ad._current_level >= 0:
+        _no_tangent("expert_balance", logits)
+    logits = _adjacent(logits)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return ExpertBalance(*_Balance.apply(logits, ids, code))
+    return ExpertBalance(*_balance(logits, ids, code, False)[:2])
