@@ -245,8 +245,10 @@ def _own(s):
         return int4_linear(s["x"], s["codes"], s["scales"], s["zeros"], s["bias"], group=s["group"])
     if kind == "experts":
         sort = expert_sort(s["ids"], s["codes"].shape[0])
-        y = int4_expert_linear(s["x"], s["codes"], s["scales"], sort, s["zeros"], s["bias"], group=s["group"], gather=True)
-        return expert_combine(y, s["weights"], sort)
+        # rows in 32 bits until they are added up: the plain form rounds once, too
+        y = int4_expert_linear(s["x"], s["codes"], s["scales"], sort, s["zeros"], s["bias"], group=s["group"], gather=True,
+                               out_dtype=torch.float32)
+        return expert_combine(y, s["weights"], sort).to(s["x"].dtype)
     if kind == "route":
         ids, weights = expert_route(s["logits"], s["top"], scores=s["scores"], bias=s["bias"], normalize=s["normalize"],
                                     scale=s["scale"])
