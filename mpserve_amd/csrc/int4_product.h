@@ -15,15 +15,27 @@ struct Int4Args : ProductArgs {
   int32_t scale_type, groups, shift;  // groups a row; blocks a group, as a power of two
 };
 
-// Scale and zero of a weight's row `row` (of all experts') and group.
-__device__ inline float int4_scale(const Int4Args &a, int64_t row, int32_t group) {
-  return load_as_float(a.scales, a.scale_type, row * a.groups + group);
-}
-__device__ inline float int4_zero(const Int4Args &a, int64_t row, int32_t group) {
-  return a.zeros ? (float)(a.zeros[row * a.groups + group] & 31) : 8.0f;
+// Eight codes as they are, 0 to 15, in 16 bits, exactly: a byte below 16 is an FP8 (e4m3) number too, 2^-9 times its
+// value, which the conversions multiply by 2^9. Three masks and shifts and four conversions for eight values.
+template <int XT>
+__device__ inline u32x4 int4_codes(uint32_t codes) {
+  const uint32_t lo = codes & 0x0f0f0f0fu, hi = codes >> 4 & 0x0f0f0f0fu;
+  u32x4 v;
+  if constexpr (XT == MPS_TYPE_BF16) {
+    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false));
+    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true));
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true));
+  } else {
+    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false));
+    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true));
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true));
+  }
+  return v;
 }
 
-// Eight codes less their zero, exactly, in 16 bits.
+// Eight codes less their zero, exactly, in 16 bits: three times the instructions.
 template <int XT>
 __device__ inline u32x4 int4_values(uint32_t codes, float zero) {
   const uint32_t lo = codes & 0x0f0f0f0fu, hi = codes >> 4 & 0x0f0f0f0fu;
@@ -37,6 +49,17 @@ __device__ inline u32x4 int4_values(uint32_t codes, float zero) {
   return v;
 }
 
+// Eight ones: x times these is the sum of x.
+template <int XT>
+__device__ inline u32x4 int4_ones() {
+  constexpr uint32_t two = XT == MPS_TYPE_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  return u32x4{two, two, two, two};
+}
+
+__device__ inline float scale_value(uint32_t bits, int32_t type) {
+  return type == MPS_TYPE_BF16 ? Elem<MPS_TYPE_BF16>::get((uint16_t)bits) : Elem<MPS_TYPE_F16>::get((uint16_t)bits);
+}
+
 template <int XT>
 __device__ inline f32x4 mfma16(u32x4 x, u32x4 w, f32x4 c) {
   if constexpr (XT == MPS_TYPE_BF16)
@@ -44,5 +67,57 @@ __device__ inline f32x4 mfma16(u32x4 x, u32x4 w, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, w), c, 0, 0, 0);
 }
+
+// A period is 16 blocks. Groups of at least 128 have at most four of a row's scales in one (kFew), finer ones up to
+// sixteen; a row's scales and zeros are read a period ahead in windows of that many, at any alignment, which
+// near a row's end begin earlier: `window_start`, alike for all rows.
+template <bool kFew>
+struct Window {
+  static constexpr int kEntries = kFew ? 4 : 16, kBytes = kFew ? 16 : 48;  // of LDS, a row: scales, then zeros
+  uint32_t scales[kEntries / 2], zeros[kEntries / 4];
+};
+template <bool kFew>
+__device__ inline int32_t window_start(const Int4Args &a, int32_t period) {
+  return max(0, min((16 * period) >> a.shift, a.groups - Window<kFew>::kEntries));
+}
+template <bool kFew>
+__device__ inline void load_window(const Int4Args &a, int64_t row, int32_t start, Window<kFew> &w) {
+  constexpr int kEntries = Window<kFew>::kEntries;
+  const uint16_t *const s = static_cast<const uint16_t *>(a.scales) + row * a.groups + start;
+  const uint8_t *const z = a.zeros + row * a.groups + start;
+  if (a.groups >= kEntries) {
+    __builtin_memcpy(w.scales, s, sizeof(w.scales));
+    if (a.zeros) __builtin_memcpy(w.zeros, z, sizeof(w.zeros));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEntries / 2; ++i) w.scales[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kEntries / 4; ++i) w.zeros[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i)
+      if (i < a.groups) {
+        w.scales[i / 2] |= (uint32_t)s[i] << (16 * (i % 2));
+        if (a.zeros) w.zeros[i / 4] |= (uint32_t)z[i] << (8 * (i % 4));
+      }
+  }
+}
+template <bool kFew>
+__device__ inline void put_window(const Int4Args &a, const Window<kFew> &w, uint8_t *lds) {
+  constexpr int kEntries = Window<kFew>::kEntries;
+  uint32_t *const to = reinterpret_cast<uint32_t *>(lds);
+#pragma unroll
+  for (int i = 0; i < kEntries / 2; ++i) to[i] = w.scales[i];
+#pragma unroll
+  for (int i = 0; i < kEntries / 4; ++i) to[kEntries / 2 + i] = a.zeros ? w.zeros[i] & 0x1f1f1f1fu : 0x08080808u;
+}
+template <bool kFew>
+__device__ inline void read_window(const Int4Args &a, const uint8_t *row, int32_t entry, float &scale, float &zero) {
+  scale = scale_value(*reinterpret_cast<const uint16_t *>(row + 2 * entry), a.scale_type);
+  zero = (float)row[2 * Window<kFew>::kEntries + entry];
+}
+
+// Few rows (int4_rows.hip): x is 16-bit rows of whole 16-byte pieces.
+Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus);
+void launch_int4_rows(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
 
 }  // namespace mps

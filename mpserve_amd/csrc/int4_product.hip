@@ -7,41 +7,14 @@
 namespace mps {
 namespace {
 
-// A wave a 16 x 16 tile, from memory: lane 16 g + r has piece g of a block of k, of row r of x and of the weight.
-template <int XT>
-__global__ __launch_bounds__(64) void int4_simple_kernel(Int4Args a) {
-  const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-  Tile tile = {0, (int32_t)blockIdx.y * 16, 0};
-  tile.end = min(a.rows, tile.first + 16);
-  if (a.offsets) tile = find_tile(a.offsets, a.experts, a.rows, 16, blockIdx.y);
-  if (tile.expert < 0) return;
-  const bool none = tile.expert >= max(a.experts, 1);
-  const int32_t n0 = blockIdx.x * 16;
-  int32_t from = min(tile.first + r, tile.end - 1);
-  if (a.gather) from = min((uint32_t)a.order[from] / (uint32_t)a.top, (uint32_t)a.x_rows - 1);
-  const uint16_t *const x = static_cast<const uint16_t *>(a.x) + from * a.x_stride;
-  const int64_t w_row = (int64_t)(none ? 0 : tile.expert) * a.n + min(n0 + r, a.n - 1);
-  const uint8_t *const w = a.w + w_row * a.row_blocks * 16;
-  f32x4 sum = {0, 0, 0, 0};
-  for (int32_t b0 = 0; b0 < (none ? 0 : a.row_blocks); b0 += 1 << a.shift) {
-    const int32_t group = b0 >> a.shift;
-    const float scale = int4_scale(a, w_row, group), zero = int4_zero(a, w_row, group);
-    f32x4 part = {0, 0, 0, 0};
-    for (int32_t b = b0; b < min(a.row_blocks, b0 + (1 << a.shift)); ++b) {
-      const u32x4 xv = load_row8(x, (int64_t)b * 32 + g * 8, a.k);
-      const uint32_t codes = *reinterpret_cast<const uint32_t *>(w + (int64_t)b * 16 + g * 4);
-      part = mfma16<XT>(xv, int4_values<XT>(codes, zero), part);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(scale, part[i], sum[i]);
-  }
-  const int32_t col = n0 + r;
-  if (col >= a.n) return;
-  const float bias = a.bias && !none ? load_as_float(a.bias, a.bias_type, (int64_t)tile.expert * a.n + col) : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t row = tile.first + 4 * g + i;
-    if (row < tile.end) store_as(a.out, a.out_type, (int64_t)row * a.n + col, sum[i] + bias);
+// x[rows, k] as rows of whole blocks, `width` elements wide, with zeros past column k; eight elements a work-item.
+__global__ __launch_bounds__(256) void int4_pack_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride, int32_t k, int32_t width,
+                                                        uint16_t *__restrict__ out) {
+  const uint32_t pieces = (uint32_t)width / 8;
+  for (int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x; unit < rows * pieces; unit += (int64_t)gridDim.x * 256) {
+    const int64_t row = unit / pieces;
+    const int32_t col = (int32_t)(unit - row * pieces) * 8;
+    *reinterpret_cast<u32x4 *>(out + row * width + col) = load_row8(x + row * stride, col, k);
   }
 }
 
@@ -73,6 +46,32 @@ int check(const mps_int4_product *p) {
   return MPS_OK;
 }
 
+// Which kernel takes a product, and what it needs.
+struct Way {
+  Int4Args args;
+  int choice;
+  bool packed;  // x is packed into the workspace first
+  int64_t workspace;
+};
+Way way_of(const mps_int4_product *p) {
+  Way w = {};
+  Int4Args &a = w.args;
+  a.x = p->x, a.x_stride = p->x_stride, a.w = p->w, a.bias = p->bias, a.out = p->out;
+  a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
+  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)(p->gather ? p->rows / p->top : p->rows);
+  a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
+  a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
+  a.bias_type = p->bias_type, a.out_type = p->out_type;
+  a.scales = p->scales, a.zeros = p->zeros, a.scale_type = p->scale_type;
+  a.groups = (int32_t)((p->k + p->group - 1) / p->group);
+  while ((int64_t)32 << a.shift < p->group) ++a.shift;
+  const Prediction rows = predict_int4_rows(a, p->x_type, compute_units());
+  w.choice = rows.choice;
+  w.packed = p->k > 0 && !piece_rows(p->x, p->x_stride, p->k);
+  if (w.packed) w.workspace = a.x_rows * packed_width(p->k) * 2;
+  return w;
+}
+
 }  // namespace
 }  // namespace mps
 
@@ -85,7 +84,7 @@ int mps_int4_product_workspace(const mps_int4_product *p, int64_t *bytes) {
   const int rc = check(p);
   if (rc != MPS_OK) return rc;
   if (!bytes) return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product: null pointer");
-  *bytes = 0;
+  *bytes = p->rows > 0 && p->n > 0 ? way_of(p).workspace : 0;
   return MPS_OK;
 }
 
@@ -93,24 +92,20 @@ int mps_int4_multiply(const mps_int4_product *p, void *workspace, int64_t worksp
   last_error().clear();
   const int rc = check(p);
   if (rc != MPS_OK || p->rows == 0 || p->n == 0) return rc;
-  Int4Args a = {};
-  a.x = p->x, a.x_stride = p->x_stride, a.w = p->w, a.bias = p->bias, a.out = p->out;
-  a.offsets = p->experts > 0 ? p->offsets : nullptr, a.order = p->order;
-  a.rows = (int32_t)p->rows, a.x_rows = (int32_t)(p->gather ? p->rows / p->top : p->rows);
-  a.n = (int32_t)p->n, a.k = (int32_t)p->k, a.row_blocks = (int32_t)mx_blocks(p->k);
-  a.experts = (int32_t)p->experts, a.top = (int32_t)p->top, a.gather = p->gather;
-  a.bias_type = p->bias_type, a.out_type = p->out_type;
-  a.scales = p->scales, a.zeros = p->zeros, a.scale_type = p->scale_type;
-  a.groups = (int32_t)((p->k + p->group - 1) / p->group);
-  while ((int64_t)32 << a.shift < p->group) ++a.shift;
-  const int64_t tiles = product_tiles(a, 16);
-  const dim3 grid((unsigned)((a.n + 15) / 16), (unsigned)tiles);
-  if (tiles > 65535) return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product: too many rows");
+  const Way way = way_of(p);
+  if (way.choice < 0) return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product: %lld x %lld outputs are too many", (long long)p->rows, (long long)p->n);
+  if (way.workspace > 0 && (!workspace || workspace_bytes < way.workspace || !aligned16(workspace)))
+    return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product: %lld bytes of workspace are needed, 16-byte aligned", (long long)way.workspace);
+  Int4Args a = way.args;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (p->x_type == MPS_TYPE_BF16)
-    hipLaunchKernelGGL(int4_simple_kernel<MPS_TYPE_BF16>, grid, dim3(64), 0, s, a);
-  else
-    hipLaunchKernelGGL(int4_simple_kernel<MPS_TYPE_F16>, grid, dim3(64), 0, s, a);
+  if (way.packed) {
+    const int32_t width = (int32_t)packed_width(p->k);
+    const dim3 grid(workgroups(((int64_t)a.x_rows * (width / 8) + 255) / 256));
+    hipLaunchKernelGGL(int4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), (int64_t)a.x_rows, p->x_stride, a.k,
+                       width, static_cast<uint16_t *>(workspace));
+    a.x = workspace, a.x_stride = width, a.k = width;
+  }
+  launch_int4_rows(a, p->x_type, way.choice, s);
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
 }

@@ -210,6 +210,9 @@ inline double expected_halves(const ProductArgs &a, int64_t size) {
 
 constexpr double kMostWorkItems = 4294967295.0;  // of a grid, in one direction
 
+// The current device's CUs; asked once a device (mxfp4_product.hip).
+int32_t compute_units();
+
 // One of a kernel's shapes (-1: none fits a grid), and the microseconds that it is predicted to take (the launch and the first
 // loads, alike for all, are left out).
 struct Prediction {

@@ -59,7 +59,8 @@ int check(const mps_mxfp4_product *p) {
   return MPS_OK;
 }
 
-// The current device's CUs; asked once a device.
+}  // namespace
+
 int32_t compute_units() {
   constexpr int kDevices = 64;
   static std::atomic<int32_t> known[kDevices];
@@ -70,6 +71,8 @@ int32_t compute_units() {
   known[device].store(cus, std::memory_order_relaxed);
   return cus;
 }
+
+namespace {
 
 // Which kernel takes a product, and what it needs.
 struct Way {
