@@ -13,7 +13,17 @@ struct Int4Args : ProductArgs {
   const void *scales;
   const uint8_t *zeros;  // nullptr: 8
   int32_t scale_type, groups, shift;  // groups a row; blocks a group, as a power of two
+  const void *sums;                   // many rows: x's sums over groups, `sums_row` bytes a row of x
+  int64_t sums_row;
 };
+
+// Scale and zero of a weight's row `row` (of all experts') and group.
+__device__ inline float int4_scale(const Int4Args &a, int64_t row, int32_t group) {
+  return load_as_float(a.scales, a.scale_type, row * a.groups + group);
+}
+__device__ inline float int4_zero(const Int4Args &a, int64_t row, int32_t group) {
+  return a.zeros ? (float)(a.zeros[row * a.groups + group] & 31) : 8.0f;
+}
 
 // Eight codes as they are, 0 to 15, in 16 bits, exactly: a byte below 16 is an FP8 (e4m3) number too, 2^-9 times its
 // value, which the conversions multiply by 2^9. Three masks and shifts and four conversions for eight values.
@@ -119,5 +129,11 @@ __device__ inline void read_window(const Int4Args &a, const uint8_t *row, int32_
 // Few rows (int4_rows.hip): x is 16-bit rows of whole 16-byte pieces.
 Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus);
 void launch_int4_rows(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
+
+// Many rows (int4_tile.hip): x is 16-bit rows of whole blocks at 16-byte addresses, with its sums: 16 groups at a time, the
+// first eight bits (and sign) of each, the next eight and the rest as BF16, 32 bytes each; zeros past the last group.
+Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus);
+void launch_int4_tiles(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
+inline int64_t sums_row_bytes(int32_t groups) { return (int64_t)(groups + 15) / 16 * 96; }
 
 }  // namespace mps

@@ -18,6 +18,43 @@ __global__ __launch_bounds__(256) void int4_pack_kernel(const uint16_t *__restri
   }
 }
 
+// The sums of x over groups, in FP32 by a tree, as three BF16 numbers; and x packed, if asked for. A wave takes 512 columns of a row,
+// or a group where that is more: eight a lane.
+template <int XT>
+__global__ __launch_bounds__(256) void int4_sums_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride, int32_t k, int32_t groups,
+                                                        int32_t shift, uint8_t *__restrict__ sums, int64_t sums_row, int32_t width,
+                                                        uint16_t *__restrict__ packed) {
+  const int lane = threadIdx.x & 63;
+  const int32_t span = shift > 4 ? 32 << shift : 512, in_group = shift > 4 ? 64 : 4 << shift;  // columns a wave; lanes a group
+  const int32_t padded = (groups + 15) / 16 * 16, spans = (int32_t)((((int64_t)padded << shift) * 32 + span - 1) / span);
+  const int64_t units = rows * spans;
+  for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (int64_t)gridDim.x * 4) {
+    const int64_t row = unit / spans;
+    const int64_t first = (unit - row * spans) * span;
+    const uint16_t *const from = x + row * stride;
+    float sum = 0;
+    for (int64_t col = first + lane * 8; col < first + span && col - lane * 8 < width; col += 512) {
+      const u32x4 v = load_row8(from, col, k);
+      if (packed && col < width) *reinterpret_cast<u32x4 *>(packed + row * width + col) = v;
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[2 * i] = Elem<XT>::get((uint16_t)v[i]), f[2 * i + 1] = Elem<XT>::get((uint16_t)(v[i] >> 16));
+      sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+    }
+    for (int d = 1; d < in_group; d *= 2) sum += __shfl_xor(sum, d);
+    const int32_t group = (int32_t)(first / 32 >> shift) + lane / in_group;
+    if (lane % in_group == 0 && group < padded) {
+      uint16_t *const to = reinterpret_cast<uint16_t *>(sums + row * sums_row + group / 16 * 96) + group % 16;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint16_t piece = Elem<MPS_TYPE_BF16>::put(sum);
+        to[16 * i] = piece;
+        sum -= Elem<MPS_TYPE_BF16>::get(piece);
+      }
+    }
+  }
+}
+
 int check(const mps_int4_product *p) {
   if (!p) return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product is NULL");
   if (p->x_type != MPS_TYPE_BF16 && p->x_type != MPS_TYPE_F16)
@@ -49,9 +86,10 @@ int check(const mps_int4_product *p) {
 // Which kernel takes a product, and what it needs.
 struct Way {
   Int4Args args;
+  bool tiles;  // int4_tile.hip, else int4_rows.hip: the one predicted to be done earlier
   int choice;
   bool packed;  // x is packed into the workspace first
-  int64_t workspace;
+  int64_t packed_bytes, workspace;  // the packed x, then its sums
 };
 Way way_of(const mps_int4_product *p) {
   Way w = {};
@@ -65,10 +103,14 @@ Way way_of(const mps_int4_product *p) {
   a.scales = p->scales, a.zeros = p->zeros, a.scale_type = p->scale_type;
   a.groups = (int32_t)((p->k + p->group - 1) / p->group);
   while ((int64_t)32 << a.shift < p->group) ++a.shift;
-  const Prediction rows = predict_int4_rows(a, p->x_type, compute_units());
-  w.choice = rows.choice;
-  w.packed = p->k > 0 && !piece_rows(p->x, p->x_stride, p->k);
-  if (w.packed) w.workspace = a.x_rows * packed_width(p->k) * 2;
+  const int32_t cus = compute_units();
+  const Prediction rows = predict_int4_rows(a, p->x_type, cus), tiles = predict_int4_tiles(a, p->x_type, cus);
+  w.tiles = tiles.choice >= 0 && (rows.choice < 0 || tiles.us < rows.us);
+  w.choice = w.tiles ? tiles.choice : rows.choice;
+  w.packed = p->k > 0 && !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
+  if (w.packed) w.packed_bytes = a.x_rows * packed_width(p->k) * 2;
+  if (w.tiles) a.sums_row = sums_row_bytes(a.groups);
+  w.workspace = w.packed_bytes + a.x_rows * a.sums_row;
   return w;
 }
 
@@ -98,14 +140,29 @@ int mps_int4_multiply(const mps_int4_product *p, void *workspace, int64_t worksp
     return fail(MPS_ERR_INVALID_ARGUMENT, "int4 product: %lld bytes of workspace are needed, 16-byte aligned", (long long)way.workspace);
   Int4Args a = way.args;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (way.packed) {
-    const int32_t width = (int32_t)packed_width(p->k);
+  const int32_t width = (int32_t)packed_width(p->k), k = a.k;
+  uint16_t *const packed = way.packed ? static_cast<uint16_t *>(workspace) : nullptr;
+  const uint16_t *const x = static_cast<const uint16_t *>(p->x);
+  if (way.tiles && k > 0) {
+    uint8_t *const sums = static_cast<uint8_t *>(workspace) + way.packed_bytes;
+    const int64_t spans = ((int64_t)((a.groups + 15) / 16 * 16) << a.shift) / (a.shift > 4 ? 1 << a.shift : 16);
+    const dim3 grid(workgroups(((int64_t)a.x_rows * spans + 3) / 4));
+    if (p->x_type == MPS_TYPE_BF16)
+      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_BF16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, a.groups, a.shift, sums,
+                         a.sums_row, width, packed);
+    else
+      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_F16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, a.groups, a.shift, sums,
+                         a.sums_row, width, packed);
+    a.sums = sums;
+  } else if (way.packed) {
     const dim3 grid(workgroups(((int64_t)a.x_rows * (width / 8) + 255) / 256));
-    hipLaunchKernelGGL(int4_pack_kernel, grid, dim3(256), 0, s, static_cast<const uint16_t *>(p->x), (int64_t)a.x_rows, p->x_stride, a.k,
-                       width, static_cast<uint16_t *>(workspace));
-    a.x = workspace, a.x_stride = width, a.k = width;
+    hipLaunchKernelGGL(int4_pack_kernel, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, width, packed);
   }
-  launch_int4_rows(a, p->x_type, way.choice, s);
+  if (way.packed) a.x = workspace, a.x_stride = width, a.k = width;
+  if (way.tiles)
+    launch_int4_tiles(a, p->x_type, way.choice, s);
+  else
+    launch_int4_rows(a, p->x_type, way.choice, s);
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
 }
