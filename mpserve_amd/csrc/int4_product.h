@@ -59,6 +59,13 @@ __device__ inline u32x4 int4_values(uint32_t codes, float zero) {
   return v;
 }
 
+// 16 bytes a lane from memory to LDS, lane after lane from `to` (alike for all lanes) on. By an instruction of its own, since behind the
+// compiler's the next read of LDS waits for all such loads; the kernels wait for theirs by count.
+__device__ inline uint32_t lds_address(const uint8_t *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p; }
+__device__ inline void copy16_apart(const uint8_t *from, uint32_t to) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+
 // Eight ones: x times these is the sum of x.
 template <int XT>
 __device__ inline u32x4 int4_ones() {

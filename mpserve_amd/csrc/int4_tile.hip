@@ -1,11 +1,13 @@
-// Products of many rows: tiles of 32 FT rows of x times 32 WN weight rows, a wave 32 of these and all of x's, with both operands'
-// pieces of k staged in LDS.
+// Products of many rows: tiles of 32 FT WT rows of x times 32 FN WN weight rows, a wave FT x FN fragments of 32 x 32, with
+// both operands' pieces of k staged in LDS.
 //
 // A step covers 64 elements of k: 128 bytes of every row of x, a cache line, and 32 of codes, which are widened in registers,
-// after LDS. Pieces of 16 bytes go from memory to a ring of S stages in LDS without passing through registers; piece p of row r of x
-// lies at place p ^ (r / 2 % 8), of codes at p ^ (r / 8 % 2), so that the sixteen lanes that LDS serves in a cycle
-// meet all banks. A step's fragments are read while the one before is multiplied, quarter by quarter, so that a
-// stage is free again, and the next one has to be there, at one place: the step's barrier.
+// after LDS. A stage is two steps. Pieces of 16 bytes go from memory to a ring of three stages in LDS without passing through
+// registers; piece p of row r of x lies at place p ^ (r / 2 % 8), of codes at p ^ (r / 8 % 2), so that the sixteen lanes that
+// LDS serves in a cycle meet all banks. A step's fragments are read while the one before is multiplied, quarter by quarter.
+// A stage's one barrier stands before its second step, for two things: the next stage has come, and nobody needs the one
+// before any more, whose fragments all have used, so that no wave waits there for reads of its own. (BF16, groups of 128, 4096 x 4096 x
+// 14336: loads and reads in a row behind the barrier 560 us, among the products 517; the zeros' product with its loads a chunk ahead 504.)
 //
 // The matrix cores multiply x by the whole numbers q as they are. Products of columns that share a scale are summed by
 // themselves and added with the scale in FP32. What the zeros take away, sum over groups of s z sum x, is another
@@ -17,17 +19,24 @@
 namespace mps {
 namespace {
 
+// What a piece past the end of a row of x is read from.
+__device__ __attribute__((aligned(16))) const uint32_t kNothing[4] = {0, 0, 0, 0};
+
 enum Chain { kBlock, kStep, kPair };  // columns that certainly share a scale: 32, 64, 128
 
-template <Chain C, int FT, int WN, int S>
+constexpr int kStages = 3;
+
+template <Chain C, int FT, int FN, int WT, int WN>
 struct Shape {
-  static constexpr int kBT = 32 * FT, kBN = 32 * WN, kThreads = 64 * WN;
-  static constexpr int kXLoads = kBT * 8 / kThreads, kLoads = kXLoads + 1;  // loads a work-item and step
-  static constexpr int kXBytes = kBT * 128, kStage = kXBytes + kBN * 32;
-  static constexpr int kEntries = C == kBlock ? 16 : 8;  // scales of a row and period of 16 blocks
+  static constexpr int kBT = 32 * FT * WT, kBN = 32 * FN * WN, kWaves = WT * WN, kThreads = 64 * kWaves;
+  static constexpr int kXLoads = kBT * 8 / kThreads, kWLoads = (kBN * 2 + kThreads - 1) / kThreads;  // a work-item and step
+  static constexpr int kLoads = 2 * (kXLoads + kWLoads);                                             // and stage
+  static constexpr int kWLanes = kBN * 2 / kWaves < 64 ? kBN * 2 / kWaves : 64;                      // that load codes
+  static constexpr int kXBytes = kBT * 128, kStep = kXBytes + kBN * 32, kStage = 2 * kStep;
+  static constexpr int kEntries = 8, kPeriod = C == kBlock ? 2 : 4;  // scales of a row in a period; stages a period
   static constexpr int kSBytes = kBN * kEntries * 2;
-  static constexpr int kPitch = 36;  // floats of a row of sums, turned round
-  static constexpr int kStaged = S * kStage + 2 * kSBytes, kTurned = WN * 32 * kPitch * 4;
+  static constexpr int kPitch = 32 * FN + 4;  // floats of a row of sums, turned round
+  static constexpr int kStaged = kStages * kStage + 2 * kSBytes, kTurned = kWaves * 32 * kPitch * 4;
   static constexpr int kLds = kStaged > kTurned ? kStaged : kTurned;
   static_assert(kBT * 8 % kThreads == 0 && kLds <= 160 * 1024 && kBN <= kThreads, "");
 };
@@ -40,12 +49,13 @@ __device__ inline f32x16 mfma32(u32x4 x, u32x4 w, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, w), c, 0, 0, 0);
 }
 
-template <int XT, Chain C, int FT, int WN, int S>
-__global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT > 2 ? 2 : 4))) void int4_tile_kernel(Int4Args a, int32_t tiles_t, int32_t tiles_n) {
-  typedef Shape<C, FT, WN, S> H;
+template <int XT, Chain C, int FT, int FN, int WT, int WN>
+__global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void int4_tile_kernel(Int4Args a, int32_t tiles_t, int32_t tiles_n) {
+  typedef Shape<C, FT, FN, WT, WN> H;
   __shared__ __attribute__((aligned(16))) uint8_t lds[H::kLds];
-  uint8_t *const ss = lds + S * H::kStage;
+  uint8_t *const ss = lds + kStages * H::kStage;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, g = lane >> 5;
+  const int wt = wave / WN, wn = wave % WN;
 
   if (a.offsets) tiles_t = count_tiles(a.offsets, a.experts, a.rows, H::kBT);  // the host knows a bound only
   // Workgroups go to the 8 XCDs in turn. Each XCD takes a stretch of the tiles, in which
@@ -61,7 +71,7 @@ __global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT >
   if (a.offsets) tile = find_tile(a.offsets, a.experts, a.rows, H::kBT, tile_t);
   if (tile.expert < 0) return;
   const bool none = tile.expert >= max(a.experts, 1);  // rows of no expert
-  const int32_t blocks = none ? 0 : a.row_blocks, steps = (blocks + 1) / 2;
+  const int32_t blocks = none ? 0 : a.row_blocks, pairs = (blocks + 3) / 4;  // of steps
 
   // Where this lane's pieces come from. Rows past the tile's end or the weight's are the last ones (what they
   // give is not stored), pieces past a row's end its last one.
@@ -69,25 +79,42 @@ __global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT >
     const int32_t from = min(tile.first + i, tile.end - 1);
     return a.gather ? min((uint32_t)a.order[from] / (uint32_t)a.top, (uint32_t)a.x_rows - 1) : from;
   };
-  const int xrow = tid / 8, wrow = tid / 2;
-  const int32_t x_piece = (tid % 8) ^ (xrow >> 1 & 7), w_piece = (tid % 2) ^ (wrow >> 3 & 1), x_pieces = blocks * 4;
+  const int w_first_piece = wave * H::kWLanes + lane;  // of the first load's
+  const int xrow = tid / 8, wrow = w_first_piece / 2;
+  const uint32_t x_piece = ((tid % 8) ^ (xrow >> 1 & 7)) * 16, w_piece = ((w_first_piece % 2) ^ (wrow >> 3 & 1)) * 16;
+  const uint32_t x_end = blocks * 64, w_last = blocks * 16 - 16;
   const uint8_t *x_from[H::kXLoads];
 #pragma unroll
-  for (int i = 0; i < H::kXLoads; ++i) x_from[i] = static_cast<const uint8_t *>(a.x) + row_of(xrow + i * (H::kThreads / 8)) * a.x_stride * 2;
+  for (int i = 0; i < H::kXLoads; ++i)
+    x_from[i] = static_cast<const uint8_t *>(a.x) + row_of(xrow + i * (H::kThreads / 8)) * a.x_stride * 2 + x_piece;
   const int64_t w_first = (int64_t)(none ? 0 : tile.expert) * a.n + n0;
   const int32_t last_col = a.n - 1 - n0;
-  const uint8_t *const w_from = a.w + (w_first + min(wrow, last_col)) * a.row_blocks * 16;
-  auto fetch = [&](int32_t step, uint32_t slot) {
-    uint8_t *const to = lds + slot * H::kStage;
-    const uint32_t x_at = (uint32_t)min(step * 8 + x_piece, x_pieces - 1) * 16;
+  const uint8_t *w_from[H::kWLoads];
 #pragma unroll
-    for (int i = 0; i < H::kXLoads; ++i) copy16(x_from[i] + x_at, to + wave * 1024 + i * H::kThreads * 16);
-    copy16(w_from + (uint32_t)min(step * 2 + w_piece, blocks - 1) * 16, to + H::kXBytes + wave * 1024);
+  for (int i = 0; i < H::kWLoads; ++i) w_from[i] = a.w + (w_first + min(wrow + i * (H::kThreads / 2), last_col)) * a.row_blocks * 16;
+  // Load l of a stage, to `to` in LDS. The stages at a row's end may be parts of one or none at all: x's pieces past
+  // its end are zeros, the codes' what they are.
+  const uint32_t lds_at = lds_address(lds) + wave * 1024, w_lds_at = lds_address(lds) + H::kXBytes + wave * H::kWLanes * 16;
+  auto fetch = [&](int32_t pair, uint32_t to, int l, auto whole) {
+    const int h = l / (H::kLoads / 2), i = l % (H::kLoads / 2);
+    if (i < H::kXLoads) {
+      const uint32_t at = pair * 256 + h * 128;
+      const uint8_t *from = x_from[i] + at;
+      if (!decltype(whole)::value) from = at + x_piece < x_end ? from : reinterpret_cast<const uint8_t *>(kNothing);
+      copy16_apart(from, lds_at + to + h * H::kStep + i * H::kThreads * 16);
+    } else if (H::kWLanes == 64 || lane < H::kWLanes) {
+      const uint32_t at = pair * 64 + h * 32 + w_piece;
+      copy16_apart(w_from[i - H::kXLoads] + (decltype(whole)::value ? at : min(at, w_last)), w_lds_at + to + h * H::kStep + (i - H::kXLoads) * H::kThreads * 16);
+    }
+  };
+  auto fetch_all = [&](int32_t pair, uint32_t to) {
+#pragma unroll
+    for (int l = 0; l < H::kLoads; ++l) fetch(pair, to, l, std::false_type{});
   };
 
   // Scales come a period ahead, through registers: a row's kEntries from its first group in the period on, near the
   // row's end from earlier on, alike for all rows.
-  auto scales_start = [&](int32_t period) -> int32_t { return max(0, min((16 * period) >> a.shift, a.groups - H::kEntries)); };
+  auto scales_start = [&](int32_t period) -> int32_t { return max(0, min((4 * H::kPeriod * period) >> a.shift, a.groups - H::kEntries)); };
   // A row that has fewer in all has them in both buffers from the start.
   uint32_t scales[H::kEntries / 2] = {};
   const bool turns = a.groups >= H::kEntries, has_scales = tid < H::kBN;
@@ -97,59 +124,47 @@ __global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT >
   };
   auto put_scales = [&](int32_t period) {
     u32x4 *const to = reinterpret_cast<u32x4 *>(ss + (period & 1) * H::kSBytes + tid * H::kEntries * 2);
-    if (has_scales) {
-#pragma unroll
-      for (int i = 0; i < H::kEntries / 8; ++i) to[i] = u32x4{scales[4 * i], scales[4 * i + 1], scales[4 * i + 2], scales[4 * i + 3]};
-    }
+    if (has_scales) *to = u32x4{scales[0], scales[1], scales[2], scales[3]};
   };
-  auto scale_of = [&](int32_t block) -> float {
-    const int32_t period = block / 16, entry = (block >> a.shift) - scales_start(period);
-    return scale_value(*reinterpret_cast<const uint16_t *>(ss + (period & 1) * H::kSBytes + (wave * 32 + r) * H::kEntries * 2 + entry * 2), a.scale_type);
+  auto scale_of = [&](int n, int32_t block) -> float {
+    const int32_t period = block / (4 * H::kPeriod), entry = (block >> a.shift) - scales_start(period);
+    return scale_value(*reinterpret_cast<const uint16_t *>(ss + (period & 1) * H::kSBytes + ((wn * FN + n) * 32 + r) * H::kEntries * 2 + entry * 2),
+                       a.scale_type);
   };
 
   // Lanes 0-31 and 32-63 take a half each of a step's 64 elements: of either block where blocks have scales of their
   // own, else a block. Quarter q is eight elements of each half.
-  f32x16 acc[FT] = {}, part[FT] = {};
+  f32x16 acc[FT][FN] = {}, part[FT][FN] = {};
   u32x4 fx[4][FT];
-  uint32_t fw[4], fw_next[4];
-  const int x_lane = r * 128, w_lane = (wave * 32 + r) * 32;
+  uint32_t fw[2][FN][4];  // of even and odd steps
+  u32x4 w0[FN], w1[FN];   // widened: of the even and the odd quarter
+  const int x_lane = (wt * FT * 32 + r) * 128, w_lane = (wn * FN * 32 + r) * 32;
   auto x_place = [&](int q) -> int { return ((C == kBlock ? 4 * (q >> 1) + 2 * g + (q & 1) : 4 * g + q) ^ (r >> 1 & 7)) * 16 + x_lane; };
-  auto read_x = [&](int q, uint32_t slot) {
-    const uint8_t *const from = lds + slot * H::kStage + x_place(q);
+  auto read_x = [&](int q, int t, uint32_t at) { fx[q][t] = *reinterpret_cast<const u32x4 *>(lds + at + x_place(q) + t * 4096); };
+  auto read_w = [&](uint32_t (&to)[FN][4], uint32_t at) {
+    const uint8_t *const from = lds + at + H::kXBytes + w_lane;
 #pragma unroll
-    for (int t = 0; t < FT; ++t) fx[q][t] = *reinterpret_cast<const u32x4 *>(from + t * 4096);
-  };
-  auto read_w = [&](uint32_t (&to)[4], uint32_t slot) {
-    const uint8_t *const from = lds + slot * H::kStage + H::kXBytes + w_lane;
-    if constexpr (C == kBlock) {
+    for (int n = 0; n < FN; ++n) {
+      if constexpr (C == kBlock) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t v = *reinterpret_cast<const uint64_t *>(from + (h ^ (r >> 3 & 1)) * 16 + g * 8);
-        to[2 * h] = (uint32_t)v, to[2 * h + 1] = (uint32_t)(v >> 32);
+        for (int h = 0; h < 2; ++h) {
+          const uint64_t v = *reinterpret_cast<const uint64_t *>(from + n * 1024 + (h ^ (r >> 3 & 1)) * 16 + g * 8);
+          to[n][2 * h] = (uint32_t)v, to[n][2 * h + 1] = (uint32_t)(v >> 32);
+        }
+      } else {
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(from + n * 1024 + (g ^ (r >> 3 & 1)) * 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) to[n][q] = v[q];
       }
-    } else {
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(from + (g ^ (r >> 3 & 1)) * 16);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) to[q] = v[q];
     }
   };
-  // A last step of one block: the other's pieces are taken as zeros. So are those of a step past the last.
-  auto cut = [&](int32_t step) {
-    if (2 * step + 1 < blocks) return;
+  float pending[FN] = {};  // the scales of the products that `part` holds
+  int64_t cols[FN];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const bool past = (C == kBlock ? q >= 2 : g == 1) || (C == kPair && 2 * step >= blocks);
+  for (int n = 0; n < FN; ++n) cols[n] = w_first + min((wn * FN + n) * 32 + r, last_col);
+  if (pairs > 0) {
 #pragma unroll
-      for (int t = 0; t < FT; ++t)
-        if (past) fx[q][t] = u32x4{0, 0, 0, 0};
-    }
-  };
-
-  float pending = 0;  // the scale of the products that `part` holds
-  if (steps > 0) {
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-      if (i < steps) fetch(i, i);
+    for (int i = 0; i < kStages - 1; ++i) fetch_all(i, i * H::kStage);
     if (turns) {
       get_scales(0);
     } else {
@@ -160,132 +175,217 @@ __global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT >
       for (int i = 0; i < H::kEntries / 2; ++i) scales[i] = few[2 * i] | (uint32_t)few[2 * i + 1] << 16;
     }
     // What the zeros take away: 16 groups at a time.
-    const int64_t col = w_first + min(wave * 32 + r, last_col);
     const uint8_t *sums[FT];
 #pragma unroll
-    for (int t = 0; t < FT; ++t) sums[t] = static_cast<const uint8_t *>(a.sums) + (int64_t)row_of(t * 32 + r) * a.sums_row + g * 16;
+    for (int t = 0; t < FT; ++t) sums[t] = static_cast<const uint8_t *>(a.sums) + (int64_t)row_of((wt * FT + t) * 32 + r) * a.sums_row + g * 16;
+    struct Chunk {
+      uint32_t s[FN][4], z[FN][2];
+      u32x4 x[FT][3];
+    };
+    auto get_chunk = [&](int32_t c, Chunk &k) {
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        const int64_t from = cols[n] * a.groups;
+        const uint16_t *const s = static_cast<const uint16_t *>(a.scales) + from;
+        k.z[n][0] = k.z[n][1] = 0x08080808u;
+        if (c + 16 <= a.groups) {
+          __builtin_memcpy(k.s[n], s + c + 8 * g, 16);
+          if (a.zeros) __builtin_memcpy(k.z[n], a.zeros + from + c + 8 * g, 8);
+        } else {  // without branches among the loads, so that they are in flight together
+          uint32_t e[8], f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = s[min(c + 8 * g + i, a.groups - 1)];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c + 8 * g + i >= a.groups) e[i] = 0;  // a scale of 0.0
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k.s[n][i] = e[2 * i] | e[2 * i + 1] << 16;
+          if (a.zeros) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = a.zeros[from + min(c + 8 * g + i, a.groups - 1)];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) k.z[n][i] = f[4 * i] | f[4 * i + 1] << 8 | f[4 * i + 2] << 16 | f[4 * i + 3] << 24;
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < FT; ++t)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) k.x[t][i] = *reinterpret_cast<const u32x4 *>(sums[t] + c / 16 * 96 + i * 32);
+    };
+    Chunk now, soon;
+    get_chunk(0, now);
     for (int32_t c = 0; c < a.groups; c += 16) {
-      uint32_t sb[8], zb[8];  // loads without branches, so that they are in flight together
+      if (c + 16 < a.groups) get_chunk(c + 16, soon);
+      u32x4 hi[FN], lo[FN];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sb[i] = static_cast<const uint16_t *>(a.scales)[col * a.groups + min(c + 8 * g + i, a.groups - 1)], zb[i] = 8;
-      if (a.zeros) {
+      for (int n = 0; n < FN; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) zb[i] = a.zeros[col * a.groups + min(c + 8 * g + i, a.groups - 1)] & 31;
-      }
-      u32x4 hi, lo;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t z = now.z[n][i / 2] >> (16 * (i % 2)) & 0x1f1f;
+          const float f0 = -scale_value(now.s[n][i] & 0xffff, a.scale_type) * (float)(z & 255), f1 = -scale_value(now.s[n][i] >> 16, a.scale_type) * (float)(z >> 8);
+          hi[n][i] = pack2(f0, f1, MPS_TYPE_BF16);
+          lo[n][i] = pack2(f0 - __uint_as_float(hi[n][i] << 16), f1 - __uint_as_float(hi[n][i] & 0xffff0000u), MPS_TYPE_BF16);
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float f[2];
+      for (int t = 0; t < FT; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          f[j] = c + 8 * g + 2 * i + j < a.groups ? -scale_value(sb[2 * i + j], a.scale_type) * (float)zb[2 * i + j] : 0.0f;
-        hi[i] = pack2(f[0], f[1], MPS_TYPE_BF16);
-        lo[i] = pack2(f[0] - __uint_as_float(hi[i] << 16), f[1] - __uint_as_float(hi[i] & 0xffff0000u), MPS_TYPE_BF16);
-      }
-#pragma unroll
-      for (int t = 0; t < FT; ++t) {
-        const uint8_t *const from = sums[t] + c / 16 * 96;
-        const u32x4 x0 = *reinterpret_cast<const u32x4 *>(from), x1 = *reinterpret_cast<const u32x4 *>(from + 32), x2 = *reinterpret_cast<const u32x4 *>(from + 64);
-        acc[t] = mfma32<MPS_TYPE_BF16>(x2, hi, acc[t]);
-        acc[t] = mfma32<MPS_TYPE_BF16>(x1, lo, acc[t]);
-        acc[t] = mfma32<MPS_TYPE_BF16>(x1, hi, acc[t]);
-        acc[t] = mfma32<MPS_TYPE_BF16>(x0, lo, acc[t]);
-        acc[t] = mfma32<MPS_TYPE_BF16>(x0, hi, acc[t]);
-      }
+        for (int n = 0; n < FN; ++n) {
+          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][2], hi[n], acc[t][n]);
+          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][1], lo[n], acc[t][n]);
+          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][1], hi[n], acc[t][n]);
+          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][0], lo[n], acc[t][n]);
+          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][0], hi[n], acc[t][n]);
+        }
+      now = soon;
     }
     put_scales(0);
     if (!turns) put_scales(1);
+    if (turns && H::kPeriod < pairs) get_scales(1);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int q = 0; q < 4; ++q) read_x(q, 0);
-    read_w(fw, 0);
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int t = 0; t < FT; ++t) read_x(q, t, 0);
+    read_w(fw[0], 0);
+#pragma unroll
+    for (int n = 0; n < FN; ++n) w0[n] = int4_codes<XT>(fw[0][n][0]);
   }
-  uint32_t slot = 0;  // of this step
-  auto body = [&](int32_t step, auto odd) {
-    const uint32_t next = slot + 1 == S ? 0 : slot + 1;
-    if (step + S <= steps)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * H::kLoads) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + S < steps) fetch(step + S, slot);
-    if (turns && step % 8 == 0 && step + 8 < steps) get_scales(step / 8 + 1);
-    if (turns && step % 8 == 6 && step + 2 < steps) put_scales(step / 8 + 1);
-    cut(step);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const u32x4 w = int4_codes<XT>(fw[q]);
-      // Where another scale begins, what has been summed with the last one is added, and the sums begin again.
-      if (C == kBlock ? q % 2 == 0 : q == 0 && !decltype(odd)::value) {
-        const float scale = scale_of(C == kBlock ? min(2 * step + (q >> 1), blocks - 1) : 2 * step);
-#pragma unroll
-        for (int t = 0; t < FT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][i] = __builtin_fmaf(pending, part[t][i], acc[t][i]);
-          asm volatile("" : "+v"(acc[t]));  // the sums stay where they are
-          __builtin_amdgcn_sched_barrier(0);
-          part[t] = mfma32<XT>(fx[q][t], w, f32x16{});
-          asm volatile("" : "+v"(part[t]));
-        }
-        pending = scale;
-      } else {
-#pragma unroll
-        for (int t = 0; t < FT; ++t) {
-          part[t] = mfma32<XT>(fx[q][t], w, part[t]);
-          asm volatile("" : "+v"(part[t]));
-        }
+  // Where this stage, the next and the one after it lie, and the stage at which scales are turned.
+  uint32_t here = 0, then = H::kStage, after = 2 * H::kStage;
+  int32_t turn = turns && H::kPeriod < pairs ? H::kPeriod - 2 : INT32_MAX;
+  // A step. The fragments' products come in an order in which, where another scale begins, the 16 multiply-adds a lane that
+  // add what has been summed with the last one stand beside two products each. Between two products there is room for
+  // a read of the next step's fragments, a load of the stage after the next, or the widening of a quarter's codes.
+  auto body = [&](int32_t pair, auto odd, auto whole) {
+    constexpr int kOdd = decltype(odd)::value, kM = FT * FN;
+    if constexpr (kOdd == 1) {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      if (__builtin_expect(pair == turn, 0)) {
+        const int32_t period = pair / H::kPeriod + 1;  // the next one
+        put_scales(period);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const bool more = (period + 1) * H::kPeriod < pairs;
+        if (more) get_scales(period + 1);
+        turn = more ? turn + H::kPeriod : INT32_MAX;
       }
-      read_x(q, next);  // past the last step: of a stage that nobody writes
-      if (q == 1) read_w(fw_next, next);
-      __builtin_amdgcn_sched_barrier(0);
     }
+    const uint32_t next = kOdd ? then : here + H::kStep;
+    int load = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) fw[q] = fw_next[q];
-    slot = next;
+    for (int h = 0; h < 2; ++h) {
+      const bool fresh = C == kBlock || (h == 0 && (C == kStep || kOdd == 0));
+      float scale[FN];
+      if (fresh) {
+#pragma unroll
+        for (int n = 0; n < FN; ++n) scale[n] = scale_of(n, min(4 * pair + 2 * kOdd + (C == kBlock ? h : 0), blocks - 1));
+      }
+#pragma unroll
+      for (int s = 0; s < 2 * kM; ++s) {
+        // Fresh: 0, 1, 0', 2, 1', 3, 2' ..; else 0, 1, 2 .. 0', 1', 2' ..
+        const int second = fresh ? (s == 2 * kM - 1 || (s > 0 && s % 2 == 0)) : s >= kM;
+        const int i = fresh ? (s == 0 ? 0 : s == 2 * kM - 1 ? kM - 1 : second ? s / 2 - 1 : (s + 1) / 2) : s % kM;
+        const int t = i % FT, n = i / FT, q = 2 * h + second;
+        if (fresh && !second) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[t][n][j] = __builtin_fmaf(pending[n], part[t][n][j], acc[t][n][j]);
+          asm volatile("" : "+v"(acc[t][n]));  // the sums stay where they are
+          __builtin_amdgcn_sched_barrier(0);
+          part[t][n] = mfma32<XT>(fx[q][t], w0[n], f32x16{});
+        } else {
+          part[t][n] = mfma32<XT>(fx[q][t], second ? w1[n] : w0[n], part[t][n]);
+        }
+        asm volatile("" : "+v"(part[t][n]));
+        if (n == FN - 1) read_x(q, t, next);
+        if (s == 0) {
+#pragma unroll
+          for (int m = 0; m < FN; ++m) w1[m] = int4_codes<XT>(fw[kOdd][m][2 * h + 1]);
+        }
+        if (h == 0 && s == 1) read_w(fw[kOdd ^ 1], next);
+        if (!second && i == kM - 1) {  // the last of the even quarter
+#pragma unroll
+          for (int m = 0; m < FN; ++m) w0[m] = int4_codes<XT>(h == 0 ? fw[kOdd][m][2] : fw[kOdd ^ 1][m][0]);
+        }
+        if (kOdd == 1 && load < H::kLoads) fetch(pair + 2, after, load++, whole);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (fresh) {
+#pragma unroll
+        for (int n = 0; n < FN; ++n) pending[n] = scale[n];
+      }
+    }
+    if constexpr (kOdd == 1) {
+      static_assert(H::kLoads <= 4 * kM, "");
+      const uint32_t last = here;
+      here = then, then = after, after = last;
+    }
   };
+  int32_t pair = 0;
 #pragma unroll 1
-  for (int32_t step = 0; step < steps; step += C == kPair ? 2 : 1) {
-    body(step, std::false_type{});
-    if constexpr (C == kPair) body(step + 1, std::true_type{});  // where there is none, of zeros
+  for (; 4 * pair + 12 <= blocks; ++pair) {  // the stage after the next is a whole one
+    body(pair, std::integral_constant<int, 0>{}, std::true_type{});
+    body(pair, std::integral_constant<int, 1>{}, std::true_type{});
   }
+#pragma unroll 1
+  for (; pair < pairs; ++pair) {
+    body(pair, std::integral_constant<int, 0>{}, std::false_type{});
+    body(pair, std::integral_constant<int, 1>{}, std::false_type{});
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the last stage
   bool finite = true;
 #pragma unroll
   for (int t = 0; t < FT; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      acc[t][i] = __builtin_fmaf(pending, part[t][i], acc[t][i]);
-      finite &= __builtin_fabsf(acc[t][i]) < __builtin_inff();
-    }
-  if (__builtin_expect(__syncthreads_or(!finite), 0)) {  // all again, a step at a time, with scales and zeros from memory
+    for (int n = 0; n < FN; ++n)
 #pragma unroll
-    for (int t = 0; t < FT; ++t) acc[t] = f32x16{};
-    const int64_t col = w_first + min(wave * 32 + r, last_col);
+      for (int i = 0; i < 16; ++i) {
+        acc[t][n][i] = __builtin_fmaf(pending[n], part[t][n][i], acc[t][n][i]);
+        finite &= __builtin_fabsf(acc[t][n][i]) < __builtin_inff();
+      }
+  uint32_t *const flags = reinterpret_cast<uint32_t *>(ss);
+  uint32_t again = 0;
+  __syncthreads();
+  flags[wave] = __any(!finite);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < H::kWaves; ++w) again |= flags[w];
+  if (__builtin_expect(__builtin_amdgcn_readfirstlane(again), 0)) {  // all again, a step at a time, with scales and zeros from memory
+#pragma unroll
+    for (int t = 0; t < FT; ++t)
+#pragma unroll
+      for (int n = 0; n < FN; ++n) acc[t][n] = f32x16{};
 #pragma unroll 1
-    for (int32_t step = 0; step < steps; ++step) {
+    for (int32_t step = 0; 2 * step < blocks; ++step) {
+      const uint32_t at_step = step % 2 * H::kStep;
       __syncthreads();
-      fetch(step, 0);
+      fetch_all(step / 2, 0);
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-      for (int q = 0; q < 4; ++q) read_x(q, 0);
-      read_w(fw, 0);
-      cut(step);
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int t = 0; t < FT; ++t) read_x(q, t, at_step);
+      read_w(fw[0], at_step);
 #pragma unroll
       for (int h = 0; h < (C == kBlock ? 2 : 1); ++h) {
         if (2 * step + h >= blocks) break;
         const int32_t at = (2 * step + h) >> a.shift;
-        const float s = int4_scale(a, col, at), zero = int4_zero(a, col, at);
 #pragma unroll
-        for (int t = 0; t < FT; ++t) part[t] = f32x16{};
+        for (int n = 0; n < FN; ++n) {
+          const float s = int4_scale(a, cols[n], at), zero = int4_zero(a, cols[n], at);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (C == kBlock && q / 2 != h) continue;
-          const u32x4 w = int4_values<XT>(fw[q], zero);
+          for (int t = 0; t < FT; ++t) part[t][n] = f32x16{};
 #pragma unroll
-          for (int t = 0; t < FT; ++t) part[t] = mfma32<XT>(fx[q][t], w, part[t]);
+          for (int q = 0; q < 4; ++q) {
+            if (C == kBlock && q / 2 != h) continue;
+            const u32x4 w = int4_values<XT>(fw[0][n][q], zero);
+#pragma unroll
+            for (int t = 0; t < FT; ++t) part[t][n] = mfma32<XT>(fx[q][t], w, part[t][n]);
+          }
+#pragma unroll
+          for (int t = 0; t < FT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][n][i] = __builtin_fmaf(s, part[t][n][i], acc[t][n][i]);
         }
-#pragma unroll
-        for (int t = 0; t < FT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][i] = __builtin_fmaf(s, part[t][i], acc[t][i]);
       }
     }
     __syncthreads();
@@ -293,52 +393,59 @@ __global__ __launch_bounds__(64 * WN) __attribute__((amdgpu_waves_per_eu(2, FT >
 
   // A lane's 16 sums are rows 8 i + 4 g .. + 3 of column r. The wave turns 32 rows at a time round through its own part
   // of LDS, so that a store has neighbouring columns.
-  constexpr int kPitch = H::kPitch;
+  constexpr int kPitch = H::kPitch, kLanes = 4 * FN, kPasses = 32 * kLanes / 64;
   float *const mine = reinterpret_cast<float *>(lds) + wave * 32 * kPitch;
-  const int32_t col = n0 + wave * 32 + lane % 4 * 8;
+  const int32_t col = n0 + wn * FN * 32 + lane % kLanes * 8;
   f32x4 bias[2] = {};
   if (a.bias && !none) bias[0] = load_bias4(a, tile.expert, col), bias[1] = load_bias4(a, tile.expert, col + 4);
 #pragma unroll
   for (int t = 0; t < FT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int n = 0; n < FN; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mine[(8 * i + 4 * g + j) * kPitch + r] = acc[t][4 * i + j];
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[(8 * i + 4 * g + j) * kPitch + n * 32 + r] = acc[t][n][4 * i + j];
     __builtin_amdgcn_wave_barrier();
-    f32x4 v[2][2];
+    f32x4 v[kPasses][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kPasses; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) v[i][h] = *reinterpret_cast<const f32x4 *>(mine + (i * 16 + lane / 4) * kPitch + lane % 4 * 8 + 4 * h) + bias[h];
+      for (int h = 0; h < 2; ++h)
+        v[i][h] = *reinterpret_cast<const f32x4 *>(mine + (i * (64 / kLanes) + lane / kLanes) * kPitch + lane % kLanes * 8 + 4 * h) + bias[h];
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int32_t row = tile.first + t * 32 + i * 16 + lane / 4;
+    for (int i = 0; i < kPasses; ++i) {
+      const int32_t row = tile.first + (wt * FT + t) * 32 + i * (64 / kLanes) + lane / kLanes;
       if (row < tile.end && col < a.n) store8(a, row, col, v[i][0], v[i][1]);
     }
   }
 }
 
-template <int XT, Chain C, int FT, int WN, int S>
+template <int XT, Chain C, int FT, int FN, int WT, int WN>
 void launch(const Int4Args &a, hipStream_t stream) {
-  typedef Shape<C, FT, WN, S> H;
+  typedef Shape<C, FT, FN, WT, WN> H;
   const int64_t tt = product_tiles(a, H::kBT), tn = (a.n + H::kBN - 1) / H::kBN;
   const int64_t grid = (tt * tn + 7) / 8 * 8;
-  hipLaunchKernelGGL((int4_tile_kernel<XT, C, FT, WN, S>), dim3((unsigned)grid), dim3(WN * 64), 0, stream, a, (int32_t)tt, (int32_t)tn);
+  hipLaunchKernelGGL((int4_tile_kernel<XT, C, FT, FN, WT, WN>), dim3((unsigned)grid), dim3(H::kThreads), 0, stream, a, (int32_t)tt, (int32_t)tn);
 }
 
+// The tiles, in microseconds: `start` is what a tile takes at any k, `few` and `full` what k = 4096 adds to a tile that has a
+// CU to itself, on a card with few of them and a full one, and `many` to each of several. Groups of 64 and of 32 cost more.
 struct Choice {
   int32_t bt, bn;
-  float start, one, many;
+  float start, few, full, many, step, block;
 };
-constexpr Choice kChoices[] = {{128, 256, 4.6f, 51.0f, 53.0f}, {128, 128, 2.6f, 35.0f, 30.0f}, {64, 128, 1.8f, 26.0f, 18.5f}};
+constexpr Choice kChoices[] = {{128, 256, 9.0f, 42.0f, 58.0f, 63.0f, 1.15f, 1.75f}, {64, 256, 7.0f, 25.0f, 41.0f, 34.4f, 1.15f, 1.5f},
+                               {64, 128, 6.0f, 18.0f, 30.0f, 15.8f, 1.15f, 1.45f}, {32, 128, 5.0f, 16.0f, 18.5f, 8.5f, 1.15f, 1.5f}};
 
 template <int XT, Chain C>
 void launch_chain(const Int4Args &a, int choice, hipStream_t stream) {
   switch (choice) {
-    case 0: return launch<XT, C, 4, 8, 3>(a, stream);
-    case 1: return launch<XT, C, 4, 4, 3>(a, stream);
-    default: return launch<XT, C, 2, 4, 3>(a, stream);
+    case 0: return launch<XT, C, 4, 1, 1, 8>(a, stream);
+    case 1: return launch<XT, C, 2, 1, 1, 8>(a, stream);
+    case 2: return launch<XT, C, 2, 1, 1, 4>(a, stream);
+    default: return launch<XT, C, 1, 1, 1, 4>(a, stream);
   }
 }
 template <int XT>
@@ -359,9 +466,16 @@ Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus) {
   for (const Choice &c : kChoices) {
     const int at = i++;
     if (((double)product_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) + 8) * 512 > kMostWorkItems) continue;
-    const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) / cus, k = a.row_blocks / 128.0;
-    const double each = __builtin_ceil(tiles - 0.01);
-    const double us = each <= 1 ? c.start + c.one * k : each * (c.start + c.many * k);
+    const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) / cus;
+    const double k = a.row_blocks / 128.0 * (a.shift == 0 ? c.block : a.shift == 1 ? c.step : 1.0f);
+    // The count of experts' tiles is a guess: the mean over a tenth less and more, lest another round of a few tiles comes
+    // unawares. Experts' weights are no other tile's, and come later.
+    const double start = c.start + (a.offsets ? 3.5 : 0), spread = a.offsets ? 0.1 : 0;
+    double us = 0;
+    for (int j = -1; j <= 1; ++j) {
+      const double n = tiles * (1 + spread * j), each = __builtin_ceil(n - 0.01);
+      us += (each <= 1 ? start + (c.few + (c.full - c.few) * n) * k : each * (start + c.many * k)) / 3;
+    }
     if (best.choice < 0 || us < best.us) best = {at, us};
   }
   return best;
