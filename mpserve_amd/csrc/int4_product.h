@@ -97,26 +97,26 @@ template <bool kFew>
 __device__ inline int32_t window_start(const Int4Args &a, int32_t period) {
   return max(0, min((16 * period) >> a.shift, a.groups - Window<kFew>::kEntries));
 }
+// A row that has fewer in all has them in its window from the start (load_all). The loads have no branches among them, behind which the
+// compiler would wait for all that are under way. Without zeros, others' bytes stand in for them.
+__device__ inline const uint8_t *zeros_or_any(const Int4Args &a) { return a.zeros ? a.zeros : static_cast<const uint8_t *>(a.scales); }
 template <bool kFew>
 __device__ inline void load_window(const Int4Args &a, int64_t row, int32_t start, Window<kFew> &w) {
+  __builtin_memcpy(w.scales, static_cast<const uint16_t *>(a.scales) + row * a.groups + start, sizeof(w.scales));
+  __builtin_memcpy(w.zeros, zeros_or_any(a) + row * a.groups + start, sizeof(w.zeros));
+}
+template <bool kFew>
+__device__ inline void load_all(const Int4Args &a, int64_t row, Window<kFew> &w) {
   constexpr int kEntries = Window<kFew>::kEntries;
-  const uint16_t *const s = static_cast<const uint16_t *>(a.scales) + row * a.groups + start;
-  const uint8_t *const z = a.zeros + row * a.groups + start;
-  if (a.groups >= kEntries) {
-    __builtin_memcpy(w.scales, s, sizeof(w.scales));
-    if (a.zeros) __builtin_memcpy(w.zeros, z, sizeof(w.zeros));
-  } else {
+  const uint16_t *const s = static_cast<const uint16_t *>(a.scales) + row * a.groups;
+  const uint8_t *const z = zeros_or_any(a) + row * a.groups;
+  uint32_t e[kEntries], f[kEntries];
 #pragma unroll
-    for (int i = 0; i < kEntries / 2; ++i) w.scales[i] = 0;
+  for (int i = 0; i < kEntries; ++i) e[i] = s[min(i, a.groups - 1)], f[i] = z[min(i, a.groups - 1)];
 #pragma unroll
-    for (int i = 0; i < kEntries / 4; ++i) w.zeros[i] = 0;
+  for (int i = 0; i < kEntries / 2; ++i) w.scales[i] = e[2 * i] | e[2 * i + 1] << 16;
 #pragma unroll
-    for (int i = 0; i < kEntries; ++i)
-      if (i < a.groups) {
-        w.scales[i / 2] |= (uint32_t)s[i] << (16 * (i % 2));
-        if (a.zeros) w.zeros[i / 4] |= (uint32_t)z[i] << (8 * (i % 4));
-      }
-  }
+  for (int i = 0; i < kEntries / 4; ++i) w.zeros[i] = f[4 * i] | f[4 * i + 1] << 8 | f[4 * i + 2] << 16 | f[4 * i + 3] << 24;
 }
 template <bool kFew>
 __device__ inline void put_window(const Int4Args &a, const Window<kFew> &w, uint8_t *lds) {

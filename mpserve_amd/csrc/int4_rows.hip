@@ -7,7 +7,7 @@
 //
 // A stage is U cache lines of every row of x (64 U elements) and the weights of the same k, 32 U bytes a row. Pieces of 16
 // bytes lie so that the sixteen lanes that LDS serves in a cycle meet all banks: piece p of row r of x at place p ^ (r / 2 % 8),
-// of P pieces of a weight row at p ^ (r / (16 / P)). In a lane 16 g + r of a 16-row fragment, x takes piece g of one
+// of P pieces of a weight row at p ^ (r / (16 / P)); a single row of x lies as it is, and all lanes read it. In a lane 16 g + r of a 16-row fragment, x takes piece g of one
 // block of k after the other.
 //
 // The matrix cores multiply x by the whole numbers q as they are, and by ones, of which one fragment serves all
@@ -25,17 +25,18 @@ __device__ inline void wait_loads() {
 
 template <bool kFew, int XL, int FN, int U, int W, int S>
 struct Rows {
-  static constexpr int kRows = 8 * XL, kFT = XL < 2 ? 1 : XL / 2;  // rows of x; 16-row fragments
+  static constexpr bool kOne = XL == 0;                            // a single row of x, whose lines a load has side by side
+  static constexpr int kRows = kOne ? 1 : 8 * XL, kFT = XL < 2 ? 1 : XL / 2;  // rows of x; 16-row fragments
   static constexpr int kBN = 16 * FN, kWPieces = 2 * U, kWL = kBN * kWPieces / 64;
   static constexpr int kSteps = 8 / U;         // stages a period
-  static constexpr int kLoads = XL * U + kWL;  // a stage
+  static constexpr int kXLoads = kOne ? 1 : XL, kLoads = kOne ? 1 + kWL : XL * U + kWL;  // x's a line; all of a stage
   static constexpr int kLine = kRows * 128, kXBytes = U * kLine, kWBytes = kWL * 1024, kStage = kXBytes + kWBytes;
   static constexpr int kWindow = Window<kFew>::kBytes, kSL = (kBN + 63) / 64;
   static constexpr int kWave = S * kStage + kBN * kWindow;  // LDS bytes of a wave
   static constexpr int kChain = kFew ? (2 * U < 4 ? 2 * U : 4) : 1;  // blocks that certainly share a scale
   static constexpr int kSums = W * kFT * FN * 1024;
   static constexpr int kLds = W * kWave > kSums ? W * kWave : kSums;
-  static_assert(kBN * kWPieces % 64 == 0 && kLds <= 160 * 1024 && (S - 1) * kLoads < 64, "");
+  static_assert(kBN * kWPieces % 64 == 0 && U <= 8 && kLds <= 160 * 1024 && (S - 1) * kLoads < 64, "");
 };
 
 template <int XT, bool kFew, int XL, int FN, int U, int W, int S>
@@ -57,14 +58,17 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
   if (wave < periods) {
     const int32_t items = ((periods - wave + W - 1) / W) * R::kSteps;
     // Where this lane's pieces come from; rows past the tile's end or the weight's are the last ones.
-    const int32_t x_piece = (lane % 8) ^ (lane / 16), x_pieces = a.k / 8;
-    const uint8_t *x_from[XL];
+    const int32_t x_piece = R::kOne ? lane : (lane % 8) ^ (lane / 16), x_pieces = a.k / 8;
+    const uint8_t *x_from[R::kXLoads];
 #pragma unroll
-    for (int i = 0; i < XL; ++i) {
-      int32_t from = min(tile.first + 8 * i + lane / 8, tile.end - 1);
+    for (int i = 0; i < R::kXLoads; ++i) {
+      int32_t from = min(tile.first + 8 * i + (R::kOne ? 0 : lane / 8), tile.end - 1);
       if (a.gather) from = min((uint32_t)a.order[from] / (uint32_t)a.top, (uint32_t)a.x_rows - 1);
       x_from[i] = static_cast<const uint8_t *>(a.x) + from * a.x_stride * 2;
     }
+    // Of eight rows those that are not there are not read: what LDS holds of them gives sums that nobody looks at.
+    const bool has_row = R::kOne ? lane < 8 * U : lane / 8 < tile.end - tile.first;
+    const uint32_t lds_at = lds_address(mine);
     const int64_t w_first = (int64_t)tile.expert * a.n + n0;
     const uint8_t *const w_base = a.w + w_first * blocks * 16;
     const uint32_t w_row_bytes = (uint32_t)blocks * 16, w_last = (uint32_t)min(R::kBN - 1, a.n - 1 - n0) * w_row_bytes;
@@ -75,25 +79,31 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
     auto period_of = [&](int32_t item) { return wave + W * (item / R::kSteps); };
     auto fetch = [&](int32_t item, int slot) {
       const int32_t step = period_of(item) * R::kSteps + item % R::kSteps;
-      uint8_t *const to = mine + slot * R::kStage;
+      if constexpr (R::kOne) {
+        if (has_row) copy16_apart(x_from[0] + min(step * U * 8 + x_piece, x_pieces - 1) * 16, lds_at + slot * R::kStage);
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {  // eight rows a load, so odd loads have the other half of the keys
-        const int32_t x_at[2] = {min((step * U + u) * 8 + x_piece, x_pieces - 1) * 16, min((step * U + u) * 8 + (x_piece ^ 4), x_pieces - 1) * 16};
+        for (int u = 0; u < U; ++u) {  // eight rows a load, so odd loads have the other half of the keys
+          const int32_t x_at[2] = {min((step * U + u) * 8 + x_piece, x_pieces - 1) * 16, min((step * U + u) * 8 + (x_piece ^ 4), x_pieces - 1) * 16};
+          if (XL > 1 || has_row) {
 #pragma unroll
-        for (int i = 0; i < XL; ++i) copy16(x_from[i] + x_at[i & 1], to + u * R::kLine + i * 1024);
+            for (int i = 0; i < XL; ++i) copy16_apart(x_from[i] + x_at[i & 1], lds_at + slot * R::kStage + u * R::kLine + i * 1024);
+          }
+        }
       }
       const uint32_t w_at[2] = {(uint32_t)min(step * R::kWPieces + w_piece, blocks - 1) * 16,
                                 (uint32_t)min(step * R::kWPieces + (w_piece ^ 4), blocks - 1) * 16};
 #pragma unroll
       for (int i = 0; i < R::kWL; ++i)
-        copy16(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at[R::kWPieces == 8 ? i & 1 : 0]),
-               to + R::kXBytes + i * 1024);
+        copy16_apart(w_base + (min((uint32_t)(wrow + i * (64 / R::kWPieces)) * w_row_bytes, w_last) + w_at[R::kWPieces == 8 ? i & 1 : 0]),
+                     lds_at + slot * R::kStage + R::kXBytes + i * 1024);
     };
     Window<kFew> window[R::kSL];
+    const bool turns = a.groups >= Window<kFew>::kEntries;
+    auto scales_row = [&](int i) -> int64_t { return w_first + min(min(i * 64 + lane, R::kBN - 1), a.n - 1 - n0); };
     auto get_scales = [&](int32_t period) {
 #pragma unroll
-      for (int i = 0; i < R::kSL; ++i)
-        load_window(a, w_first + min(min(i * 64 + lane, R::kBN - 1), a.n - 1 - n0), window_start<kFew>(a, period), window[i]);
+      for (int i = 0; i < R::kSL; ++i) load_window(a, scales_row(i), window_start<kFew>(a, period), window[i]);
     };
     auto put_scales = [&]() {  // LDS keeps a wave's order
 #pragma unroll
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
           fw[b][n] = *reinterpret_cast<const uint32_t *>(wl + (n * 16 + r) * R::kWPieces * 16 + (b ^ (r / (16 / R::kWPieces))) * 16 + g * 4);
 #pragma unroll
         for (int t = 0; t < kFT; ++t)
-          fx[b][t] = *reinterpret_cast<const u32x4 *>(xl + b / 2 * R::kLine + (t * 16 + r) % R::kRows * 128 + ((4 * (b % 2) + g) ^ (r >> 1)) * 16);
+          fx[b][t] = *reinterpret_cast<const u32x4 *>(xl + b / 2 * R::kLine + (t * 16 + r) % R::kRows * 128 + ((4 * (b % 2) + g) ^ (R::kOne ? 0 : r >> 1)) * 16);
       }
       const int32_t first = 16 * period + in * 2 * U, start = window_start<kFew>(a, period);
       // Pieces past the end of x's rows hold other elements: they are taken as zeros.
@@ -158,7 +168,12 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
       }
     };
 
-    get_scales(wave);
+    if (turns) {
+      get_scales(wave);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::kSL; ++i) load_all(a, scales_row(i), window[i]);
+    }
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
       if (i < items) fetch(i, i);
@@ -166,7 +181,7 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
     for (int32_t item = 0; item < items; ++item) {
       if (item % R::kSteps == 0) {
         put_scales();
-        if (item + R::kSteps < items) get_scales(period_of(item) + W);
+        if (turns && item + R::kSteps < items) get_scales(period_of(item) + W);
       }
       if (item + S - 1 < items) {
         fetch(item + S - 1, slot == 0 ? S - 1 : slot - 1);
@@ -184,7 +199,7 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
 #pragma unroll
       for (int n = 0; n < FN; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) finite &= __builtin_fabsf(acc[t][n][i]) < __builtin_inff();
+        for (int i = 0; i < 4; ++i) finite &= __builtin_fabsf(acc[t][n][i]) < __builtin_inff() || tile.first + t * 16 + 4 * g + i >= tile.end;
     if (__builtin_expect(__any(!finite), 0)) {
 #pragma unroll
       for (int t = 0; t < kFT; ++t)
@@ -193,7 +208,7 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
 #pragma unroll 1
       for (int32_t item = 0; item < items; ++item) {
         if (item % R::kSteps == 0) {
-          get_scales(period_of(item));
+          if (turns) get_scales(period_of(item));
           put_scales();
         }
         fetch(item, 0);
@@ -229,14 +244,20 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
   }
 }
 
-// The shapes of a workgroup: 8 XL rows of x, 16 FN weight rows, U lines a stage, W waves, S stages. `resident` of them fit a
-// CU, and one takes `us` for each period of k that a wave has.
+// The shapes of a workgroup: 8 XL rows of x or one, 16 FN weight rows, U lines a stage, W waves, S stages. `resident` of them fit
+// a CU, and one takes `us` for each period of k that a wave has; workgroups past the first on a CU cost `start` each beside. One token
+// through 4096 x 14336, 4096 x 4096 and 14336 x 4096 (k x n) takes, in microseconds: one row and 32 weight rows 8.1, 5.4, 11.4; one and 16
+// 9.3, 4.4, 8.5; eight rows and 32 weight rows, four waves 9.2, 6.4, 16.8, eight waves 10.9, 5.6, 12.0; eight and 16 14.0, 4.7, 9.1.
+// 64 x 8192 x 8192: 32 rows and 64 weight rows 22.5, with three stages 23.8, 32 and 32 28, 64 and 32 23.1, 16 and 64 32.
 struct Choice {
   int32_t rows, cols, waves, resident;
   float us, start;
 };
-constexpr Choice kChoices[] = {{8, 32, 4, 2, 2.5f, 1.3f}, {8, 32, 8, 1, 2.7f, 1.9f}, {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 4, 1, 2.8f, 2.1f},
-                               {32, 32, 6, 1, 3.2f, 1.2f}, {32, 64, 4, 1, 3.8f, 2.7f}, {64, 64, 4, 1, 6.2f, 3.5f}};
+constexpr Choice kChoices[] = {{1, 32, 8, 2, 2.0f, 1.3f},  {1, 16, 8, 3, 1.4f, 1.0f},  {8, 32, 4, 2, 2.5f, 1.3f},  {8, 32, 8, 1, 2.7f, 1.9f},
+                               {8, 16, 8, 1, 2.0f, 1.0f},  {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 4, 1, 2.8f, 2.1f}, {32, 32, 6, 1, 3.2f, 1.2f},
+                               {32, 64, 4, 1, 3.7f, 2.7f}};
+// Alike for all, the launch and the first loads, which the tiles' figures have in them; and what groups below 128 take more.
+constexpr double kBase = 5.0, kFine = 1.35;
 
 template <int XT, bool kFew, int XL, int FN, int U, int W, int S>
 void launch(const Int4Args &a, hipStream_t stream) {
@@ -248,13 +269,15 @@ void launch(const Int4Args &a, hipStream_t stream) {
 template <int XT, bool kFew>
 void launch_type(const Int4Args &a, int choice, hipStream_t stream) {
   switch (choice) {
-    case 0: return launch<XT, kFew, 1, 2, 4, 4, 2>(a, stream);
-    case 1: return launch<XT, kFew, 1, 2, 4, 8, 2>(a, stream);
-    case 2: return launch<XT, kFew, 2, 2, 2, 8, 2>(a, stream);
-    case 3: return launch<XT, kFew, 2, 4, 4, 4, 2>(a, stream);
-    case 4: return launch<XT, kFew, 4, 2, 2, 6, 2>(a, stream);
-    case 5: return launch<XT, kFew, 4, 4, 2, 4, 3>(a, stream);
-    default: return launch<XT, kFew, 8, 4, 1, 4, 3>(a, stream);
+    case 0: return launch<XT, kFew, 0, 2, 4, 8, 2>(a, stream);
+    case 1: return launch<XT, kFew, 0, 1, 4, 8, 2>(a, stream);
+    case 2: return launch<XT, kFew, 1, 2, 4, 4, 2>(a, stream);
+    case 3: return launch<XT, kFew, 1, 2, 4, 8, 2>(a, stream);
+    case 4: return launch<XT, kFew, 1, 1, 4, 8, 2>(a, stream);
+    case 5: return launch<XT, kFew, 2, 2, 2, 8, 2>(a, stream);
+    case 6: return launch<XT, kFew, 2, 4, 4, 4, 2>(a, stream);
+    case 7: return launch<XT, kFew, 4, 2, 2, 6, 2>(a, stream);
+    default: return launch<XT, kFew, 4, 4, 2, 4, 2>(a, stream);
   }
 }
 
@@ -266,10 +289,12 @@ Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus) {
   int i = 0;
   for (const Choice &c : kChoices) {
     const int at = i++;
+    // One row a workgroup reads its weights for that row alone: for a single row, or experts that have hardly more.
+    if (c.rows == 1 && !a.offsets && a.rows > 1) continue;
     if (product_tiles(a, c.rows) > 65535 || (double)((a.n + c.cols - 1) / c.cols) * c.waves * 64 > kMostWorkItems) continue;
-    const double each = expected_tiles(a, c.rows) * (double)((a.n + c.cols - 1) / c.cols) / ((double)cus * c.resident);
+    const double each = (c.rows == 1 ? a.rows : expected_tiles(a, c.rows)) * (double)((a.n + c.cols - 1) / c.cols) / ((double)cus * c.resident);
     const double rounds = each <= 1 ? 1.0 : __builtin_ceil(each - 0.01);
-    const double us = rounds * (double)((periods + c.waves - 1) / c.waves) * c.us + (each > 1 ? each - 1 : 0) * c.start;
+    const double us = kBase + (rounds * (double)((periods + c.waves - 1) / c.waves) * c.us + (each > 1 ? each - 1 : 0) * c.start) * (a.shift < 2 ? kFine : 1.0);
     if (best.choice < 0 || us < best.us) best = {at, us};
   }
   return best;
