@@ -5,7 +5,7 @@
 // among its lanes by DPP moves. All sums are FP32 in a fixed order, those over tokens FP64 at their end.
 //
 // Route: `top` times the row's largest key is found and taken out. Keys are the logits themselves, compared exactly,
-// or with a bias score + bias in FP64: in FP32 two experts near the border could change places by rounding.
+// or with a bias score + bias, which are compared in FP64 where FP32 cannot tell two of them apart.
 // Balance: p = softmax or normalized sigmoids, of which a lane adds up its experts' over its rows; a second launch
 // of one workgroup adds up the workgroups' sums.
 #include <type_traits>
@@ -30,9 +30,9 @@ struct RouteArgs {
 };
 
 // `op` over the L lanes of a row; all of them get the result. Every step joins two halves that already agree.
-template <int kControl>
-__device__ inline float moved(float v) {
-  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), kControl, 0xf, 0xf, true));
+template <int kControl, typename T>
+__device__ inline T moved(T v) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int32_t, v), kControl, 0xf, 0xf, true));
 }
 template <int kControl>
 __device__ inline double moved(double v) {
@@ -41,11 +41,11 @@ __device__ inline double moved(double v) {
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), kControl, 0xf, 0xf, true);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-template <int kRows>  // 16: the other row of 16 lanes of a pair, 32: the other half of the wave
-__device__ inline void halves(float v, float &a, float &b) {
-  const uint32_t u = __float_as_uint(v);
+template <int kRows, typename T>  // 16: the other row of 16 lanes of a pair, 32: the other half of the wave
+__device__ inline void halves(T v, T &a, T &b) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const auto r = kRows == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+  a = __builtin_bit_cast(T, (uint32_t)r[0]), b = __builtin_bit_cast(T, (uint32_t)r[1]);
 }
 template <int kRows>
 __device__ inline void halves(double v, double &a, double &b) {
@@ -139,6 +139,33 @@ __device__ inline void store_vals(typename Elem<T>::raw *row, int32_t col, int32
   }
 }
 
+// exp(x) = 2^t (1 + rest ln 2), where t = x log2(e) rounded, and rest what that lost and what log2(e) has behind FP32: two steps
+// of FP32 off at most, where expf takes twice the instructions. Below x = -150, of masks too, 0; a NaN stays one.
+__device__ inline float exp_of(float x) {
+  constexpr float kLog2e = 1.44269502e+0f, kLog2eRest = 1.92596303e-8f, kLn2 = 0.693147181f;
+  x = x < -150.0f ? -150.0f : x;
+  const float t = x * kLog2e, rest = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, -t)), e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, rest * kLn2, e);
+}
+__device__ inline float one_over(float d) {  // for finite d
+  const float r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+}
+// 1 / (1 + exp(-x)): below x = -88 less than 2^-126.
+__device__ inline float sigmoid_of(float x) { return one_over(1.0f + exp_of(x < -88.0f ? 88.0f : -x)); }
+
+// The largest of a row's logits that is no NaN; 0 in a row of none but -inf, of which all differences are -inf then.
+template <int L, int V>
+__device__ inline float largest(const float (&logit)[V]) {
+  float most = logit[0] > kNone ? logit[0] : kNone;
+#pragma unroll
+  for (int j = 1; j < V; ++j) most = logit[j] > most ? logit[j] : most;
+  int32_t k = __builtin_bit_cast(int32_t, most + 0.0f);
+  k = over_row<L>(k ^ (k >> 31 & 0x7fffffff), Max());
+  most = __builtin_bit_cast(float, k ^ (k >> 31 & 0x7fffffff));
+  return most > kNone ? most : 0.0f;
+}
+
 constexpr int kRouteThreads = 256;
 
 // LDS that lanes of one wave share: what they wrote is there for the others.
@@ -148,13 +175,73 @@ __device__ inline void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// kBias: keys are scores and a bias in FP64 (its scores by kSigmoid).
+// Keys in the order of FP32 numbers, as whole numbers: their maxima need no care for NaN and go with DPP moves in one instruction.
+constexpr int32_t kNoKey = INT32_MIN;
+__device__ inline int32_t key_of(float f) {  // the two zeros are alike; -inf and NaN have no key
+  const int32_t b = __builtin_bit_cast(int32_t, f + 0.0f);
+  return f > kNone ? b ^ (b >> 31 & 0x7fffffff) : kNoKey;
+}
+__device__ inline float of_key(int32_t k) { return __builtin_bit_cast(float, k ^ (k >> 31 & 0x7fffffff)); }
+
+// One after the other the row's largest keys, ties to the lowest expert, into `mine`: the first `top`. With keys that are not
+// exact, as many more as do not follow by enough (`apart`), so that the true ones are among them; how many, alike for all rows of
+// the wave, and whether any two are too near. Mostly each row has one key that is the largest: the masks of who has it tell, and
+// the tie's longer way is left out (65536 x 128 FP32, one row in twenty of -inf alone, eight of them: 20.6 us where those rows
+// take it too, 17.8 us so).
+struct Chosen {
+  int32_t count;
+  bool sure;
+};
+template <bool kNear, int L, int V, typename Apart>
+__device__ inline Chosen choose(int32_t (&key)[V], int32_t top, int32_t *mine, Apart apart) {
+  const int in_wave = threadIdx.x & 63, in_row = in_wave & (L - 1), row_in_wave = in_wave / L;
+  int32_t last = INT32_MAX, i = 0;
+  bool sure = true;
+  for (;; ++i) {
+    int32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) best = __builtin_elementwise_max(best, key[j]);
+    best = __builtin_elementwise_max(over_row<L>(best, Max()), kNoKey + 1);  // no key is that: a row without any finds none
+    const bool some = best != kNoKey + 1;
+    if constexpr (kNear) {
+      const bool far = apart(last, best);
+      if (__all(!some || (i >= top && far))) break;
+      sure &= !some || far;
+      last = best;
+    } else if (i == top) {
+      break;
+    }
+    uint64_t who[V];
+    int32_t at = V, hits = 0;
+#pragma unroll
+    for (int j = V - 1; j >= 0; --j) {
+      const bool has = key[j] == best;
+      who[j] = __ballot(has);
+      hits += __popcll(who[j]);
+      at = has ? j : at;  // the first of this lane's
+      key[j] = has ? kNoKey : key[j];
+    }
+    bool won = at < V;
+    if (hits * L != __popcll(__ballot(some))) {
+      const uint64_t lanes = __ballot(won), own = L == 64 ? lanes : lanes >> (row_in_wave * L) & ((1ull << (L & 63)) - 1);
+      won = __ffsll((unsigned long long)own) - 1 == in_row;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if ((who[j] >> in_wave & 1) && !(won && j == at)) key[j] = best;
+    }
+    if (won) mine[i] = in_row * V + at;
+  }
+  return {i, (bool)__all(sure)};
+}
+
+// kBias: keys are scores and a bias. In FP32 they are off by less than 2^-19 of 1 or of themselves (exponentials 2^-22, their sum over
+// lanes and a lane's experts 2^-20, the sum with the bias 2^-24); where two that follow each other are not 2^-17 apart, those chosen and
+// all that are near the last of them are put in order by keys in FP64. (All keys in FP64: 8192 x 256 15.3 us, 12.9 us so.)
 template <int T, int L, int V, bool kSigmoid, bool kBias>
 __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a) {
-  typedef std::conditional_t<kBias, double, float> Key;
   typedef typename Elem<T>::raw raw;
   constexpr int kRows = 64 / L, kWaves = kRouteThreads / 64;
-  __shared__ int32_t chosen[kWaves * kRows * L * V];
+  __shared__ int32_t chosen[kWaves * kRows * L * V], sorted[kBias ? kWaves * kRows * L * V : 1];
   const int wave = threadIdx.x >> 6, in_wave = threadIdx.x & 63, in_row = in_wave & (L - 1), row_in_wave = in_wave / L;
   int32_t *const mine = chosen + (wave * kRows + row_in_wave) * L * V;
   const int64_t step = (int64_t)gridDim.x * kWaves * kRows;
@@ -164,11 +251,11 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
     const raw *const row = static_cast<const raw *>(a.logits) + t * a.stride;
     float logit[V];
     load_vals<T, V>(row, in_row * V, a.experts, logit);
-    float most = kNone;
-#pragma unroll
-    for (int j = 0; j < V; ++j) most = __builtin_elementwise_max(most, logit[j]);
-    most = over_row<L>(most, Max());
-    float nan = 0;  // softmax: a NaN or an infinity makes all of the row's scores NaN
+    for (int32_t i = in_row; i < (kBias ? L * V : a.top); i += L) mine[i] = -1;
+    wave_sync();
+    // Softmax without a division by the chosen ones' sum, or as part of keys: its largest logit and its sum. A NaN or an
+    // infinity makes all of the row's scores NaN.
+    float most = 0, total = 1.0f, nan = 0, score[V];
     if constexpr (!kSigmoid) {
       bool any = false;
 #pragma unroll
@@ -176,82 +263,98 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
       const uint64_t rows = __ballot(any);
       const uint64_t own = L == 64 ? rows : rows >> (row_in_wave * L) & ((1ull << (L & 63)) - 1);
       if (own) nan = __builtin_nanf("");
-    }
-    Key key[V];
-    if constexpr (kBias) {
-      double sum = 1.0;
-      if constexpr (!kSigmoid) {
-        sum = 0.0;
+      if (kBias || !a.normalize) {
+        most = largest<L>(logit);
+        total = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          key[j] = logit[j] > kNone ? exp((double)logit[j] - (double)most) : 0.0;
-          sum += key[j];
-        }
-        sum = over_row<L>(sum, Sum());
+        for (int j = 0; j < V; ++j) score[j] = exp_of(logit[j] - most), total += score[j];
+        total = over_row<L>(total, Sum());
       }
+    }
+    int32_t key[V];
+    if constexpr (kBias) {
+      float bias[V];
+      const float by = kSigmoid ? 1.0f : one_over(total);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int32_t e = in_row * V + j;
-        const double b = e < a.experts ? (double)a.bias[e] : 0.0;
-        const double k = (kSigmoid ? 1.0 / (1.0 + exp(-(double)logit[j])) : key[j] / sum) + b;
-        key[j] = logit[j] > kNone && k == k ? k : (double)kNone;
+        bias[j] = a.bias[min(in_row * V + j, a.experts - 1)];
+        const float k = (kSigmoid ? sigmoid_of(logit[j]) : score[j] * by) + bias[j];
+        key[j] = logit[j] > kNone ? key_of(k) : kNoKey;
+      }
+      const Chosen c = choose<true, L, V>(key, a.top, mine, [](int32_t last, int32_t best) {
+        const float f = of_key(best);
+        return last == INT32_MAX || of_key(last) - f > 0x1p-17f * __builtin_elementwise_max(1.0f, __builtin_fabsf(f));
+      });
+      if (__builtin_expect(!c.sure, 0)) {
+        wave_sync();
+        double sum = 1.0;
+        if constexpr (!kSigmoid) {
+          sum = 0.0;
+#pragma unroll 1
+          for (int j = 0; j < V; ++j) sum += exp((double)Elem<T>::get(row[min(in_row * V + j, a.experts - 1)]) - (double)most) * (in_row * V + j < a.experts ? 1.0 : 0.0);
+          sum = over_row<L>(sum, Sum());
+        }
+        // An expert's place: how many of the others have a larger key, or the same and a lower number. One a lane and turn.
+        for (int32_t i0 = 0; i0 < c.count; i0 += L) {
+          const int32_t e = i0 + in_row < c.count ? mine[i0 + in_row] : -1;
+          auto exact = [&](int32_t of) -> double {
+            const double l = (double)Elem<T>::get(row[max(of, 0)]);
+            return (kSigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - (double)most) / sum) + (double)a.bias[max(of, 0)];
+          };
+          const double own = exact(e);
+          int32_t place = 0;
+          for (int32_t j0 = 0; j0 < c.count; j0 += L) {
+            const int32_t their = j0 + in_row < c.count ? mine[j0 + in_row] : -1;
+            const double their_key = i0 == j0 ? own : exact(their);
+            for (int32_t j = 0; j < L && j0 + j < c.count; ++j) {
+              const double k = __shfl(their_key, j, L);
+              const int32_t o = __shfl(their, j, L);
+              place += o >= 0 && (k > own || (k == own && o < e));
+            }
+          }
+          wave_sync();
+          if (e >= 0) sorted[(wave * kRows + row_in_wave) * L * V + place] = e;
+        }
+        wave_sync();
+        for (int32_t i = in_row; i < c.count; i += L)
+          if (mine[i] >= 0) mine[i] = sorted[(wave * kRows + row_in_wave) * L * V + i];
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = logit[j] > kNone ? logit[j] : kNone;  // a NaN's, too
-    }
-    for (int32_t i = in_row; i < a.top; i += L) mine[i] = -1;
-    wave_sync();
-    for (int32_t i = 0; i < a.top; ++i) {
-      Key best = key[0];
-#pragma unroll
-      for (int j = 1; j < V; ++j) best = __builtin_elementwise_max(best, key[j]);
-      best = over_row<L>(best, Max());
-      const bool some = best > (Key)kNone;
-      int32_t at = V;  // the first of this lane's that has it
-#pragma unroll
-      for (int j = V - 1; j >= 0; --j) at = key[j] == best ? j : at;
-      const uint64_t hits = __ballot(some && at < V);
-      const uint64_t own = L == 64 ? hits : hits >> (row_in_wave * L) & ((1ull << (L & 63)) - 1);
-      if (hits == 0) break;  // no row of this wave has any left
-      const bool won = some && at < V && __ffsll((unsigned long long)own) - 1 == in_row;  // ties: the lowest expert
-      if (won) mine[i] = in_row * V + at;
-#pragma unroll
-      for (int j = 0; j < V; ++j) key[j] = won && j == at ? (Key)kNone : key[j];
+      for (int j = 0; j < V; ++j) key[j] = key_of(logit[j]);
+      choose<false, L, V>(key, a.top, mine, [](int32_t, int32_t) { return true; });
     }
     wave_sync();
     // Weights: those of a row's choice relative to its largest chosen logit, where they are divided by their sum.
-    float top_logit = kNone;
+    const int32_t first = in_row < a.top ? mine[in_row] : -1;
+    const float first_logit = Elem<T>::get(row[max(first, 0)]);
+    auto chosen_logit = [&](int32_t i, int32_t e) -> float { return i == in_row ? first_logit : Elem<T>::get(row[max(e, 0)]); };
+    float base = most;
     if (a.normalize) {
-      for (int32_t i = in_row; i < a.top; i += L)
-        if (mine[i] >= 0) top_logit = __builtin_elementwise_max(top_logit, Elem<T>::get(row[mine[i]]));
-      top_logit = over_row<L>(top_logit, Max());
+      int32_t top_key = first >= 0 ? key_of(first_logit) : kNoKey;
+      for (int32_t i = in_row + L; i < a.top; i += L)
+        if (mine[i] >= 0) top_key = __builtin_elementwise_max(top_key, key_of(Elem<T>::get(row[mine[i]])));
+      base = of_key(over_row<L>(top_key, Max()));
     }
-    const float base = a.normalize ? top_logit : most;
-    auto value = [&](int32_t e) -> float {
-      if (e < 0) return 0.0f;
-      const float l = Elem<T>::get(row[e]);
-      if constexpr (kSigmoid) {  // sigmoids that are all small, as multiples of exp(base)
-        return a.normalize && base < 0 ? expf(l - base) / (1.0f + expf(l)) : 1.0f / (1.0f + expf(-l));
-      } else {
-        return expf(l - base) + nan;
-      }
+    auto value = [&](int32_t i, int32_t e) -> float {
+      const float l = chosen_logit(i, e);
+      float v;
+      if constexpr (kSigmoid)  // sigmoids that are all small, as multiples of exp(base)
+        v = a.normalize && base < 0 ? exp_of(l - base) * sigmoid_of(-l) : sigmoid_of(l);
+      else
+        v = exp_of(l - base) + nan;
+      return e >= 0 ? v : 0.0f;
     };
-    float total = 0;
+    const float first_value = value(in_row, first);
     if (a.normalize) {
-      for (int32_t i = in_row; i < a.top; i += L) total += value(mine[i]);
-      total = over_row<L>(total, Sum());
-    } else if constexpr (kSigmoid) {
-      total = 1.0f;
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) total += logit[j] > kNone ? expf(logit[j] - base) : 0.0f;
+      total = first_value;
+      for (int32_t i = in_row + L; i < a.top; i += L) total += value(i, mine[i]);
       total = over_row<L>(total, Sum());
     }
     if (token)
       for (int32_t i = in_row; i < a.top; i += L) {
         const int32_t e = mine[i];
-        const float share = e >= 0 ? value(e) / total : 0.0f;
+        const float share = e >= 0 ? (i == in_row ? first_value : value(i, e)) / total : 0.0f;
         a.ids[t * a.top + i] = e;
         a.weights[t * a.top + i] = share * a.scale;
         if (a.shares) a.shares[t * a.top + i] = share;
@@ -287,7 +390,7 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_grad_kernel(RouteA
       const int32_t e = a.ids[t * a.top + i];
       if (e < 0 || e >= a.experts) continue;
       float d = a.shares[t * a.top + i] * (a.dweights[t * a.top + i] - back);
-      if constexpr (kSigmoid) d *= 1.0f / (1.0f + expf(Elem<T>::get(row[e])));
+      if constexpr (kSigmoid) d *= sigmoid_of(-Elem<T>::get(row[e]));
       mine[e] = d * a.scale;
     }
     wave_sync();
@@ -296,20 +399,15 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_grad_kernel(RouteA
     for (int j = 0; j < V; ++j) d[j] = mine[in_row * V + j];
     if constexpr (!kSigmoid) {
       if (!a.normalize) {
-        float logit[V], most = kNone, total = 0;
+        float logit[V], e[V], total = 0;
         load_vals<T, V>(row, in_row * V, a.experts, logit);
+        const float most = largest<L>(logit);
 #pragma unroll
-        for (int j = 0; j < V; ++j) most = __builtin_elementwise_max(most, logit[j]);
-        most = over_row<L>(most, Max());
-        float e[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          e[j] = logit[j] > kNone ? expf(logit[j] - most) : logit[j] == kNone ? 0.0f : logit[j];
-          total += e[j];
-        }
+        for (int j = 0; j < V; ++j) e[j] = exp_of(logit[j] - most), total += e[j];
         total = over_row<L>(total, Sum());
+        const float by = total == 0.0f ? 0.0f : one_over(total) * c * a.scale;
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] -= logit[j] == kNone ? 0.0f : e[j] / total * c * a.scale;
+        for (int j = 0; j < V; ++j) d[j] -= logit[j] == kNone ? 0.0f : e[j] * by;
       }
     }
     if (token) store_vals<T, V>(static_cast<raw *>(a.dlogits) + t * a.experts, in_row * V, a.experts, d);
@@ -337,25 +435,22 @@ constexpr int kBalanceThreads = 512;
 // p of a row's kVals experts (of a row of -inf throughout: zeros, and `empty`), and for sigmoids 1 - sigmoid.
 template <int L, int V, bool kSigmoid>
 __device__ inline bool shares_of(const float (&logit)[V], float (&p)[V], float (&rest)[V]) {
-  float most = kNone, total = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) most = __builtin_elementwise_max(most, logit[j]);
-  most = over_row<L>(most, Max());
+  const float most = largest<L>(logit);
+  float total = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     if constexpr (kSigmoid) {  // sigmoids that are all small, as multiples of exp(most)
-      const float e = expf(-logit[j]);  // infinite for small logits: the sigmoid is 0, and 1 - it 1
-      rest[j] = 1.0f / (1.0f + expf(logit[j]));
-      p[j] = most < 0 ? expf(logit[j] - most) * rest[j] : 1.0f / (1.0f + e);
+      rest[j] = sigmoid_of(-logit[j]);
+      p[j] = most < 0 ? exp_of(logit[j] - most) * rest[j] : sigmoid_of(logit[j]);
     } else {
-      p[j] = expf(logit[j] - most);
+      p[j] = exp_of(logit[j] - most);
     }
-    if (logit[j] == kNone) p[j] = 0.0f;
+    if (kSigmoid && logit[j] == kNone) p[j] = 0.0f;
     total += p[j];
   }
   total = over_row<L>(total, Sum());
   const bool empty = total == 0.0f;  // no: some p is 1, or at least 1/2, or NaN
-  const float by = empty ? 0.0f : 1.0f / total;
+  const float by = empty ? 0.0f : one_over(total);
 #pragma unroll
   for (int j = 0; j < V; ++j) p[j] *= by;
   return empty;
@@ -370,29 +465,37 @@ __device__ inline void count_ids(const BalanceArgs &a, int32_t *counts) {
   }
 }
 
-// The last step, by one workgroup, from `blocks` workgroups' sums: work-items share out first the blocks of an expert, then
-// the experts.
+// The last step, by one workgroup, from `blocks` workgroups' sums: work-items share out first the blocks of an expert, of which each
+// has kFlight under way at a time, then the experts. (65536 x 128, 256 blocks: 26 us with 512 work-items and loads as they come.)
+template <int kThreads>
 struct FinishWork {
-  double p[kBalanceThreads], all[kBalanceThreads];
-  int32_t count[kBalanceThreads];
-  double pairs[kBalanceThreads];
+  double p[kThreads], all[kThreads], pairs[kThreads];
+  int32_t count[kThreads];
 };
-__device__ inline void finish_balance(const BalanceArgs &a, int32_t blocks, const float *sums, const int32_t *parts, FinishWork &work) {
+template <int kThreads, int kFlight>
+__device__ inline void finish_balance(const BalanceArgs &a, int32_t blocks, const float *sums, const int32_t *parts, FinishWork<kThreads> &work) {
   const int tid = threadIdx.x;
   int32_t width = 1;
-  while (width < a.experts && width < kBalanceThreads) width *= 2;
-  const int32_t shares = kBalanceThreads / width, keys = a.experts + 1;
+  while (width < a.experts && width < kThreads) width *= 2;
+  const int32_t shares = kThreads / width, keys = a.experts + 1;
+  int32_t tokens = 0;
+  for (int32_t b = tid; b < blocks; b += kThreads) tokens += parts[(int64_t)b * keys + a.experts];
   double pairs = 0.0, all = 0.0;
   for (int32_t e0 = 0; e0 < a.experts; e0 += width) {
-    const int32_t e = e0 + tid % width;
+    const int32_t e = e0 + tid % width, from = min(e, a.experts - 1);
     int32_t count = 0;
     double p = 0.0;
-    if (e < a.experts) {
-#pragma unroll 8
-      for (int32_t b = tid / width; b < blocks; b += shares) {
-        count += parts[(int64_t)b * keys + e];
-        p += (double)sums[(int64_t)b * a.experts + e];
+    for (int32_t b = tid / width; b < blocks; b += shares * kFlight) {
+      float f[kFlight];
+      int32_t c[kFlight];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const int32_t at = min(b + i * shares, blocks - 1);
+        f[i] = sums[(int64_t)at * a.experts + from], c[i] = parts[(int64_t)at * keys + from];
       }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i)
+        if (b + i * shares < blocks) p += (double)f[i], count += c[i];
     }
     work.p[tid] = p, work.count[tid] = count;
     __syncthreads();
@@ -404,11 +507,9 @@ __device__ inline void finish_balance(const BalanceArgs &a, int32_t blocks, cons
     }
     __syncthreads();
   }
-  int32_t tokens = 0;
-  for (int32_t b = tid; b < blocks; b += kBalanceThreads) tokens += parts[(int64_t)b * keys + a.experts];
   work.pairs[tid] = pairs, work.all[tid] = all, work.count[tid] = tokens;
   __syncthreads();
-  for (int d = kBalanceThreads / 2; d > 0; d /= 2) {
+  for (int d = kThreads / 2; d > 0; d /= 2) {
     if (tid < d) work.pairs[tid] += work.pairs[tid + d], work.all[tid] += work.all[tid + d], work.count[tid] += work.count[tid + d];
     __syncthreads();
   }
@@ -425,7 +526,7 @@ __global__ __launch_bounds__(kBalanceThreads) void expert_balance_kernel(Balance
   constexpr int kRows = 64 / L, kWaves = kBalanceThreads / 64, kE = L * V;
   __shared__ float sums[kWaves][kE];
   __shared__ int32_t counts[kE + 1];
-  __shared__ FinishWork work;
+  __shared__ FinishWork<kBalanceThreads> work;
   const int wave = threadIdx.x >> 6, in_wave = threadIdx.x & 63, in_row = in_wave & (L - 1), row_in_wave = in_wave / L;
   for (int32_t i = threadIdx.x; i <= kE; i += kBalanceThreads) counts[i] = 0;
   __syncthreads();
@@ -436,12 +537,19 @@ __global__ __launch_bounds__(kBalanceThreads) void expert_balance_kernel(Balance
   float sum[V] = {};
   int32_t rows = 0;
   const int64_t step = (int64_t)gridDim.x * kWaves * kRows;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * kRows; t0 < a.tokens; t0 += step) {
+  auto load = [&](int64_t t0, float (&logit)[V]) {
+    load_vals<T, V>(static_cast<const raw *>(a.logits) + min(t0 + row_in_wave, a.tokens - 1) * a.stride, in_row * V, a.experts, logit);
+  };
+  int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * kRows;
+  float now[V], soon[V];  // a row's logits, and the next one's, which are loaded meanwhile
+  if (t0 < a.tokens) load(t0, now);
+  for (; t0 < a.tokens; t0 += step) {
     const bool token = t0 + row_in_wave < a.tokens;
-    const int64_t t = token ? t0 + row_in_wave : a.tokens - 1;
-    float logit[V], p[V], rest[V];
-    load_vals<T, V>(static_cast<const raw *>(a.logits) + t * a.stride, in_row * V, a.experts, logit);
-    const bool empty = shares_of<L, V, kSigmoid>(logit, p, rest);
+    float p[V], rest[V];
+    if (t0 + step < a.tokens) load(t0 + step, soon);
+    const bool empty = shares_of<L, V, kSigmoid>(now, p, rest);
+#pragma unroll
+    for (int j = 0; j < V; ++j) now[j] = soon[j];
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] += token ? p[j] : 0.0f;
     rows += token && !empty && in_row == 0;
@@ -463,15 +571,16 @@ __global__ __launch_bounds__(kBalanceThreads) void expert_balance_kernel(Balance
   }
   if (gridDim.x == 1) {
     __syncthreads();
-    finish_balance(a, 1, sums[0], counts, work);
+    finish_balance<kBalanceThreads, 1>(a, 1, sums[0], counts, work);
   } else {
     for (int32_t e = threadIdx.x; e <= a.experts; e += kBalanceThreads) a.parts[(int64_t)blockIdx.x * (a.experts + 1) + e] = counts[e];
   }
 }
 
-__global__ __launch_bounds__(kBalanceThreads) void expert_balance_sum_kernel(BalanceArgs a, int32_t blocks) {
-  __shared__ FinishWork work;
-  finish_balance(a, blocks, a.sums, a.parts, work);
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void expert_balance_sum_kernel(BalanceArgs a, int32_t blocks) {
+  __shared__ FinishWork<kSumThreads> work;
+  finish_balance<kSumThreads, 16>(a, blocks, a.sums, a.parts, work);
 }
 
 // dlogit[t, e] = dloss experts / (N T) p (counts[e] - sum_j counts[j] p[t, j]) (1 - sigmoid, for sigmoids).
@@ -647,7 +756,7 @@ int mps_expert_balance(const void *logits, int32_t type, int64_t tokens, int64_t
   MPS_BY_LOGITS(type, experts, CALL);
 #undef CALL
 #undef LAUNCH
-  if (blocks > 1) hipLaunchKernelGGL(expert_balance_sum_kernel, dim3(1), dim3(kBalanceThreads), 0, s, a, blocks);
+  if (blocks > 1) hipLaunchKernelGGL(expert_balance_sum_kernel, dim3(1), dim3(kSumThreads), 0, s, a, blocks);
   MPS_HIP_CHECK(hipGetLastError());
   return MPS_OK;
 }

@@ -323,11 +323,11 @@ class _NoSecond(torch.autograd.Function):
 
 
 def _only_gradient(gradient, name, ctx, grad):
-    if not torch.is_grad_enabled():
-        return gradient(ctx, grad)
-    with torch.no_grad():
-        d = gradient(ctx, grad)
-    return _NoSecond.apply(d, name, grad, ctx.saved_tensors[0])
+    if torch.is_grad_enabled():
+        with torch.no_grad():
+            d = gradient(ctx, grad)
+        return _NoSecond.apply(d, name, grad, ctx.saved_tensors[0])
+    return gradient(ctx, grad)
 
 
 class _Route(torch.autograd.Function):
@@ -337,7 +337,8 @@ class _Route(torch.autograd.Function):
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids, weights if shares is None else shares)
-        ctx.how = code, normalize, scale
+        # what the backward pass would ask for again, on the engine's thread
+        ctx.how = _native.lib().mps_expert_route_grad, _TYPES[logits.dtype], *logits.shape, logits.stride(0), top, code, normalize, scale
         return ids, weights
 
     @staticmethod
@@ -347,13 +348,13 @@ class _Route(torch.autograd.Function):
 
 def _route_grad(ctx, dweights):
     logits, ids, shares = ctx.saved_tensors
-    (t, experts), (code, normalize, scale) = logits.shape, ctx.how
-    dweights = dweights.contiguous()
-    dlogits = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
-    _call(logits.device, _native.lib().mps_expert_route_grad, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0),
-          ids.shape[1], code, normalize, scale, ids.data_ptr(), shares.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
+    entry, kind, t, experts, stride, top, code, normalize, scale = ctx.how
+    if not dweights.is_contiguous():
+        dweights = dweights.contiguous()
+    dlogits = logits.new_empty((t, experts))
+    _call(logits.device, entry, logits.data_ptr(), kind, t, experts, stride, top, code, normalize, scale, ids.data_ptr(), shares.data_ptr(),
+          dweights.data_ptr(), dlogits.data_ptr())
     return dlogits
-
 
 
 def expert_route(logits: torch.Tensor, top: int, *, scores: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -409,7 +410,7 @@ class _Balance(torch.autograd.Function):
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, kept)  # not the counts: a program may add up its ranks' in place
-        ctx.code = code
+        ctx.how = _native.lib().mps_expert_balance_grad, _TYPES[logits.dtype], *logits.shape, logits.stride(0), code
         return loss, counts
 
     @staticmethod
@@ -419,13 +420,10 @@ class _Balance(torch.autograd.Function):
 
 def _balance_grad(ctx, dloss):
     logits, kept = ctx.saved_tensors
-    t, experts = logits.shape
-    dloss = dloss.contiguous()
-    dlogits = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
-    _call(logits.device, _native.lib().mps_expert_balance_grad, logits.data_ptr(), _TYPES[logits.dtype], t, experts, logits.stride(0),
-          ctx.code, kept.data_ptr(), dloss.data_ptr(), dlogits.data_ptr())
+    entry, kind, t, experts, stride, code = ctx.how
+    dlogits = logits.new_empty((t, experts))
+    _call(logits.device, entry, logits.data_ptr(), kind, t, experts, stride, code, kept.data_ptr(), dloss.data_ptr(), dlogits.data_ptr())
     return dlogits
-
 
 
 def expert_balance(logits: torch.Tensor, ids: torch.Tensor, *, scores: str = "softmax") -> ExpertBalance:
