@@ -248,13 +248,14 @@ __global__ __launch_bounds__(W * 64) void int4_rows_kernel(Int4Args a) {
 // a CU, and one takes `us` for each period of k that a wave has; workgroups past the first on a CU cost `start` each beside. One token
 // through 4096 x 14336, 4096 x 4096 and 14336 x 4096 (k x n) takes, in microseconds: one row and 32 weight rows 8.1, 5.4, 11.4; one and 16
 // 9.3, 4.4, 8.5; eight rows and 32 weight rows, four waves 9.2, 6.4, 16.8, eight waves 10.9, 5.6, 12.0; eight and 16 14.0, 4.7, 9.1.
-// 64 x 8192 x 8192: 32 rows and 64 weight rows 22.5, with three stages 23.8, 32 and 32 28, 64 and 32 23.1, 16 and 64 32.
+// 64 x 8192 x 8192: 32 rows and 64 weight rows 23.5, with three stages 24.8, with eight waves of half the stages 26.9, 32 and 32 29,
+// 16 and 64 30. 32 x 4096 x 14336: 32 and 64 14.6, 16 and 64 19.0, with four waves 20.7; 64 x 4096 x 4096: 12.5, 9.1, 10.8, and 32 and 32 9.7.
 struct Choice {
   int32_t rows, cols, waves, resident;
   float us, start;
 };
 constexpr Choice kChoices[] = {{1, 32, 8, 2, 2.0f, 1.3f},  {1, 16, 8, 3, 1.4f, 1.0f},  {8, 32, 4, 2, 2.5f, 1.3f},  {8, 32, 8, 1, 2.7f, 1.9f},
-                               {8, 16, 8, 1, 2.0f, 1.0f},  {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 4, 1, 2.8f, 2.1f}, {32, 32, 6, 1, 3.2f, 1.2f},
+                               {8, 16, 8, 1, 2.0f, 1.0f},  {16, 32, 8, 1, 3.2f, 2.5f}, {16, 64, 8, 1, 5.5f, 2.1f}, {32, 32, 6, 1, 3.2f, 1.2f},
                                {32, 64, 4, 1, 3.7f, 2.7f}};
 // Alike for all, the launch and the first loads, which the tiles' figures have in them; and what groups below 128 take more.
 constexpr double kBase = 5.0, kFine = 1.35;
@@ -275,7 +276,7 @@ void launch_type(const Int4Args &a, int choice, hipStream_t stream) {
     case 3: return launch<XT, kFew, 1, 2, 4, 8, 2>(a, stream);
     case 4: return launch<XT, kFew, 1, 1, 4, 8, 2>(a, stream);
     case 5: return launch<XT, kFew, 2, 2, 2, 8, 2>(a, stream);
-    case 6: return launch<XT, kFew, 2, 4, 4, 4, 2>(a, stream);
+    case 6: return launch<XT, kFew, 2, 4, 2, 8, 2>(a, stream);
     case 7: return launch<XT, kFew, 4, 2, 2, 6, 2>(a, stream);
     default: return launch<XT, kFew, 4, 4, 2, 4, 2>(a, stream);
   }
