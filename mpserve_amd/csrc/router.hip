@@ -8,6 +8,7 @@
 // or with a bias score + bias, which are compared in FP64 where FP32 cannot tell two of them apart.
 // Balance: p = softmax or normalized sigmoids, of which a lane adds up its experts' over its rows; a second launch
 // of one workgroup adds up the workgroups' sums.
+#include <algorithm>
 #include <type_traits>
 
 #include "mxfp4_common.h"
@@ -577,6 +578,7 @@ __global__ __launch_bounds__(kBalanceThreads) void expert_balance_kernel(Balance
   }
 }
 
+constexpr unsigned kGradBlocks = 1024;  // 65536 x 128 BF16: a workgroup for every 16 rows 20.3 us, these 14.3 us
 constexpr int kSumThreads = 1024;
 __global__ __launch_bounds__(kSumThreads) void expert_balance_sum_kernel(BalanceArgs a, int32_t blocks) {
   __shared__ FinishWork<kSumThreads> work;
@@ -589,6 +591,13 @@ __global__ __launch_bounds__(kRouteThreads) void expert_balance_grad_kernel(Bala
   typedef typename Elem<T>::raw raw;
   constexpr int kRows = 64 / L, kWaves = kRouteThreads / 64;
   const int wave = threadIdx.x >> 6, in_wave = threadIdx.x & 63, in_row = in_wave & (L - 1), row_in_wave = in_wave / L;
+  const int64_t step = (int64_t)gridDim.x * kWaves * kRows;
+  auto load = [&](int64_t t0, float (&logit)[V]) {
+    load_vals<T, V>(static_cast<const raw *>(a.logits) + min(t0 + row_in_wave, a.tokens - 1) * a.stride, in_row * V, a.experts, logit);
+  };
+  int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * kRows;
+  float soon[V];  // the next row's logits, which are loaded meanwhile
+  if (t0 < a.tokens) load(t0, soon);
   float count[V];
   double n = 0;
 #pragma unroll
@@ -599,12 +608,13 @@ __global__ __launch_bounds__(kRouteThreads) void expert_balance_grad_kernel(Bala
   n = over_row<L>(n, Sum());
   const double tokens = a.kept[a.experts];
   const float factor = n > 0 && tokens > 0 ? (float)((double)*a.dloss * a.experts / (n * tokens)) : 0.0f;
-  const int64_t step = (int64_t)gridDim.x * kWaves * kRows;
-  for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * kRows; t0 < a.tokens; t0 += step) {
+  for (; t0 < a.tokens; t0 += step) {
     const bool token = t0 + row_in_wave < a.tokens;
     const int64_t t = token ? t0 + row_in_wave : a.tokens - 1;
     float logit[V], p[V], rest[V], c = 0;
-    load_vals<T, V>(static_cast<const raw *>(a.logits) + t * a.stride, in_row * V, a.experts, logit);
+#pragma unroll
+    for (int j = 0; j < V; ++j) logit[j] = soon[j];
+    if (t0 + step < a.tokens) load(t0 + step, soon);
     shares_of<L, V, kSigmoid>(logit, p, rest);
 #pragma unroll
     for (int j = 0; j < V; ++j) c = __builtin_fmaf(count[j], p[j], c);
@@ -773,7 +783,7 @@ int mps_expert_balance_grad(const void *logits, int32_t type, int64_t tokens, in
   a.kept = const_cast<int32_t *>(kept), a.dloss = dloss, a.dlogits = dlogits;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define LAUNCH(T, L, V, S) \
-  hipLaunchKernelGGL((expert_balance_grad_kernel<T, L, V, S>), dim3(route_grid<L>(tokens)), dim3(kRouteThreads), 0, s, a)
+  hipLaunchKernelGGL((expert_balance_grad_kernel<T, L, V, S>), dim3(std::min(route_grid<L>(tokens), kGradBlocks)), dim3(kRouteThreads), 0, s, a)
 #define CALL(T, L, V) \
   if (scores == MPS_SCORES_SIGMOID) { LAUNCH(T, L, V, true); } else { LAUNCH(T, L, V, false); }
   MPS_BY_LOGITS(type, experts, CALL);
