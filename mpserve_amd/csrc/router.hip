@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
     for (int32_t i = in_row; i < (kBias ? L * V : a.top); i += L) mine[i] = -1;
     wave_sync();
     // Softmax without a division by the chosen ones' sum, or as part of keys: its largest logit and its sum. A NaN or an
-    // infinity makes all of the row's scores NaN.
+    // infinity makes all of the row's scores NaN; as parts of keys these count as 0, so that experts are taken, with NaN for weights.
     float most = 0, total = 1.0f, nan = 0, score[V];
     if constexpr (!kSigmoid) {
       bool any = false;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         bias[j] = a.bias[min(in_row * V + j, a.experts - 1)];
-        const float k = (kSigmoid ? sigmoid_of(logit[j]) : score[j] * by) + bias[j];
+        const float k = (kSigmoid ? sigmoid_of(logit[j]) : nan == 0.0f ? score[j] * by : 0.0f) + bias[j];
         key[j] = logit[j] > kNone ? key_of(k) : kNoKey;
       }
       const Chosen c = choose<true, L, V>(key, a.top, mine, [](int32_t last, int32_t best) {
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
           const int32_t e = i0 + in_row < c.count ? mine[i0 + in_row] : -1;
           auto exact = [&](int32_t of) -> double {
             const double l = (double)Elem<T>::get(row[max(of, 0)]);
-            return (kSigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - (double)most) / sum) + (double)a.bias[max(of, 0)];
+            return (kSigmoid ? 1.0 / (1.0 + exp(-l)) : nan == 0.0f ? exp(l - (double)most) / sum : 0.0) + (double)a.bias[max(of, 0)];
           };
           const double own = exact(e);
           int32_t place = 0;

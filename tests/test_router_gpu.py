@@ -107,6 +107,49 @@ def test_route_keeps_nan_in_its_row():
     assert bool(torch.isfinite(weights).all()) and float(weights[4, 0]) == 1.0  # a NaN of an expert that is not taken
 
 
+@pytest.mark.parametrize("experts", (64, 256, 1000))
+def test_route_with_a_bias_keeps_nan_in_its_row(experts):
+    """Softmax scores that are all NaN still choose, by the bias, and give NaN for weights."""
+    logits = logits_of(1, 6, experts, torch.float32)
+    bias = torch.randn(experts, generator=gen(5), device=DEV)
+    bias[20:40] = bias[3]  # ties, for which keys are made again in 64 bits
+    clean = expert_route(logits, 30, bias=bias)
+    logits[2, 10], logits[4, 11], logits[2, 12] = float("nan"), float("inf"), NONE
+    for normalize in (True, False):
+        ids, weights = expert_route(logits, 30, bias=bias, normalize=normalize)
+        for row, without in ((2, (10, 12)), (4, ())):
+            order = sorted((e for e in range(experts) if e not in without), key=lambda e: (-float(bias[e]), e))
+            assert ids[row].tolist() == order[:30]
+            assert bool(torch.isnan(weights[row]).all())
+        rest = [0, 1, 3, 5]
+        assert torch.equal(ids[rest], clean.ids[rest]) and bool(torch.isfinite(weights[rest]).all())
+    ids, weights = expert_route(logits, 4, scores="sigmoid", bias=bias)
+    assert bool((ids[2] != 10).all()) and bool(torch.isfinite(weights).all())
+
+
+@pytest.mark.parametrize("scores", ("softmax", "sigmoid"))
+@pytest.mark.parametrize("experts,top", ((20, 6), (128, 8), (256, 8), (1000, 100)))
+def test_route_with_keys_that_are_near_one_another(scores, experts, top):
+    """Rows beside one another, of keys that lie within FP32's errors in groups, that are all alike, that are masked but for a few, and
+    that are far apart; the order is that of 64 bits."""
+    g = gen(experts)
+    base = torch.randint(-3, 4, (40, experts), generator=g, device=DEV).float()
+    logits = base + 2.0 ** -18 * torch.randint(0, 5, (40, experts), generator=g, device=DEV)
+    logits[5], logits[6] = 0.0, NONE
+    logits[7, 2:] = NONE
+    logits[8] = torch.randn(experts, generator=g, device=DEV)
+    for bias in (torch.zeros(experts, device=DEV), 0.25 * torch.randint(-1, 2, (experts,), generator=g, device=DEV).float()):
+        ids, weights = expert_route(logits, top, scores=scores, bias=bias)
+        want_ids, want = plain.route(logits, top, scores, bias)
+        # FP64 of both sides agrees to some 2^-50 of 1; keys nearer than that have no order to check
+        key = plain.scores_of(logits, scores) + bias.double()
+        at = [torch.gather(torch.where(logits > NONE, key, torch.full_like(key, -9.0)), 1, i.clamp(min=0).long()) for i in (ids, want_ids)]
+        assert torch.equal(ids < 0, want_ids < 0)
+        assert bool((((at[0] - at[1]).abs() <= 2.0 ** -45) | (ids < 0)).all())
+        for row in range(40):
+            assert len(set(i for i in ids[row].tolist() if i >= 0)) == int((ids[row] >= 0).sum())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("scores", ("softmax", "sigmoid"))
 @pytest.mark.parametrize("normalize", (True, False))
