@@ -421,8 +421,9 @@ int mps_int4_multiply(const mps_int4_product *product, void *workspace, int64_t 
 
 /* The `top` experts of each row of logits[tokens, experts] (`stride` elements from row to row) and their weights:
  * ids and weights are [tokens, top], by falling key, ties to the lower expert. The key is the logit, or with
- * bias[experts] score + bias in 64 bits; a score is the row's softmax or the logit's sigmoid. Experts whose logit or key is -inf
- * or NaN are not taken: where fewer than `top` are left, ids are -1 and weights 0. A weight is scale * share; a share is the
+ * bias[experts] score + bias, compared as in 64 bits; a score is the row's softmax or the logit's sigmoid. Experts whose logit or
+ * key is -inf or NaN are not taken: where fewer than `top` are left, ids are -1 and weights 0. In a row with a NaN or an infinity
+ * the softmax scores are NaN, and so are the weights; the bias alone is the key there. A weight is scale * share; a share is the
  * expert's score, with `normalize` divided by the sum of the row's chosen scores. shares[tokens, top] may be NULL. */
 int mps_expert_route(const void *logits, int32_t type, int64_t tokens, int64_t experts, int64_t stride, int64_t top,
                      int32_t scores, const float *bias, int32_t normalize, float scale, int32_t *ids, float *weights,

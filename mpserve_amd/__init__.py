@@ -5,7 +5,9 @@
 * ``mpserve_amd.decode.DecodePlan`` — one launch for many tensors.
 * ``mpserve_amd.vllm_fp8_huffman`` — the vLLM ``fp8_huffman`` quantization method.
 * ``mpserve_amd.mxfp4`` — 4-bit floating-point weights: quantization and products.
-* ``mpserve_amd.experts`` — tokens to their experts and back, and products with MXFP4 experts;
+* ``mpserve_amd.int4`` — products with int4 weights, of an AWQ checkpoint or the AWQ decode ops.
+* ``mpserve_amd.experts`` — a mixture's router and its balance loss, tokens to their experts and back,
+  and products with MXFP4 and int4 experts;
   ``mpserve_amd.mxfp4_experts`` is a block of them.
 """
 __version__ = "0.1.0"

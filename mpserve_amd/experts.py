@@ -365,7 +365,8 @@ def expert_route(logits: torch.Tensor, top: int, *, scores: str = "softmax", bia
     ``"sigmoid"``. The experts of the largest logits are taken, or with ``bias [experts]`` (FP32) those of the largest
     ``score + bias``, compared in FP64; ties go to the lower expert. The bias counts for the choice only. A weight is the expert's score,
     with ``normalize`` divided by the sum of the token's chosen scores, times ``scale``. An expert whose logit or
-    bias is -inf (or whose logit is NaN) is not taken: where fewer than ``top`` are left, as in a row of padding, ids are
+    bias is -inf or NaN is not taken (a token's softmax weights are NaN where it has a logit that is NaN or +inf, and the
+    bias alone chooses there): where fewer than ``top`` are left, as in a row of padding, ids are
     -1 and weights 0, which :func:`expert_sort` and :func:`expert_combine` take for no expert. The gradient is that of the
     weights; the choice has none."""
     code = _check_logits(logits, scores)
