@@ -431,7 +431,9 @@ void launch(const Int4Args &a, hipStream_t stream) {
 }
 
 // The tiles, in microseconds: `start` is what a tile takes at any k, `few` and `full` what k = 4096 adds to a tile that has a
-// CU to itself, on a card with few of them and a full one, and `many` to each of several. Groups of 64 and of 32 cost more.
+// CU to itself, on a card with few of them and a full one, and `many` to each of several. Groups of 64 and of 32 cost more. The four in turn take, of groups of 128 (rows x k x n): 96 x
+// 4096 x 14336 59, 43, 35, 34; 256 x 4096 x 4096 52, 36, 26, 23; 256 x 4096 x 14336 59, 45, 45, 58; 1024 x 4096 x 14336 129, 158, 145,
+// 190; 4096 x 4096 x 14336 461, 563, 548, 710; of groups of 32, FP16, 1024 x 8192 x 28672 904, 829, 795, 1037.
 struct Choice {
   int32_t bt, bn;
   float start, few, full, many, step, block;

@@ -128,6 +128,9 @@ def _int4_product(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ze
 
 
 def _int4_multiply(p: "_native.MpsInt4Product", device: torch.device) -> None:
+    if torch._C._cuda_getDevice() != device.index:  # the choice of a kernel goes by the device's compute units
+        with torch.cuda.device(device):
+            return _int4_multiply(p, device)
     lib = _native.lib()
     need = ctypes.c_int64(0)
     rc = lib.mps_int4_product_workspace(p, need)

@@ -39,7 +39,7 @@ SHAPES = [  # t, k, n, group
     (1030, 672, 384, 256), (1, 1030, 16, 64), (130, 2056, 520, 32), (50, 2056, 2100, 128), (500, 1030, 1030, 64),
     (130, 500, 1030, 128), (70, 500, 20000, 128), (1, 500, 20000, 32), (700, 96, 4300, 128), (1100, 64, 8300, 64),
     (2100, 32, 8300, 32), (2300, 704, 8500, 128), (4500, 160, 5000, 32), (250, 1030, 4101, 64), (2000, 1030, 4101, 256),
-    (4, 14336, 300, 128), (20, 8192, 700, 2048),
+    (4, 14336, 300, 128), (20, 8192, 700, 2048), (16, 4090, 13000, 128), (13, 4096, 14000, 32),
 ]
 
 
@@ -152,6 +152,29 @@ def test_linear_output_past_32_bits():
     w = plain.weight(values, scales, z, 32).T
     for rows in (slice(0, 3), slice(t // 2, t // 2 + 3), slice(67107, 67112), slice(t - 3, t)):
         assert torch.equal(y[rows], (x[rows].double() @ w).float().to(torch.bfloat16))
+
+
+def test_codes_and_x_past_32_bits():
+    """Codes of over 2^32 bytes (the last expert's lie behind them), and x of over 2^31 elements."""
+    g = gen(3)
+    experts, n, k, group = 33, 16384, 16384, 512
+    codes = torch.randint(0, 256, (experts, n, k // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.exp2(torch.randint(-1, 2, (experts, n, k // group), generator=g, device=DEV).float()).to(torch.bfloat16)
+    z = torch.randint(0, 17, scales.shape, generator=g, device=DEV, dtype=torch.uint8)
+    for t in (2, 600):  # few rows an expert, and tiles of them
+        x = whole_numbers(g, t, k, torch.bfloat16)
+        ids = torch.full((t, 1), experts - 1, dtype=torch.int32, device=DEV)
+        ids[0] = 0
+        y = int4_expert_linear(x, codes, scales, expert_sort(ids, experts), z, group=group, gather=True, out_dtype=torch.float32)
+        for rows, e in ((slice(0, 1), 0), (slice(1, t), experts - 1)):
+            want = int4_linear(x[rows], codes[e], scales[e], z[e], group=group, out_dtype=torch.float32)
+            assert torch.equal(y[rows], want)  # whole numbers, whose sums are exact in any order
+    t = 2 ** 31 // k + 70
+    x = torch.zeros(t, k, dtype=torch.bfloat16, device=DEV)
+    x[-70:] = whole_numbers(g, 70, k, torch.bfloat16)
+    y = int4_linear(x, codes[1, :100], scales[1, :100], z[1, :100], group=group, out_dtype=torch.float32)
+    assert not bool(y[:-70].any())
+    assert torch.equal(y[-70:], int4_linear(x[-70:], codes[1, :100], scales[1, :100], z[1, :100], group=group, out_dtype=torch.float32))
 
 
 def test_awq_checkpoint():

@@ -214,6 +214,22 @@ def test_logits_of_any_layout():
             assert torch.equal(ga[0], gb[0])
 
 
+def test_logits_past_32_bits():
+    """Over 2^31 logits: the last rows are as right as by themselves."""
+    experts, more = 256, 1000
+    t = 2 ** 31 // experts + more
+    logits = torch.full((t, experts), NONE, dtype=torch.bfloat16, device=DEV)
+    logits[-more:] = logits_of(1, more, experts, torch.bfloat16)
+    last = logits[-more:].clone().requires_grad_()
+    logits.requires_grad_()
+    a, b = expert_route(logits, 2), expert_route(last, 2)
+    assert torch.equal(a.ids[-more:], b.ids) and torch.equal(a.weights[-more:], b.weights) and not bool((a.ids[:-more] >= 0).any())
+    la, lb = expert_balance(logits, a.ids), expert_balance(last, b.ids)
+    assert torch.equal(la.counts, lb.counts) and abs(float(la.loss.detach()) - float(lb.loss.detach())) <= 2.0 ** -12
+    (ga,), (gb,) = (torch.autograd.grad((w * w).sum() + loss, x) for w, loss, x in ((a.weights, la.loss, logits), (b.weights, lb.loss, last)))
+    assert torch.equal(ga[-more:], gb) and not bool(ga[:1000].any()) and not bool(ga[t // 2:t // 2 + 1000].any())
+
+
 BALANCE = [(1, 1, 1), (1, 8, 2), (37, 60, 2), (100, 16, 4), (64, 33, 3), (500, 64, 4), (1000, 128, 8), (300, 256, 8), (50, 500, 6), (70, 1000, 8),
            (40000, 8, 2), (20000, 60, 6), (9000, 128, 8), (5000, 1024, 4)]
 
