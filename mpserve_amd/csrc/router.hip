@@ -185,8 +185,8 @@ __device__ inline int32_t key_of(float f) {  // the two zeros are alike; -inf an
 __device__ inline float of_key(int32_t k) { return __builtin_bit_cast(float, k ^ (k >> 31 & 0x7fffffff)); }
 
 // One after the other the row's largest keys, ties to the lowest expert, into `mine`: the first `top`. With keys that are not
-// exact, as many more as do not follow by enough (`apart`), so that the true ones are among them; how many, alike for all rows of
-// the wave, and whether any two are too near. Mostly each row has one key that is the largest: the masks of who has it tell, and
+// exact, as many more as do not follow the last of these by enough (`apart`), so that the true ones are among them; how many, alike
+// for all rows of the wave, and whether any are too near. Mostly each row has one key that is the largest: the masks of who has it tell, and
 // the tie's longer way is left out (65536 x 128 FP32, one row in twenty of -inf alone, eight of them: 20.6 us where those rows
 // take it too, 17.8 us so).
 struct Chosen {
@@ -208,7 +208,7 @@ __device__ inline Chosen choose(int32_t (&key)[V], int32_t top, int32_t *mine, A
       const bool far = apart(last, best);
       if (__all(!some || (i >= top && far))) break;
       sure &= !some || far;
-      last = best;
+      last = i < top ? best : last;
     } else if (i == top) {
       break;
     }
@@ -235,9 +235,10 @@ __device__ inline Chosen choose(int32_t (&key)[V], int32_t top, int32_t *mine, A
   return {i, (bool)__all(sure)};
 }
 
-// kBias: keys are scores and a bias. In FP32 they are off by less than 2^-19 of 1 or of themselves (exponentials 2^-22, their sum over
-// lanes and a lane's experts 2^-20, the sum with the bias 2^-24); where two that follow each other are not 2^-17 apart, those chosen and
-// all that are near the last of them are put in order by keys in FP64. (All keys in FP64: 8192 x 256 15.3 us, 12.9 us so.)
+// kBias: keys are scores and a bias. In FP32 they are off by less than 2^-19 of the row's largest score (exponentials 2^-22, their sum over
+// lanes and a lane's experts 2^-20) and 2^-24 of themselves, by the sum with the bias; where two that follow each other are not 2^-17 and
+// 2^-22 of these apart, those chosen and all that are near the last of them are put in order by keys in FP64. In a row whose
+// experts are all alike (a router that starts from zeros) the order is that of FP32, ties. (All keys in FP64: 8192 x 256 15.3 us, 12.9 us so.)
 template <int T, int L, int V, bool kSigmoid, bool kBias>
 __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a) {
   typedef typename Elem<T>::raw raw;
@@ -275,16 +276,22 @@ __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a
     int32_t key[V];
     if constexpr (kBias) {
       float bias[V];
+      bool alike = true;
+      const float first_logit = Elem<T>::get(row[0]), first_bias = a.bias[0];
       const float by = kSigmoid ? 1.0f : one_over(total);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         bias[j] = a.bias[min(in_row * V + j, a.experts - 1)];
+        alike &= in_row * V + j >= a.experts || (logit[j] == first_logit && bias[j] == first_bias);
         const float k = (kSigmoid ? sigmoid_of(logit[j]) : nan == 0.0f ? score[j] * by : 0.0f) + bias[j];
         key[j] = logit[j] > kNone ? key_of(k) : kNoKey;
       }
-      const Chosen c = choose<true, L, V>(key, a.top, mine, [](int32_t last, int32_t best) {
+      const uint64_t others = __ballot(!alike);
+      const bool ties = (L == 64 ? others : others >> (row_in_wave * L) & ((1ull << (L & 63)) - 1)) == 0;
+      const float score_error = 0x1p-17f * (nan == 0.0f ? by : 0.0f);
+      const Chosen c = choose<true, L, V>(key, a.top, mine, [&](int32_t last, int32_t best) {
         const float f = of_key(best);
-        return last == INT32_MAX || of_key(last) - f > 0x1p-17f * __builtin_elementwise_max(1.0f, __builtin_fabsf(f));
+        return ties || last == INT32_MAX || of_key(last) - f > __builtin_fmaf(0x1p-22f, __builtin_fabsf(f), score_error);
       });
       if (__builtin_expect(!c.sure, 0)) {
         wave_sync();
