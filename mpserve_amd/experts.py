@@ -298,6 +298,16 @@ def _adjacent(logits: torch.Tensor) -> torch.Tensor:
     return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
 
 
+def _kept(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A tensor that a forward pass saved. Autograd's saved-tensor hooks may give back other memory, laid out in another way (an
+    offload's copy of a slice of columns has its rows side by side); what has another size, type or device is refused: kernels
+    would read past its end."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"a saved-tensor hook gave back {tuple(t.shape)} {t.dtype} on {t.device} for what was saved as "
+                           f"{tuple(shape)} {dtype} on {device}")
+    return t
+
+
 def _route(logits, top, code, bias, normalize, scale, shares):
     (t, experts), device = logits.shape, logits.device
     ids = torch.empty((t, top), dtype=torch.int32, device=device)
@@ -337,8 +347,8 @@ class _Route(torch.autograd.Function):
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids, weights if shares is None else shares)
-        # what the backward pass would ask for again, on the engine's thread
-        ctx.how = _native.lib().mps_expert_route_grad, _TYPES[logits.dtype], *logits.shape, logits.stride(0), top, code, normalize, scale
+        # what the backward pass would ask for again, on the engine's thread; not the stride, which a hook may change
+        ctx.how = _native.lib().mps_expert_route_grad, logits.dtype, logits.shape, top, code, normalize, scale
         return ids, weights
 
     @staticmethod
@@ -348,12 +358,15 @@ class _Route(torch.autograd.Function):
 
 def _route_grad(ctx, dweights):
     logits, ids, shares = ctx.saved_tensors
-    entry, kind, t, experts, stride, top, code, normalize, scale = ctx.how
-    if not dweights.is_contiguous():
-        dweights = dweights.contiguous()
+    entry, dtype, shape, top, code, normalize, scale = ctx.how
+    (t, experts), device, chosen = shape, dweights.device, dweights.shape
+    logits = _adjacent(_kept(logits, shape, dtype, device))
+    ids = _kept(ids, chosen, torch.int32, device).contiguous()
+    shares = _kept(shares, chosen, torch.float32, device).contiguous()
+    dweights = dweights.contiguous()
     dlogits = logits.new_empty((t, experts))
-    _call(logits.device, entry, logits.data_ptr(), kind, t, experts, stride, top, code, normalize, scale, ids.data_ptr(), shares.data_ptr(),
-          dweights.data_ptr(), dlogits.data_ptr())
+    _call(device, entry, logits.data_ptr(), _TYPES[dtype], t, experts, logits.stride(0), top, code, normalize, scale, ids.data_ptr(),
+          shares.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
     return dlogits
 
 
@@ -411,7 +424,7 @@ class _Balance(torch.autograd.Function):
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, kept)  # not the counts: a program may add up its ranks' in place
-        ctx.how = _native.lib().mps_expert_balance_grad, _TYPES[logits.dtype], *logits.shape, logits.stride(0), code
+        ctx.how = _native.lib().mps_expert_balance_grad, logits.dtype, logits.shape, code  # as in _Route
         return loss, counts
 
     @staticmethod
@@ -421,9 +434,13 @@ class _Balance(torch.autograd.Function):
 
 def _balance_grad(ctx, dloss):
     logits, kept = ctx.saved_tensors
-    entry, kind, t, experts, stride, code = ctx.how
+    entry, dtype, shape, code = ctx.how
+    (t, experts), device = shape, dloss.device
+    logits = _adjacent(_kept(logits, shape, dtype, device))
+    kept = _kept(kept, (experts + 1,), torch.int32, device).contiguous()
     dlogits = logits.new_empty((t, experts))
-    _call(logits.device, entry, logits.data_ptr(), kind, t, experts, stride, code, kept.data_ptr(), dloss.data_ptr(), dlogits.data_ptr())
+    _call(device, entry, logits.data_ptr(), _TYPES[dtype], t, experts, logits.stride(0), code, kept.data_ptr(), dloss.data_ptr(),
+          dlogits.data_ptr())
     return dlogits
 
 
