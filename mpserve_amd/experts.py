@@ -132,16 +132,28 @@ def _first_gradient(backward):
     return run
 
 
+def _kept(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A tensor that a forward pass saved. Autograd's saved-tensor hooks may give back other memory, laid out in another way (an
+    offload's copy of a slice of columns has its rows side by side); what has another size, type or device is refused: kernels
+    would read past its end."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"a saved-tensor hook gave back {tuple(t.shape)} {t.dtype} on {t.device} for what was saved as "
+                           f"{tuple(shape)} {dtype} on {device}")
+    return t
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order, positions, offsets):
         ctx.save_for_backward(positions)
+        ctx.how = positions.shape
         return _gather_rows(x, order, positions, offsets)
 
     @staticmethod
     @_first_gradient
     def backward(ctx, drows):
         (positions,) = ctx.saved_tensors
+        positions = _kept(positions, ctx.how, torch.int32, drows.device).contiguous()
         return _sum_rows(drows.contiguous(), None, positions), None, None, None
 
 
@@ -150,15 +162,22 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, y, weights, order, positions, offsets):
         # y is needed for the weights' gradient only
         ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, weights, order, positions, offsets)
+        ctx.how = weights.dtype, weights.shape, offsets.shape
         return _sum_rows(y, weights, positions)
 
     @staticmethod
     @_first_gradient
     def backward(ctx, dout):
         y, weights, order, positions, offsets = ctx.saved_tensors
-        t, top = weights.shape
+        weights_type, shape, ends = ctx.how
+        (t, top), device, i32 = shape, dout.device, torch.int32
         dout = dout.contiguous()
         width, dy, dweights = dout.shape[1], None, None
+        if y is not None:
+            y = _kept(y, (t * top, width), dout.dtype, device).contiguous()
+        weights = _kept(weights, shape, weights_type, device).contiguous()
+        order, positions = _kept(order, (t * top,), i32, device).contiguous(), _kept(positions, shape, i32, device).contiguous()
+        offsets = _kept(offsets, ends, i32, device).contiguous()
         if ctx.needs_input_grad[0]:
             dy = torch.empty((t * top, width), dtype=dout.dtype, device=dout.device)
         if ctx.needs_input_grad[1]:
@@ -296,16 +315,6 @@ def _check_logits(logits: torch.Tensor, scores: str) -> int:
 
 def _adjacent(logits: torch.Tensor) -> torch.Tensor:
     return logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
-
-
-def _kept(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A tensor that a forward pass saved. Autograd's saved-tensor hooks may give back other memory, laid out in another way (an
-    offload's copy of a slice of columns has its rows side by side); what has another size, type or device is refused: kernels
-    would read past its end."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise RuntimeError(f"a saved-tensor hook gave back {tuple(t.shape)} {t.dtype} on {t.device} for what was saved as "
-                           f"{tuple(shape)} {dtype} on {device}")
-    return t
 
 
 def _route(logits, top, code, bias, normalize, scale, shares):

@@ -79,6 +79,27 @@ def test_what_is_not_the_saved_tensor_is_refused(calls, call, change):
     assert len(calls) == before
 
 
+def test_combine_and_gather_take_what_hooks_give(calls):
+    t, top, width, num = 5, 2, 16, 4
+    order, positions, offsets = torch.zeros(t * top, dtype=torch.int32), torch.zeros(t, top, dtype=torch.int32), torch.zeros(num + 1, dtype=torch.int32)
+    apart = lambda v: v.t().contiguous().t() if v.dim() == 2 else v.repeat(2, 1).t().contiguous().t()[0]  # noqa: E731
+    y, weights, x = torch.randn(t * top, width).requires_grad_(), torch.rand(t, top).requires_grad_(), torch.randn(t, width).requires_grad_()
+    for change, fine in ((apart, True), (lambda v: v[:-1], False), (lambda v: v.to("meta"), False), (lambda v: v.half(), False)):
+        for call, leaves in ((lambda: experts._Combine.apply(y, weights, order, positions, offsets), (y, weights)),
+                             (lambda: experts._Gather.apply(x, order, positions, offsets), (x,))):
+            with Hooks(change) as hooks:
+                out = call()
+            before = len(calls)
+            if fine:
+                torch.autograd.grad(out, leaves, torch.ones_like(out))
+                given = {v.data_ptr() for v in hooks.given if not v.is_contiguous()}
+                assert given and not given & set(a for a in calls[-1][1] if isinstance(a, int) and a > 2 ** 20)
+            else:
+                with pytest.raises(RuntimeError, match="saved-tensor hook"):
+                    torch.autograd.grad(out, leaves, torch.ones_like(out))
+                assert len(calls) == before
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("scores,normalize", (("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)))
 def test_gradients_of_a_slice_that_is_kept_on_the_host(scores, normalize):
@@ -92,4 +113,19 @@ def test_gradients_of_a_slice_that_is_kept_on_the_host(scores, normalize):
             chosen = experts.expert_route(x, 4, scores=scores, normalize=normalize, scale=2.5)
             loss = experts.expert_balance(x, chosen.ids, scores=scores).loss
         got.append([torch.autograd.grad(out, x, dout)[0] for out, dout in ((chosen.weights, chosen.weights.detach() + 1), (loss, loss.detach()))])
+    assert all(torch.equal(a, b) and bool(a.any()) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+def test_experts_of_rows_that_are_kept_on_the_host():
+    t, top, width, num = 70, 3, 40, 8
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randint(-1, num, (t, top), generator=g).cuda()
+    x, weights = torch.randn(t, width, generator=g).cuda().requires_grad_(), torch.rand(t, top, generator=g).cuda().requires_grad_()
+    sort, dout = experts.expert_sort(ids, num), torch.randn(t, width, generator=g).cuda()
+    got = []
+    for hooks in (torch.autograd.graph.save_on_cpu(), contextlib.nullcontext()):
+        with hooks:
+            out = experts.expert_combine(experts.expert_gather(x, sort) * 2, weights, sort)
+        got.append(torch.autograd.grad(out, (x, weights), dout))
     assert all(torch.equal(a, b) and bool(a.any()) for a, b in zip(*got))
