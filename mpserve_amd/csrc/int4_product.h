@@ -13,7 +13,7 @@ struct Int4Args : ProductArgs {
   const void *scales;
   const uint8_t *zeros;  // nullptr: 8
   int32_t scale_type, groups, shift;  // groups a row; blocks a group, as a power of two
-  const void *sums;                   // many rows: x's sums over groups, `sums_row` bytes a row of x
+  const void *sums;                   // many rows: x's sums, `sums_row` bytes a row of x
   int64_t sums_row;
 };
 
@@ -64,6 +64,19 @@ __device__ inline u32x4 int4_values(uint32_t codes, float zero) {
 __device__ inline uint32_t lds_address(const uint8_t *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p; }
 __device__ inline void copy16_apart(const uint8_t *from, uint32_t to) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+}
+
+// An address that is alike for all lanes, in scalar registers.
+__device__ inline const uint8_t *scalar(const uint8_t *p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const uint8_t *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 |
+                                           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
+}
+
+// The same from `base`, alike for all lanes, and a lane's bytes behind it, which take one register. The base may come from a vector
+// instruction, behind which a load has to keep five instructions' distance: the compiler does not see that this is one.
+__device__ inline void copy16_apart(const uint8_t *base, uint32_t from, uint32_t to) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(__builtin_amdgcn_readfirstlane(to)), "v"(from), "s"(scalar(base)) : "memory");
 }
 
 // Eight ones: x times these is the sum of x.
@@ -137,10 +150,13 @@ __device__ inline void read_window(const Int4Args &a, const uint8_t *row, int32_
 Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus);
 void launch_int4_rows(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
 
-// Many rows (int4_tile.hip): x is 16-bit rows of whole blocks at 16-byte addresses, with its sums: 16 groups at a time, the
-// first eight bits (and sign) of each, the next eight and the rest as BF16, 32 bytes each; zeros past the last group.
+// Many rows (int4_tile.hip): x is 16-bit rows of whole blocks at 16-byte addresses, with its sums over spans of a group or, of a larger
+// one, 128 columns. A sum is three BF16 numbers, the first eight bits (and sign), the next eight and the rest. A row has first, second, third and
+// first again of each span; then the second ones by themselves; zeros past the last span, to a multiple of 16.
 Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus);
 void launch_int4_tiles(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
-inline int64_t sums_row_bytes(int32_t groups) { return (int64_t)(groups + 15) / 16 * 96; }
+inline int32_t sums_shift(const Int4Args &a) { return a.shift < 2 ? a.shift : 2; }
+inline int32_t sums_spans(const Int4Args &a) { return (int32_t)(((int64_t)a.row_blocks + (1 << sums_shift(a)) - 1) >> sums_shift(a)); }
+inline int64_t sums_row_bytes(const Int4Args &a) { return (int64_t)(sums_spans(a) + 15) / 16 * 160; }
 
 }  // namespace mps

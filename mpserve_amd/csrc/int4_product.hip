@@ -20,39 +20,38 @@ __global__ __launch_bounds__(256) void int4_pack_kernel(const uint16_t *__restri
   }
 }
 
-// The sums of x over groups, in FP32 by a tree, as three BF16 numbers; and x packed, if asked for. A wave takes 512 columns of a row,
-// or a group where that is more: eight a lane.
+// The sums of x over spans of 32 << shift columns, at most 128, in FP32 by a tree, as three BF16 numbers; and x packed, if asked for. A wave takes
+// 512 columns of a row, eight a lane.
 template <int XT>
-__global__ __launch_bounds__(256) void int4_sums_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride, int32_t k, int32_t groups,
+__global__ __launch_bounds__(256) void int4_sums_kernel(const uint16_t *__restrict__ x, int64_t rows, int64_t stride, int32_t k, int32_t spans,
                                                         int32_t shift, uint8_t *__restrict__ sums, int64_t sums_row, int32_t width,
                                                         uint16_t *__restrict__ packed) {
-  const int lane = threadIdx.x & 63;
-  const int32_t span = shift > 4 ? 32 << shift : 512, in_group = shift > 4 ? 64 : 4 << shift;  // columns a wave; lanes a group
-  const int32_t padded = (groups + 15) / 16 * 16, spans = (int32_t)((((int64_t)padded << shift) * 32 + span - 1) / span);
-  const int64_t units = rows * spans;
+  const int lane = threadIdx.x & 63, in_span = 4 << shift;  // lanes a span
+  const int32_t padded = (spans + 15) / 16 * 16, pieces = (padded << shift) / 16;
+  const int64_t units = rows * pieces;
   for (int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); unit < units; unit += (int64_t)gridDim.x * 4) {
-    const int64_t row = unit / spans;
-    const int64_t first = (unit - row * spans) * span;
-    const uint16_t *const from = x + row * stride;
+    const int64_t row = unit / pieces;
+    const int32_t piece = (int32_t)(unit - row * pieces), col = piece * 512 + lane * 8, span = piece * (16 >> shift) + lane / in_span;
     float sum = 0;
-    for (int64_t col = first + lane * 8; col < first + span && col - lane * 8 < width; col += 512) {
-      const u32x4 v = load_row8(from, col, k);
-      if (packed && col < width) *reinterpret_cast<u32x4 *>(packed + row * width + col) = v;
+    if (col < width) {
+      const u32x4 v = load_row8(x + row * stride, col, k);
+      if (packed) *reinterpret_cast<u32x4 *>(packed + row * width + col) = v;
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[2 * i] = Elem<XT>::get((uint16_t)v[i]), f[2 * i + 1] = Elem<XT>::get((uint16_t)(v[i] >> 16));
-      sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+      sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
     }
-    for (int d = 1; d < in_group; d *= 2) sum += __shfl_xor(sum, d);
-    const int32_t group = (int32_t)(first / 32 >> shift) + lane / in_group;
-    if (lane % in_group == 0 && group < padded) {
-      uint16_t *const to = reinterpret_cast<uint16_t *>(sums + row * sums_row + group / 16 * 96) + group % 16;
+    for (int d = 1; d < in_span; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane % in_span == 0) {
+      uint32_t p[3];
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        const uint16_t piece = Elem<MPS_TYPE_BF16>::put(sum);
-        to[16 * i] = piece;
-        sum -= Elem<MPS_TYPE_BF16>::get(piece);
+        p[i] = Elem<MPS_TYPE_BF16>::put(sum);
+        sum -= Elem<MPS_TYPE_BF16>::get((uint16_t)p[i]);
       }
+      uint8_t *const to = sums + row * sums_row;
+      *reinterpret_cast<uint64_t *>(to + span * 8) = (uint64_t)(p[2] | p[0] << 16) << 32 | (p[0] | p[1] << 16);
+      *reinterpret_cast<uint16_t *>(to + padded * 8 + span * 2) = (uint16_t)p[1];
     }
   }
 }
@@ -111,7 +110,7 @@ Way way_of(const mps_int4_product *p) {
   w.choice = w.tiles ? tiles.choice : rows.choice;
   w.packed = p->k > 0 && !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));
   if (w.packed) w.packed_bytes = a.x_rows * packed_width(p->k) * 2;
-  if (w.tiles) a.sums_row = sums_row_bytes(a.groups);
+  if (w.tiles) a.sums_row = sums_row_bytes(a);
   w.workspace = w.packed_bytes + a.x_rows * a.sums_row;
   return w;
 }
@@ -147,13 +146,13 @@ int mps_int4_multiply(const mps_int4_product *p, void *workspace, int64_t worksp
   const uint16_t *const x = static_cast<const uint16_t *>(p->x);
   if (way.tiles && k > 0) {
     uint8_t *const sums = static_cast<uint8_t *>(workspace) + way.packed_bytes;
-    const int64_t spans = ((int64_t)((a.groups + 15) / 16 * 16) << a.shift) / (a.shift > 4 ? 1 << a.shift : 16);
-    const dim3 grid(workgroups(((int64_t)a.x_rows * spans + 3) / 4));
+    const int32_t shift = sums_shift(a), spans = sums_spans(a);
+    const dim3 grid(workgroups(((int64_t)a.x_rows * (((spans + 15) / 16) << shift) + 3) / 4));
     if (p->x_type == MPS_TYPE_BF16)
-      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_BF16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, a.groups, a.shift, sums,
+      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_BF16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, spans, shift, sums,
                          a.sums_row, width, packed);
     else
-      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_F16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, a.groups, a.shift, sums,
+      hipLaunchKernelGGL(int4_sums_kernel<MPS_TYPE_F16>, grid, dim3(256), 0, s, x, (int64_t)a.x_rows, p->x_stride, k, spans, shift, sums,
                          a.sums_row, width, packed);
     a.sums = sums;
   } else if (way.packed) {

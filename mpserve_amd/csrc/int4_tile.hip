@@ -4,16 +4,19 @@
 // A step covers 64 elements of k: 128 bytes of every row of x, a cache line, and 32 of codes, which are widened in registers,
 // after LDS. A stage is two steps. Pieces of 16 bytes go from memory to a ring of three stages in LDS without passing through
 // registers; piece p of row r of x lies at place p ^ (r / 2 % 8), of codes at p ^ (r / 8 % 2), so that the sixteen lanes that
-// LDS serves in a cycle meet all banks. A step's fragments are read while the one before is multiplied, quarter by quarter.
+// LDS serves in a cycle meet all banks. A step's fragments are read two quarters of it ahead, among the products.
 // A stage's one barrier stands before its second step, for two things: the next stage has come, and nobody needs the one
 // before any more, whose fragments all have used, so that no wave waits there for reads of its own. (BF16, groups of 128, 4096 x 4096 x
-// 14336: loads and reads in a row behind the barrier 560 us, among the products 517; the zeros' product with its loads a chunk ahead 504.)
+// 14336: loads and reads in a row behind the barrier 560 us, among the products 500.)
 //
 // The matrix cores multiply x by the whole numbers q as they are. Products of columns that share a scale are summed by
-// themselves and added with the scale in FP32. What the zeros take away, sum over groups of s z sum x, is another
-// product, of the groups' sums of x and of s z, with which the sums begin: the sums of x (int4_sums_kernel) as three BF16
-// numbers, s z as two, which hold it exactly; of the six products the least is left out (2^-25 of the sums). Where a tile's
-// sums are not finite (x holds an infinity, or its sums pass 2^128) it makes them again from q - z.
+// themselves and added with the scale in FP32. What the zeros take away, sum over spans of s z sum x (a span is a group, at
+// most 128 columns), is another product, of the spans' sums of x and of s z: the sums of x (int4_sums_kernel) as three BF16
+// numbers, s z as two, which hold it exactly; of the six products the least is left out (2^-25 of the sums). It is taken away four spans at a
+// time, beside these spans' own products: no sum on the way is larger than the result and four spans' part. (All of it in front of the first
+// product is as fast, but where x has a mean every addition then rounds at the size of the whole: x of mean and sigma 1, 28672 columns, groups
+// of 128, results in FP32 off by 4.6e-6 of their size, so 3.8e-7.) Where a tile's sums are not finite (x holds an infinity, or its
+// sums pass 2^128) it makes them again from q - z.
 #include "int4_product.h"
 
 namespace mps {
@@ -35,8 +38,11 @@ struct Shape {
   static constexpr int kXBytes = kBT * 128, kStep = kXBytes + kBN * 32, kStage = 2 * kStep;
   static constexpr int kEntries = 8, kPeriod = C == kBlock ? 2 : 4;  // scales of a row in a period; stages a period
   static constexpr int kSBytes = kBN * kEntries * 2;
+  // Spans: their columns as a power of two of blocks; stages of four of them; bytes of all rows' four sums of x, and places for these.
+  static constexpr int kSpan = C == kBlock ? 0 : C == Chain::kStep ? 1 : 2, kFour = 1 << kSpan, kFourBytes = kBT * 32, kFours = C == kBlock ? 2 : 1;
+  static constexpr int kAhead = 2;  // quarters of a step by which x is read ahead
   static constexpr int kPitch = 32 * FN + 4;  // floats of a row of sums, turned round
-  static constexpr int kStaged = kStages * kStage + 2 * kSBytes, kTurned = kWaves * 32 * kPitch * 4;
+  static constexpr int kStaged = kStages * kStage + 2 * kSBytes + kFours * kFourBytes, kTurned = kWaves * 32 * kPitch * 4;
   static constexpr int kLds = kStaged > kTurned ? kStaged : kTurned;
   static_assert(kBT * 8 % kThreads == 0 && kLds <= 160 * 1024 && kBN <= kThreads, "");
 };
@@ -53,7 +59,7 @@ template <int XT, Chain C, int FT, int FN, int WT, int WN>
 __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void int4_tile_kernel(Int4Args a, int32_t tiles_t, int32_t tiles_n) {
   typedef Shape<C, FT, FN, WT, WN> H;
   __shared__ __attribute__((aligned(16))) uint8_t lds[H::kLds];
-  uint8_t *const ss = lds + kStages * H::kStage;
+  uint8_t *const ss = lds + kStages * H::kStage, *const xs = ss + 2 * H::kSBytes;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, g = lane >> 5;
   const int wt = wave / WN, wn = wave % WN;
 
@@ -69,6 +75,7 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
 
   Tile tile = {0, tile_t * H::kBT, min(a.rows, tile_t * H::kBT + H::kBT)};
   if (a.offsets) tile = find_tile(a.offsets, a.experts, a.rows, H::kBT, tile_t);
+  tile = {__builtin_amdgcn_readfirstlane(tile.expert), __builtin_amdgcn_readfirstlane(tile.first), __builtin_amdgcn_readfirstlane(tile.end)};
   if (tile.expert < 0) return;
   const bool none = tile.expert >= max(a.experts, 1);  // rows of no expert
   const int32_t blocks = none ? 0 : a.row_blocks, pairs = (blocks + 3) / 4;  // of steps
@@ -89,25 +96,30 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
     x_from[i] = static_cast<const uint8_t *>(a.x) + row_of(xrow + i * (H::kThreads / 8)) * a.x_stride * 2 + x_piece;
   const int64_t w_first = (int64_t)(none ? 0 : tile.expert) * a.n + n0;
   const int32_t last_col = a.n - 1 - n0;
-  const uint8_t *w_from[H::kWLoads];
+  const uint8_t *const w_base = scalar(a.w + w_first * a.row_blocks * 16);
+  uint32_t w_from[H::kWLoads];  // from there on: below 256 rows of 2^23 bytes
 #pragma unroll
-  for (int i = 0; i < H::kWLoads; ++i) w_from[i] = a.w + (w_first + min(wrow + i * (H::kThreads / 2), last_col)) * a.row_blocks * 16;
+  for (int i = 0; i < H::kWLoads; ++i) w_from[i] = (uint32_t)min(wrow + i * (H::kThreads / 2), last_col) * (uint32_t)(a.row_blocks * 16) + w_piece;
   // Load l of a stage, to `to` in LDS. The stages at a row's end may be parts of one or none at all: x's pieces past
   // its end are zeros, the codes' what they are.
   const uint32_t lds_at = lds_address(lds) + wave * 1024, w_lds_at = lds_address(lds) + H::kXBytes + wave * H::kWLanes * 16;
-  auto fetch = [&](int32_t pair, uint32_t to, int l, auto whole) {
+  auto fetch = [&](int32_t pair, uint32_t to, int l, auto whole) __attribute__((always_inline)) {
     const int h = l / (H::kLoads / 2), i = l % (H::kLoads / 2);
+    asm volatile("" : "+s"(pair));  // lest every load of an unrolled period gets an address of its own to count up
     if (i < H::kXLoads) {
       const uint32_t at = pair * 256 + h * 128;
       const uint8_t *from = x_from[i] + at;
       if (!decltype(whole)::value) from = at + x_piece < x_end ? from : reinterpret_cast<const uint8_t *>(kNothing);
       copy16_apart(from, lds_at + to + h * H::kStep + i * H::kThreads * 16);
     } else if (H::kWLanes == 64 || lane < H::kWLanes) {
-      const uint32_t at = pair * 64 + h * 32 + w_piece;
-      copy16_apart(w_from[i - H::kXLoads] + (decltype(whole)::value ? at : min(at, w_last)), w_lds_at + to + h * H::kStep + (i - H::kXLoads) * H::kThreads * 16);
+      const uint32_t at = pair * 64 + h * 32, lds_to = w_lds_at + to + h * H::kStep + (i - H::kXLoads) * H::kThreads * 16;
+      if (decltype(whole)::value)
+        copy16_apart(w_base + at, w_from[i - H::kXLoads], lds_to);
+      else
+        copy16_apart(w_base, w_from[i - H::kXLoads] - w_piece + min(at + w_piece, w_last), lds_to);
     }
   };
-  auto fetch_all = [&](int32_t pair, uint32_t to) {
+  auto fetch_all = [&](int32_t pair, uint32_t to) __attribute__((always_inline)) {
 #pragma unroll
     for (int l = 0; l < H::kLoads; ++l) fetch(pair, to, l, std::false_type{});
   };
@@ -118,9 +130,13 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
   // A row that has fewer in all has them in both buffers from the start.
   uint32_t scales[H::kEntries / 2] = {};
   const bool turns = a.groups >= H::kEntries, has_scales = tid < H::kBN;
-  const uint16_t *const s_row = static_cast<const uint16_t *>(a.scales) + (w_first + min(tid, min(H::kBN - 1, last_col))) * a.groups;
+  const uint8_t *const s_first = scalar(static_cast<const uint8_t *>(a.scales) + w_first * a.groups * 2);
   auto get_scales = [&](int32_t period) {
-    if (has_scales) __builtin_memcpy(scales, s_row + scales_start(period), sizeof(scales));
+    if (has_scales) {
+      uint32_t row = min(tid, last_col);
+      asm volatile("" : "+v"(row));
+      __builtin_memcpy(scales, s_first + (row * (uint32_t)a.groups + (uint32_t)scales_start(period)) * 2, sizeof(scales));
+    }
   };
   auto put_scales = [&](int32_t period) {
     u32x4 *const to = reinterpret_cast<u32x4 *>(ss + (period & 1) * H::kSBytes + tid * H::kEntries * 2);
@@ -135,12 +151,12 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
   // Lanes 0-31 and 32-63 take a half each of a step's 64 elements: of either block where blocks have scales of their
   // own, else a block. Quarter q is eight elements of each half.
   f32x16 acc[FT][FN] = {}, part[FT][FN] = {};
-  u32x4 fx[4][FT];
+  u32x4 fx[H::kAhead][FT];
   uint32_t fw[2][FN][4];  // of even and odd steps
   u32x4 w0[FN], w1[FN];   // widened: of the even and the odd quarter
   const int x_lane = (wt * FT * 32 + r) * 128, w_lane = (wn * FN * 32 + r) * 32;
   auto x_place = [&](int q) -> int { return ((C == kBlock ? 4 * (q >> 1) + 2 * g + (q & 1) : 4 * g + q) ^ (r >> 1 & 7)) * 16 + x_lane; };
-  auto read_x = [&](int q, int t, uint32_t at) { fx[q][t] = *reinterpret_cast<const u32x4 *>(lds + at + x_place(q) + t * 4096); };
+  auto read_x = [&](int q, int t, uint32_t at) { fx[q % H::kAhead][t] = *reinterpret_cast<const u32x4 *>(lds + at + x_place(q) + t * 4096); };
   auto read_w = [&](uint32_t (&to)[FN][4], uint32_t at) {
     const uint8_t *const from = lds + at + H::kXBytes + w_lane;
 #pragma unroll
@@ -162,6 +178,41 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
   int64_t cols[FN];
 #pragma unroll
   for (int n = 0; n < FN; ++n) cols[n] = w_first + min((wn * FN + n) * 32 + r, last_col);
+  // What the zeros take away, four sums of x at a time, which come to LDS ahead; the zeros a period ahead to registers, a column's
+  // kEntries as its scales. Addresses are made each time: registers are what the largest tiles lack.
+  const int32_t sum_row = pairs > 0 && tid < 2 * H::kBT ? row_of(tid / 2) : 0;
+  const uint8_t *const z_first = scalar(a.zeros + w_first * a.groups);
+  uint32_t zeros[FN][2];
+  auto get_sums = [&](int32_t four) {
+    if (wave < H::kBT / 32) {
+      int32_t row = sum_row;
+      asm volatile("" : "+v"(row));
+      copy16_apart(static_cast<const uint8_t *>(a.sums) + row * a.sums_row + (four * 32 + lane % 2 * 16), lds_address(xs) + four % H::kFours * H::kFourBytes + wave * 1024);
+    }
+  };
+  auto get_zeros = [&](int32_t period) {
+#pragma unroll
+    for (int n = 0; n < FN; ++n) {
+      uint32_t col = min((wn * FN + n) * 32 + r, last_col);
+      asm volatile("" : "+v"(col));
+      __builtin_memcpy(zeros[n], z_first + col * (uint32_t)a.groups + (uint32_t)scales_start(period), 8);
+    }
+  };
+  auto read_sums = [&](int32_t four, int t) -> u32x4 {
+    return *reinterpret_cast<const u32x4 *>(xs + four % H::kFours * H::kFourBytes + ((wt * FT + t) * 32 + r) * 32 + g * 16);
+  };
+  // This lane's two spans of the four: their scales, and minus s z, its first eight bits and above them what these leave.
+  auto four_entry = [&](int32_t four, int j) -> int32_t {
+    return (min((4 * four + 2 * g + j) << H::kSpan, blocks - 1) >> a.shift) - scales_start(four * H::kFour / H::kPeriod);
+  };
+  auto read_scale = [&](int32_t four, int n, int j) -> uint32_t {
+    return *reinterpret_cast<const uint16_t *>(ss + (four * H::kFour / H::kPeriod & 1) * H::kSBytes + ((wn * FN + n) * 32 + r) * H::kEntries * 2 + four_entry(four, j) * 2);
+  };
+  auto scaled_zero = [&](int32_t four, int n, int j, uint32_t scale) -> uint32_t {
+    const uint32_t zero = __builtin_amdgcn_perm(zeros[n][1], zeros[n][0], 0x0c0c0c00u | (uint32_t)four_entry(four, j)) & 31;
+    const float f = -scale_value(scale, a.scale_type) * (float)zero;
+    return pack2(f, f - Elem<MPS_TYPE_BF16>::get(Elem<MPS_TYPE_BF16>::put(f)), MPS_TYPE_BF16);
+  };
   if (pairs > 0) {
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) fetch_all(i, i * H::kStage);
@@ -170,106 +221,64 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
     } else {
       uint16_t few[H::kEntries];
 #pragma unroll
-      for (int i = 0; i < H::kEntries; ++i) few[i] = s_row[min(i, a.groups - 1)];
+      for (int i = 0; i < H::kEntries; ++i)
+        few[i] = reinterpret_cast<const uint16_t *>(s_first)[(uint32_t)min(min(tid, H::kBN - 1), last_col) * (uint32_t)a.groups + (uint32_t)min(i, a.groups - 1)];
 #pragma unroll
       for (int i = 0; i < H::kEntries / 2; ++i) scales[i] = few[2 * i] | (uint32_t)few[2 * i + 1] << 16;
     }
-    // What the zeros take away: 16 groups at a time.
-    const uint8_t *sums[FT];
+    get_sums(0);
+    if (!a.zeros) {
 #pragma unroll
-    for (int t = 0; t < FT; ++t) sums[t] = static_cast<const uint8_t *>(a.sums) + (int64_t)row_of((wt * FT + t) * 32 + r) * a.sums_row + g * 16;
-    struct Chunk {
-      uint32_t s[FN][4], z[FN][2];
-      u32x4 x[FT][3];
-    };
-    auto get_chunk = [&](int32_t c, Chunk &k) {
+      for (int n = 0; n < FN; ++n) zeros[n][0] = zeros[n][1] = 0x08080808u;
+    } else if (turns) {
+      get_zeros(0);
+    } else {
 #pragma unroll
       for (int n = 0; n < FN; ++n) {
-        const int64_t from = cols[n] * a.groups;
-        const uint16_t *const s = static_cast<const uint16_t *>(a.scales) + from;
-        k.z[n][0] = k.z[n][1] = 0x08080808u;
-        if (c + 16 <= a.groups) {
-          __builtin_memcpy(k.s[n], s + c + 8 * g, 16);
-          if (a.zeros) __builtin_memcpy(k.z[n], a.zeros + from + c + 8 * g, 8);
-        } else {  // without branches among the loads, so that they are in flight together
-          uint32_t e[8], f[8];
+        uint32_t e[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = s[min(c + 8 * g + i, a.groups - 1)];
+        for (int i = 0; i < 8; ++i) e[i] = z_first[(uint32_t)min((wn * FN + n) * 32 + r, last_col) * (uint32_t)a.groups + (uint32_t)min(i, a.groups - 1)];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + 8 * g + i >= a.groups) e[i] = 0;  // a scale of 0.0
-#pragma unroll
-          for (int i = 0; i < 4; ++i) k.s[n][i] = e[2 * i] | e[2 * i + 1] << 16;
-          if (a.zeros) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = a.zeros[from + min(c + 8 * g + i, a.groups - 1)];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) k.z[n][i] = f[4 * i] | f[4 * i + 1] << 8 | f[4 * i + 2] << 16 | f[4 * i + 3] << 24;
-          }
-        }
+        for (int i = 0; i < 2; ++i) zeros[n][i] = e[4 * i] | e[4 * i + 1] << 8 | e[4 * i + 2] << 16 | e[4 * i + 3] << 24;
       }
-#pragma unroll
-      for (int t = 0; t < FT; ++t)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) k.x[t][i] = *reinterpret_cast<const u32x4 *>(sums[t] + c / 16 * 96 + i * 32);
-    };
-    Chunk now, soon;
-    get_chunk(0, now);
-    for (int32_t c = 0; c < a.groups; c += 16) {
-      if (c + 16 < a.groups) get_chunk(c + 16, soon);
-      u32x4 hi[FN], lo[FN];
-#pragma unroll
-      for (int n = 0; n < FN; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t z = now.z[n][i / 2] >> (16 * (i % 2)) & 0x1f1f;
-          const float f0 = -scale_value(now.s[n][i] & 0xffff, a.scale_type) * (float)(z & 255), f1 = -scale_value(now.s[n][i] >> 16, a.scale_type) * (float)(z >> 8);
-          hi[n][i] = pack2(f0, f1, MPS_TYPE_BF16);
-          lo[n][i] = pack2(f0 - __uint_as_float(hi[n][i] << 16), f1 - __uint_as_float(hi[n][i] & 0xffff0000u), MPS_TYPE_BF16);
-        }
-#pragma unroll
-      for (int t = 0; t < FT; ++t)
-#pragma unroll
-        for (int n = 0; n < FN; ++n) {
-          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][2], hi[n], acc[t][n]);
-          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][1], lo[n], acc[t][n]);
-          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][1], hi[n], acc[t][n]);
-          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][0], lo[n], acc[t][n]);
-          acc[t][n] = mfma32<MPS_TYPE_BF16>(now.x[t][0], hi[n], acc[t][n]);
-        }
-      now = soon;
     }
     put_scales(0);
     if (!turns) put_scales(1);
-    if (turns && H::kPeriod < pairs) get_scales(1);
+    if (H::kPeriod == 2 && turns && H::kPeriod < pairs) get_scales(1);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < H::kAhead; ++q)
 #pragma unroll
       for (int t = 0; t < FT; ++t) read_x(q, t, 0);
     read_w(fw[0], 0);
 #pragma unroll
     for (int n = 0; n < FN; ++n) w0[n] = int4_codes<XT>(fw[0][n][0]);
   }
-  // Where this stage, the next and the one after it lie, and the stage at which scales are turned.
+  // Where this stage, the next and the one after it lie.
   uint32_t here = 0, then = H::kStage, after = 2 * H::kStage;
-  int32_t turn = turns && H::kPeriod < pairs ? H::kPeriod - 2 : INT32_MAX;
   // A step. The fragments' products come in an order in which, where another scale begins, the 16 multiply-adds a lane that
   // add what has been summed with the last one stand beside two products each. Between two products there is room for
   // a read of the next step's fragments, a load of the stage after the next, or the widening of a quarter's codes.
-  auto body = [&](int32_t pair, auto odd, auto whole) {
-    constexpr int kOdd = decltype(odd)::value, kM = FT * FN;
+  // `known`: the stage's place in its period, or -1, which makes it be asked for.
+  auto body = [&](int32_t pair, auto odd, auto whole, auto known) __attribute__((always_inline)) {
+    constexpr int kOdd = decltype(odd)::value, kM = FT * FN, kKnown = decltype(known)::value;
+    constexpr int kMade = FT == 1 ? 1 : 2;  // products behind which s z is made, from scales read behind the first
+    const int32_t place = kKnown >= 0 ? kKnown : pair % H::kPeriod;
     if constexpr (kOdd == 1) {
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-      if (__builtin_expect(pair == turn, 0)) {
+      if (place == H::kPeriod - 2 && turns && pair + 2 < pairs) {
         const int32_t period = pair / H::kPeriod + 1;  // the next one
         put_scales(period);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const bool more = (period + 1) * H::kPeriod < pairs;
-        if (more) get_scales(period + 1);
-        turn = more ? turn + H::kPeriod : INT32_MAX;
       }
+#pragma unroll
+      for (int n = 0; n < FN; ++n) asm volatile("" : "+v"(zeros[n][0]), "+v"(zeros[n][1]));  // here the wait for them costs nothing
     }
+    // The first stage of four spans takes away what their zeros do, among the odd step's products.
+    const bool takes = kOdd && place % H::kFour == 0;
+    const int32_t four = pair / H::kFour;
+    u32x4 sums[FT];
+    uint32_t sz[FN][2];
     const uint32_t next = kOdd ? then : here + H::kStep;
     int load = 0;
 #pragma unroll
@@ -291,12 +300,12 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
           for (int j = 0; j < 16; ++j) acc[t][n][j] = __builtin_fmaf(pending[n], part[t][n][j], acc[t][n][j]);
           asm volatile("" : "+v"(acc[t][n]));  // the sums stay where they are
           __builtin_amdgcn_sched_barrier(0);
-          part[t][n] = mfma32<XT>(fx[q][t], w0[n], f32x16{});
+          part[t][n] = mfma32<XT>(fx[q % H::kAhead][t], w0[n], f32x16{});
         } else {
-          part[t][n] = mfma32<XT>(fx[q][t], second ? w1[n] : w0[n], part[t][n]);
+          part[t][n] = mfma32<XT>(fx[q % H::kAhead][t], second ? w1[n] : w0[n], part[t][n]);
         }
         asm volatile("" : "+v"(part[t][n]));
-        if (n == FN - 1) read_x(q, t, next);
+        if (n == FN - 1) read_x((q + H::kAhead) % 4, t, q + H::kAhead < 4 ? here + kOdd * H::kStep : next);
         if (s == 0) {
 #pragma unroll
           for (int m = 0; m < FN; ++m) w1[m] = int4_codes<XT>(fw[kOdd][m][2 * h + 1]);
@@ -306,7 +315,41 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
           for (int m = 0; m < FN; ++m) w0[m] = int4_codes<XT>(h == 0 ? fw[kOdd][m][2] : fw[kOdd ^ 1][m][0]);
         }
-        if (kOdd == 1 && load < H::kLoads) fetch(pair + 2, after, load++, whole);
+        if (kOdd == 1) {
+          const int slot = 2 * kM * h + s;
+          if (load < H::kLoads) fetch(pair + 2, after, load++, whole);
+          if (takes) {
+            if (slot == 0 || slot == kMade) {
+#pragma unroll
+              for (int m = 0; m < FN; ++m)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) sz[m][j] = slot == 0 ? read_scale(four, m, j) : scaled_zero(four, m, j, sz[m][j]);
+            }
+#pragma unroll
+            for (int u = 0; u < FT; ++u) {
+              // all sums at once, or where registers lack one after the other
+              if (slot == (FT <= 2 ? 0 : 3 * u + 1)) sums[u] = read_sums(four, u);
+              if (slot == (FT <= 2 ? 2 * kM + u : 3 * u + 3)) {
+#pragma unroll
+                for (int m = 0; m < FN; ++m) {
+                  const uint32_t s0 = sz[m][0], s1 = sz[m][1];
+                  acc[u][m] = mfma32<MPS_TYPE_BF16>(sums[u], u32x4{s0 & 0xffff0000u, 0, s1 & 0xffff0000u, 0}, acc[u][m]);
+                  acc[u][m] = mfma32<MPS_TYPE_BF16>(sums[u], u32x4{s0 << 16 | (s0 & 0xffffu), s0, s1 << 16 | (s1 & 0xffffu), s1}, acc[u][m]);
+                  asm volatile("" : "+v"(acc[u][m]));
+                }
+              }
+            }
+          }
+          if (slot == kMade + 1 && (kKnown >= 0 || pair + 1 < pairs)) {
+            if ((place + 1) % H::kFour == 0) get_sums(four + 1);
+            if (place + 1 == H::kPeriod && turns && a.zeros) get_zeros((pair + 1) / H::kPeriod);
+          }
+          // A stage before put_scales; a period of two stages has that in its first, so these are the one's after the next.
+          if (slot == (FT == 1 ? 3 : 4) && place == 1 && turns) {
+            const int32_t period = pair / H::kPeriod + (H::kPeriod == 4 ? 1 : 2);
+            if (period * H::kPeriod < pairs) get_scales(period);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       if (fresh) {
@@ -321,15 +364,23 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
     }
   };
   int32_t pair = 0;
+  auto stage = [&](int32_t pair, auto known) __attribute__((always_inline)) {
+    body(pair, std::integral_constant<int, 0>{}, std::true_type{}, known);
+    body(pair, std::integral_constant<int, 1>{}, std::true_type{}, known);
+  };
 #pragma unroll 1
-  for (; 4 * pair + 12 <= blocks; ++pair) {  // the stage after the next is a whole one
-    body(pair, std::integral_constant<int, 0>{}, std::true_type{});
-    body(pair, std::integral_constant<int, 1>{}, std::true_type{});
+  for (; 4 * (pair + H::kPeriod) + 8 <= blocks; pair += H::kPeriod) {  // the stages after their next are whole ones
+    stage(pair, std::integral_constant<int, 0>{});
+    stage(pair + 1, std::integral_constant<int, 1>{});
+    if constexpr (H::kPeriod == 4) {
+      stage(pair + 2, std::integral_constant<int, 2>{});
+      stage(pair + 3, std::integral_constant<int, 3>{});
+    }
   }
 #pragma unroll 1
   for (; pair < pairs; ++pair) {
-    body(pair, std::integral_constant<int, 0>{}, std::false_type{});
-    body(pair, std::integral_constant<int, 1>{}, std::false_type{});
+    body(pair, std::integral_constant<int, 0>{}, std::false_type{}, std::integral_constant<int, -1>{});
+    body(pair, std::integral_constant<int, 1>{}, std::false_type{}, std::integral_constant<int, -1>{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the last stage
   bool finite = true;
@@ -360,31 +411,33 @@ __global__ __launch_bounds__(64 * WT * WN) __attribute__((amdgpu_waves_per_eu(2,
       __syncthreads();
       fetch_all(step / 2, 0);
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int t = 0; t < FT; ++t) read_x(q, t, at_step);
       read_w(fw[0], at_step);
 #pragma unroll
       for (int h = 0; h < (C == kBlock ? 2 : 1); ++h) {
         if (2 * step + h >= blocks) break;
         const int32_t at = (2 * step + h) >> a.shift;
 #pragma unroll
-        for (int n = 0; n < FN; ++n) {
-          const float s = int4_scale(a, cols[n], at), zero = int4_zero(a, cols[n], at);
+        for (int n = 0; n < FN; ++n)
 #pragma unroll
           for (int t = 0; t < FT; ++t) part[t][n] = f32x16{};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (C == kBlock && q / 2 != h) continue;
-            const u32x4 w = int4_values<XT>(fw[0][n][q], zero);
+        for (int q = C == kBlock ? 2 * h : 0; q < (C == kBlock ? 2 * h + 2 : 4); ++q) {
 #pragma unroll
-            for (int t = 0; t < FT; ++t) part[t][n] = mfma32<XT>(fx[q][t], w, part[t][n]);
+          for (int t = 0; t < FT; ++t) read_x(q, t, at_step);
+#pragma unroll
+          for (int n = 0; n < FN; ++n) {
+            const u32x4 w = int4_values<XT>(fw[0][n][q], int4_zero(a, cols[n], at));
+#pragma unroll
+            for (int t = 0; t < FT; ++t) part[t][n] = mfma32<XT>(fx[q % H::kAhead][t], w, part[t][n]);
           }
+        }
+#pragma unroll
+        for (int n = 0; n < FN; ++n) {
+          const float scale = int4_scale(a, cols[n], at);
 #pragma unroll
           for (int t = 0; t < FT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[t][n][i] = __builtin_fmaf(s, part[t][n][i], acc[t][n][i]);
+            for (int i = 0; i < 16; ++i) acc[t][n][i] = __builtin_fmaf(scale, part[t][n][i], acc[t][n][i]);
         }
       }
     }
@@ -431,20 +484,23 @@ void launch(const Int4Args &a, hipStream_t stream) {
 }
 
 // The tiles, in microseconds: `start` is what a tile takes at any k, `few` and `full` what k = 4096 adds to a tile that has a
-// CU to itself, on a card with few of them and a full one, and `many` to each of several. Groups of 64 and of 32 cost more. The four in turn take, of groups of 128 (rows x k x n): 96 x
-// 4096 x 14336 59, 43, 35, 34; 256 x 4096 x 4096 52, 36, 26, 23; 256 x 4096 x 14336 59, 45, 45, 58; 1024 x 4096 x 14336 129, 158, 145,
-// 190; 4096 x 4096 x 14336 461, 563, 548, 710; of groups of 32, FP16, 1024 x 8192 x 28672 904, 829, 795, 1037.
+// CU to itself, on a card with few of them and a full one, and `many` to each of several. Groups of 64 and of 32 cost more, and the first is not
+// for groups of 32. The four in turn take, of groups of 128 (rows x k x n): 96 x 4096 x 14336 60, 43, 35, 35; 256 x 4096 x 4096 53, 34, 27, 23;
+// 256 x 4096 x 14336 61, 47, 48, 63; 1024 x 4096 x 14336 143, 180, 163, 207; 4096 x 4096 x 14336 505, 610, 594, 769; of 64, 4096 x 4096 x 14336 594,
+// 681, 685, 885; of 32, 256 x 4096 x 14336 -, 65, 67, 90; 1024 x 8192 x 28672 (FP16) -, 828, 842, 1122.
 struct Choice {
   int32_t bt, bn;
   float start, few, full, many, step, block;
 };
-constexpr Choice kChoices[] = {{128, 256, 9.0f, 42.0f, 58.0f, 63.0f, 1.15f, 1.75f}, {64, 256, 7.0f, 25.0f, 41.0f, 34.4f, 1.15f, 1.5f},
-                               {64, 128, 6.0f, 18.0f, 30.0f, 15.8f, 1.15f, 1.45f}, {32, 128, 5.0f, 16.0f, 18.5f, 8.5f, 1.15f, 1.5f}};
+constexpr Choice kChoices[] = {{128, 256, 9.0f, 42.0f, 58.0f, 63.0f, 1.15f, 0.0f}, {64, 256, 7.0f, 25.0f, 41.0f, 34.4f, 1.15f, 1.55f},
+                               {64, 128, 6.0f, 18.0f, 30.0f, 15.8f, 1.15f, 1.7f}, {32, 128, 5.0f, 16.0f, 18.5f, 8.5f, 1.15f, 1.5f}};
 
 template <int XT, Chain C>
 void launch_chain(const Int4Args &a, int choice, hipStream_t stream) {
   switch (choice) {
-    case 0: return launch<XT, C, 4, 1, 1, 8>(a, stream);
+    case 0:
+      if constexpr (C != kBlock) launch<XT, C, 4, 1, 1, 8>(a, stream);  // whose sums' two places LDS has no room for
+      return;
     case 1: return launch<XT, C, 2, 1, 1, 8>(a, stream);
     case 2: return launch<XT, C, 2, 1, 1, 4>(a, stream);
     default: return launch<XT, C, 1, 1, 1, 4>(a, stream);
@@ -467,6 +523,7 @@ Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus) {
   int i = 0;
   for (const Choice &c : kChoices) {
     const int at = i++;
+    if (at == 0 && a.shift == 0) continue;
     if (((double)product_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) + 8) * 512 > kMostWorkItems) continue;
     const double tiles = expected_tiles(a, c.bt) * (double)((a.n + c.bn - 1) / c.bn) / cus;
     const double k = a.row_blocks / 128.0 * (a.shift == 0 ? c.block : a.shift == 1 ? c.step : 1.0f);
