@@ -132,14 +132,14 @@ def _first_gradient(backward):
     return run
 
 
-def _kept(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """A tensor that a forward pass saved. Autograd's saved-tensor hooks may give back other memory, laid out in another way (an
-    offload's copy of a slice of columns has its rows side by side); what has another size, type or device is refused: kernels
-    would read past its end."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
+def _kept(t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device, rows: bool = False) -> torch.Tensor:
+    """A tensor that a forward pass saved, contiguous, or with ``rows`` as rows that may lie apart. Autograd's saved-tensor hooks may give
+    back other memory, laid out in another way (an offload's copy of a slice of columns has its rows side by side); what has
+    another size, type or device is refused: kernels would read past its end."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
         raise RuntimeError(f"a saved-tensor hook gave back {tuple(t.shape)} {t.dtype} on {t.device} for what was saved as "
                            f"{tuple(shape)} {dtype} on {device}")
-    return t
+    return t if t.is_contiguous() or (rows and (t.stride(1) == 1 or t.shape[1] == 1)) else t.contiguous()
 
 
 class _Gather(torch.autograd.Function):
@@ -153,7 +153,7 @@ class _Gather(torch.autograd.Function):
     @_first_gradient
     def backward(ctx, drows):
         (positions,) = ctx.saved_tensors
-        positions = _kept(positions, ctx.how, torch.int32, drows.device).contiguous()
+        positions = _kept(positions, ctx.how, torch.int32, drows.device)
         return _sum_rows(drows.contiguous(), None, positions), None, None, None
 
 
@@ -174,10 +174,10 @@ class _Combine(torch.autograd.Function):
         dout = dout.contiguous()
         width, dy, dweights = dout.shape[1], None, None
         if y is not None:
-            y = _kept(y, (t * top, width), dout.dtype, device).contiguous()
-        weights = _kept(weights, shape, weights_type, device).contiguous()
-        order, positions = _kept(order, (t * top,), i32, device).contiguous(), _kept(positions, shape, i32, device).contiguous()
-        offsets = _kept(offsets, ends, i32, device).contiguous()
+            y = _kept(y, (t * top, width), dout.dtype, device)
+        weights = _kept(weights, shape, weights_type, device)
+        order, positions = _kept(order, (t * top,), i32, device), _kept(positions, shape, i32, device)
+        offsets = _kept(offsets, ends, i32, device)
         if ctx.needs_input_grad[0]:
             dy = torch.empty((t * top, width), dtype=dout.dtype, device=dout.device)
         if ctx.needs_input_grad[1]:
@@ -369,10 +369,11 @@ def _route_grad(ctx, dweights):
     logits, ids, shares = ctx.saved_tensors
     entry, dtype, shape, top, code, normalize, scale = ctx.how
     (t, experts), device, chosen = shape, dweights.device, dweights.shape
-    logits = _adjacent(_kept(logits, shape, dtype, device))
-    ids = _kept(ids, chosen, torch.int32, device).contiguous()
-    shares = _kept(shares, chosen, torch.float32, device).contiguous()
-    dweights = dweights.contiguous()
+    logits = _kept(logits, shape, dtype, device, True)
+    ids = _kept(ids, chosen, torch.int32, device)
+    shares = _kept(shares, chosen, torch.float32, device)
+    if not dweights.is_contiguous():
+        dweights = dweights.contiguous()
     dlogits = logits.new_empty((t, experts))
     _call(device, entry, logits.data_ptr(), _TYPES[dtype], t, experts, logits.stride(0), top, code, normalize, scale, ids.data_ptr(),
           shares.data_ptr(), dweights.data_ptr(), dlogits.data_ptr())
@@ -445,8 +446,8 @@ def _balance_grad(ctx, dloss):
     logits, kept = ctx.saved_tensors
     entry, dtype, shape, code = ctx.how
     (t, experts), device = shape, dloss.device
-    logits = _adjacent(_kept(logits, shape, dtype, device))
-    kept = _kept(kept, (experts + 1,), torch.int32, device).contiguous()
+    logits = _kept(logits, shape, dtype, device, True)
+    kept = _kept(kept, (experts + 1,), torch.int32, device)
     dlogits = logits.new_empty((t, experts))
     _call(device, entry, logits.data_ptr(), _TYPES[dtype], t, experts, logits.stride(0), code, kept.data_ptr(), dloss.data_ptr(),
           dlogits.data_ptr())
