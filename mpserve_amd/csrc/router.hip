@@ -592,7 +592,8 @@ __global__ __launch_bounds__(kSumThreads) void expert_balance_sum_kernel(Balance
   finish_balance<kSumThreads, 16>(a, blocks, a.sums, a.parts, work);
 }
 
-// dlogit[t, e] = dloss experts / (N T) p (counts[e] - sum_j counts[j] p[t, j]) (1 - sigmoid, for sigmoids).
+// dlogit[t, e] = dloss experts / (N T) p (counts[e] - sum_j counts[j] p[t, j]) (1 - sigmoid, for sigmoids). The p of a row add up to 1, so
+// that counts serve less their mean, too: loads that are nearly alike, which the loss is for, would else lose the digits that they share.
 template <int T, int L, int V, bool kSigmoid>
 __global__ __launch_bounds__(kRouteThreads) void expert_balance_grad_kernel(BalanceArgs a) {
   typedef typename Elem<T>::raw raw;
@@ -606,13 +607,13 @@ __global__ __launch_bounds__(kRouteThreads) void expert_balance_grad_kernel(Bala
   float soon[V];  // the next row's logits, which are loaded meanwhile
   if (t0 < a.tokens) load(t0, soon);
   float count[V];
+  int32_t whole[V];
   double n = 0;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int32_t e = in_row * V + j, c = e < a.experts ? a.kept[e] : 0;
-    count[j] = (float)c, n += c;
-  }
+  for (int j = 0; j < V; ++j) whole[j] = in_row * V + j < a.experts ? a.kept[in_row * V + j] : 0, n += whole[j];
   n = over_row<L>(n, Sum());
+#pragma unroll
+  for (int j = 0; j < V; ++j) count[j] = (float)(whole[j] - n / a.experts);
   const double tokens = a.kept[a.experts];
   const float factor = n > 0 && tokens > 0 ? (float)((double)*a.dloss * a.experts / (n * tokens)) : 0.0f;
   for (; t0 < a.tokens; t0 += step) {
