@@ -46,3 +46,27 @@ def test_gradient_of_loads_that_are_alike_is_zero():
         logits = logits_of(1, 300, experts, torch.float32).requires_grad_()
         loss, _ = expert_balance(logits, torch.arange(experts, dtype=torch.int32, device=DEV).repeat(300, 1))
         assert not bool(torch.autograd.grad(loss, logits)[0].any())
+
+
+@pytest.mark.parametrize("scores", ("softmax", "sigmoid"))
+@pytest.mark.parametrize("t,experts,dtype", (
+    (1, 8, torch.float32), (37, 60, torch.float32), (255, 64, torch.bfloat16), (2047, 8, torch.float32), (2049, 8, torch.float16), (16385, 3, torch.float32),
+    (9000, 128, torch.bfloat16), (20000, 60, torch.float32), (40000, 8, torch.float16), (65537, 128, torch.float32), (65536, 256, torch.bfloat16),
+    (5000, 1024, torch.float32), (70001, 17, torch.bfloat16)))
+def test_every_row_counts_once(t, experts, dtype, scores):
+    """Each row has one expert that is not masked, whose share is 1: the sums over tokens are whole numbers, and the loss is the nearest FP32
+    number to a quotient of whole numbers but for FP64's errors. Rows differ in what they add, the least of them 2^-20 of the whole and more
+    (a seventh of the mean of up to 70001 rows), so that one that is lost, or counts for another, shows."""
+    g = gen(t + experts)
+    mine = torch.randint(0, experts, (t,), generator=g, device=DEV)
+    logits = torch.full((t, experts), NONE, device=DEV)
+    logits[torch.arange(t, device=DEV), mine] = 4 * torch.randn(t, generator=g, device=DEV)
+    padded = torch.rand(t, generator=g, device=DEV) < (0.1 if t > 30 else 0.0)
+    logits[padded] = NONE
+    load = torch.randint(1, 8, (experts,), generator=g, device=DEV)  # pairs of an expert
+    ids = torch.repeat_interleave(torch.arange(experts, device=DEV), load)
+    ids = torch.nn.functional.pad(ids, (0, -ids.numel() % t), value=-1).view(-1, t).t().contiguous().int()
+    loss, counts = expert_balance(logits.to(dtype), ids, scores=scores)
+    assert torch.equal(counts.long(), load)
+    want = experts * float(load[mine[~padded]].sum()) / (float(load.sum()) * float((~padded).sum()))
+    assert abs(float(loss) - want) <= want * 2.0 ** -23
