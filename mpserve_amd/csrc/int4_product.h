@@ -147,13 +147,13 @@ __device__ inline void read_window(const Int4Args &a, const uint8_t *row, int32_
 }
 
 // Few rows (int4_rows.hip): x is 16-bit rows of whole 16-byte pieces.
-Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus);
+Prediction predict_int4_rows(const Int4Args &a, int32_t cus);
 void launch_int4_rows(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
 
 // Many rows (int4_tile.hip): x is 16-bit rows of whole blocks at 16-byte addresses, with its sums over spans of a group or, of a larger
 // one, 128 columns. A sum is three BF16 numbers, the first eight bits (and sign), the next eight and the rest. A row has first, second, third and
 // first again of each span; then the second ones by themselves; zeros past the last span, to a multiple of 16.
-Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus);
+Prediction predict_int4_tiles(const Int4Args &a, int32_t cus);
 void launch_int4_tiles(const Int4Args &a, int32_t x_type, int choice, hipStream_t stream);
 inline int32_t sums_shift(const Int4Args &a) { return a.shift < 2 ? a.shift : 2; }
 inline int32_t sums_spans(const Int4Args &a) { return (int32_t)(((int64_t)a.row_blocks + (1 << sums_shift(a)) - 1) >> sums_shift(a)); }

@@ -105,7 +105,7 @@ Way way_of(const mps_int4_product *p) {
   a.groups = (int32_t)((p->k + p->group - 1) / p->group);
   while ((int64_t)32 << a.shift < p->group) ++a.shift;
   const int32_t cus = compute_units();
-  const Prediction rows = predict_int4_rows(a, p->x_type, cus), tiles = predict_int4_tiles(a, p->x_type, cus);
+  const Prediction rows = predict_int4_rows(a, cus), tiles = predict_int4_tiles(a, cus);
   w.tiles = tiles.choice >= 0 && (rows.choice < 0 || tiles.us < rows.us);
   w.choice = w.tiles ? tiles.choice : rows.choice;
   w.packed = p->k > 0 && !(w.tiles ? block_rows(p->x, p->x_stride, p->k) : piece_rows(p->x, p->x_stride, p->k));

@@ -284,7 +284,7 @@ void launch_type(const Int4Args &a, int choice, hipStream_t stream) {
 
 }  // namespace
 
-Prediction predict_int4_rows(const Int4Args &a, int32_t x_type, int32_t cus) {
+Prediction predict_int4_rows(const Int4Args &a, int32_t cus) {
   Prediction best = {-1, 0};
   const int64_t periods = (a.row_blocks + 15) / 16;
   int i = 0;

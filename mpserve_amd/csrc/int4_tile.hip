@@ -518,7 +518,7 @@ void launch_type(const Int4Args &a, int choice, hipStream_t stream) {
 
 }  // namespace
 
-Prediction predict_int4_tiles(const Int4Args &a, int32_t x_type, int32_t cus) {
+Prediction predict_int4_tiles(const Int4Args &a, int32_t cus) {
   Prediction best = {-1, 0};
   int i = 0;
   for (const Choice &c : kChoices) {
