@@ -3,7 +3,7 @@
 // Both q and q - z are exact in 16 bits, so that matrix instructions multiply them by x exactly; a group's sum gets its scale in
 // FP32, and the sum of the groups is rounded once, to the output's type. Few rows are bound by the weights' bytes and go to the
 // kernel that streams them, many by the matrix cores and go to tiles; the one with the smaller predicted time is taken (4096 -> 14336,
-// groups of 128, microseconds: 32 rows 14.6 and 31; 48 rows 14336 -> 4096 23 and 90; 4096 rows 1155 and 473).
+// groups of 128, microseconds: 32 rows 14.6 and 31; 48 rows 14336 -> 4096 23 and 90; 4096 rows 1155 and, by the card, 470 to 510).
 #include "int4_product.h"
 
 namespace mps {

@@ -235,9 +235,11 @@ __device__ inline Chosen choose(int32_t (&key)[V], int32_t top, int32_t *mine, A
   return {i, (bool)__all(sure)};
 }
 
-// kBias: keys are scores and a bias. In FP32 they are off by less than 2^-19 of the row's largest score (exponentials 2^-22, their sum over
-// lanes and a lane's experts 2^-20) and 2^-24 of themselves, by the sum with the bias; where two that follow each other are not 2^-17 and
-// 2^-22 of these apart, those chosen and all that are near the last of them are put in order by keys in FP64. In a row whose
+// kBias: keys are scores and a bias. In FP32 they are off by less than 37 u of the row's largest score, u = 2^-24, and u of themselves, by the
+// sum with the bias. For the largest shape, 16 experts a lane and 64 lanes: a softmax's sum 15 + 6 additions, its exponentials 4 u and their
+// arguments' rounding |x| u, at most 4.5 u of the sum for up to 1024 terms exp(x); a score's own exponential 4 u; the reciprocal 2 u and
+// the product u. (Sigmoids: 7 u of 1.) Two keys are off by less than 74 u: where two that follow each other are not 2^-17, 128 u, and 2^-22 of
+// themselves apart, those chosen and all that are near the last of them are put in order by keys in FP64. In a row whose
 // experts are all alike (a router that starts from zeros) the order is that of FP32, ties. (All keys in FP64: 8192 x 256 15.3 us, 12.9 us so.)
 template <int T, int L, int V, bool kSigmoid, bool kBias>
 __global__ __launch_bounds__(kRouteThreads) void expert_route_kernel(RouteArgs a) {
@@ -636,7 +638,8 @@ __global__ __launch_bounds__(kRouteThreads) void expert_balance_grad_kernel(Bala
   }
 }
 
-// Workgroups of the first launch: one up to 64 rows of waves' rows, else as many as leave the second launch little to add up.
+// Workgroups of the first launch: one for up to 16384 logits and ids, which then makes the loss too; else one for every 16384, up to 256
+// and, lest the second launch has much to add up, up to 32768 experts' sums.
 int32_t balance_blocks(int64_t tokens, int64_t experts, int64_t pairs) {
   const int64_t work = tokens * experts + pairs;
   if (work <= 16384) return 1;

@@ -3,9 +3,10 @@
 A weight ``[n, k]`` is ``scales * (q - zeros)``: ``q`` whole numbers from 0 to 15, ``scales [n,
 ceil(k / group)]`` in BF16 or FP16, ``zeros`` of the same shape from 0 to 16 in uint8 (their low
 five bits count), or None where all are 8. ``group`` is a power of two, at least 32; one that is not below
-``k`` means a scale a row. This is what an AWQ checkpoint holds, and what the AWQ decode ops
-(``huffman_decode_awq_int4_bucket`` and its kin) rebuild BF16 weights from: the same whole
-numbers serve here without that step.
+``k`` means a scale a row. This is what an AWQ checkpoint holds. The AWQ builders and decode ops
+(``huffman_decode_awq_int4_bucket`` and its kin) take such whole numbers and scales too, but what they give back is the BF16
+weight that was quantised, bit by bit. The products here are with the quantised weight itself, about half a scale or less
+away from that: results are those of an AWQ model, not of the model that it was made of.
 
 * :func:`int4_pack` — whole numbers ``[..., k]`` to codes, once a weight;
 * :func:`int4_from_awq` — an AWQ checkpoint's tensors to codes, scales and zeros;
@@ -40,7 +41,7 @@ class Int4Weight(NamedTuple):
 
 def int4_pack(values: torch.Tensor) -> torch.Tensor:
     """Codes ``[..., 16 * ceil(k / 32)]`` of whole numbers ``values [..., k]`` from 0 to 15 (uint8; the low four
-    bits count), such as the AWQ ops' ``int4_values``. Works on any device."""
+    bits count), such as the ``int4_values_u8`` that the AWQ ops take. Works on any device."""
     if values is None:
         raise ValueError("values must be defined")
     if values.dtype != torch.uint8:
@@ -149,7 +150,9 @@ def int4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zero
     """``x @ w.T + bias`` for ``x [..., k]`` in BF16 or FP16 and ``w [n, k]`` in int4.
 
     Whole numbers are multiplied exactly; each group's FP32 sum gets its scale in FP32, and the sum of all is
-    rounded once, to ``out_dtype`` (default: the type of ``x``). ``bias [n]`` is BF16, FP16 or FP32."""
+    rounded once, to ``out_dtype`` (default: the type of ``x``). ``bias [n]`` is BF16, FP16 or FP32. Sums are ``x`` times
+    ``q`` less ``x`` times the zeros, taken apart for up to 512 columns at a time: FP32's errors are of these columns' sums of ``|x| (q + zeros)``,
+    and of the result."""
     _check_cuda(x, "x")
     if x.dtype not in _HALVES:
         raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
