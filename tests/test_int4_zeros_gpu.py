@@ -93,35 +93,60 @@ def spans_in_three_pieces(g, t, k, span, dtype):
     return torch.cat([first, v.float()], dim=1).view(t, k).to(dtype)
 
 
-@pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("stype", HALVES)
-@pytest.mark.parametrize("span", (32, 64, 128))
-@pytest.mark.parametrize("spans", (1, 4, 21))
-def test_every_piece_of_the_sums_and_of_scales_and_zeros_counts(spans, span, stype, dtype):
+def weight_in_two_pieces(g, shape, spans, span, stype):
+    """Whole numbers, scales and zeros [*shape, spans] of which s z has more than eight bits."""
+    values = torch.randint(0, 16, (*shape, spans * span), generator=g, device=DEV, dtype=torch.uint8)
+    zeros = torch.tensor([5, 8, 13, 15], device=DEV, dtype=torch.uint8)[torch.randint(0, 4, (*shape, spans), generator=g, device=DEV)]
+    scales = (257 / 256 if stype == torch.float16 else 129 / 128) * torch.exp2(torch.randint(-1, 2, (*shape, 1), generator=g, device=DEV).float())
+    return values, scales.expand(*shape, spans).to(stype).contiguous(), zeros
+
+
+def all_pieces_count(got, x, values, scales, zeros, span):
     """A sum's third piece is 2^-17.6 of it, the product of its second and of what eight bits leave of s z up to 2^-17. Each span adds at most
     six numbers that are not zero to a result (five of what the zeros take away, and s sum x q, which is exact), each off by a step of the
     largest sum on the way, of all spans before and four spans' part: the bound is 6 2^-23 of that, a span, below the 2^-17.6 of a
     span's part that a lost piece is, for one span and for four."""
-    t, n, k, g = 2500, 2060, spans * span, gen(spans + span)
-    x = spans_in_three_pieces(g, t, k, span, dtype)
-    values = torch.randint(0, 16, (n, k), generator=g, device=DEV, dtype=torch.uint8)
-    pick = torch.tensor([5, 8, 13, 15], device=DEV, dtype=torch.uint8)
-    zeros = pick[torch.randint(0, 4, (n, spans), generator=g, device=DEV)]
-    scales = (257 / 256 if stype == torch.float16 else 129 / 128) * torch.exp2(torch.randint(-1, 2, (n, 1), generator=g, device=DEV).float()).expand(n, spans)
-    scales = scales.to(stype).contiguous()
-    codes = int4_pack(values)
-    assert takes_tiles(x, codes, scales, zeros, span)
-    got = int4_linear(x, codes, scales, zeros, group=span, out_dtype=torch.float32).double()
+    spans = scales.shape[-1]
     w = plain.weight(values, scales, zeros, span)
-    prefix, most = torch.zeros(t, n, dtype=torch.float64, device=DEV), torch.zeros(t, n, dtype=torch.float64, device=DEV)
+    prefix = torch.zeros_like(got, dtype=torch.float64)
+    most = prefix.clone()
     part = (scales.double() * zeros.double()) * float(x[0, :span].double().sum())  # [n, spans]: the same in all rows
     for at in range(spans):
         prefix += x[:, at * span:(at + 1) * span].double() @ w[:, at * span:(at + 1) * span].T
         most = torch.maximum(most, prefix.abs())
     four = torch.stack([part[:, at:at + 4].sum(dim=1) for at in range(0, spans, 4)]).amax(dim=0)
-    off = (got - prefix).abs()
+    off = (got.double() - prefix).abs()
     bound = 6 * spans * 2.0 ** -23 * (most + four)
     assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("stype", HALVES)
+@pytest.mark.parametrize("span", (32, 64, 128))
+@pytest.mark.parametrize("spans", (1, 4, 21))
+def test_every_piece_of_the_sums_and_of_scales_and_zeros_counts(spans, span, stype, dtype):
+    t, n, g = 2500, 2060, gen(spans + span)
+    x = spans_in_three_pieces(g, t, spans * span, span, dtype)
+    values, scales, zeros = weight_in_two_pieces(g, (n,), spans, span, stype)
+    codes = int4_pack(values)
+    assert takes_tiles(x, codes, scales, zeros, span)
+    all_pieces_count(int4_linear(x, codes, scales, zeros, group=span, out_dtype=torch.float32), x, values, scales, zeros, span)
+
+
+@pytest.mark.parametrize("gather", (True, False))
+@pytest.mark.parametrize("span", (32, 64, 128))
+@pytest.mark.parametrize("spans", (1, 4))
+def test_every_piece_counts_for_experts(spans, span, gather):
+    t, n, experts, top, g = 2500, 2060, 3, 2, gen(spans + span)
+    x = spans_in_three_pieces(g, t, spans * span, span, torch.float16)
+    values, scales, zeros = weight_in_two_pieces(g, (experts, n), spans, span, torch.float16)
+    sort = expert_sort(routing(t, t, top, experts, 0.1), experts)
+    y = int4_expert_linear(x if gather else expert_gather(x, sort), int4_pack(values), scales, sort, zeros, group=span, gather=gather,
+                           out_dtype=torch.float32)
+    offsets, order = sort.offsets.tolist(), sort.order.long()
+    for e in range(experts):
+        a, b = offsets[e], offsets[e + 1]
+        all_pieces_count(y[a:b], x[order[a:b] // top], values[e], scales[e], zeros[e], span)
 
 
 @pytest.mark.parametrize("group", (32, 64, 128, 1024))
