@@ -81,7 +81,7 @@ def test_sums_of_experts_are_no_larger_than_they_need_be(t, group, gather):
 def spans_in_three_pieces(g, t, k, span, dtype):
     """x [t, k] whose sums over spans are 2^a (1.5 + 2^-8 + 2^-17): in eight bits each, none of a sum's first, second and third piece is zero.
     1/64 once, and whole numbers from 64 to 127, which any of the types hold."""
-    spans, total = k // span, (3072 + 8) * span // 32
+    spans, total = k // span, 3080 * span // 32
     v = torch.full((t * spans, span - 1), total // (span - 1), device=DEV)
     v[:, :total - int(v[0].sum())] += 1
     for col in range(0, span - 2, 2):  # neighbours apart by chance, their sum kept
